@@ -409,6 +409,106 @@ int megakernel_op_lmhead_argmax_noalloc(const void* w, long long copy_bytes, int
 /* Device time of this thread's last megakernel_op_* call (ms). */
 float megakernel_op_last_ms(void);
 
+/* ---- operators of a paged 8-bit KV cache ---------------------------------
+ * What a server keeps next to the model: a pool of blocks that sequences
+ * share, each sequence's block table, and the operators that take one layer
+ * from its QKV rows to its attention output.  The reference has one
+ * contiguous bf16 cache (src/kv_cache.cuh:11-32) and these steps only inside
+ * its kernel (src/attention.cuh); a pool, its codes and its tables are
+ * additive.
+ *
+ * All pointers inside the structs are device pointers, owned by the caller;
+ * the structs themselves are host memory, read during the call.  Calls check
+ * their arguments on the host, then only enqueue on `stream` (a hipStream_t,
+ * NULL for the null stream) on the current device, which must be the
+ * stream's: no allocation, no copy, no wait, so they may be captured into a
+ * graph.  A captured call reads lengths and tables anew at every replay; only
+ * the sizes in the structs are fixed.  They return 0, or -1 with
+ * megakernel_last_error() set; megakernel_op_last_ms() does not cover them. */
+
+#define MK_TYPE_F32 0
+#define MK_TYPE_BF16 1
+
+/* Rows of heads: element d of head h of token t at p[t * token_stride +
+ * h * head_stride + d], strides in elements.  Rows start at multiples of 16
+ * bytes.  Rows that are written may not overlap. */
+typedef struct {
+  void* p;
+  long long token_stride, head_stride;
+  int type; /* MK_TYPE_* */
+} megakernel_rows;
+
+/* A pool of n_blocks blocks of `block` positions (16, 32, 64 or 128):
+ *   k        e4m3 codes [n_blocks][n_kv][block][head_dim]
+ *   v        e4m3 codes [n_blocks][n_kv][head_dim][block]
+ *   k_scale, v_scale  fp32 [n_blocks][n_kv], powers of two
+ * value = code * scale.  head_dim 64 or 128.  Codes and scales of a block
+ * need no initial value. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int n_blocks, block, n_kv, head_dim;
+} megakernel_kv8_cache;
+
+/* Rows of n_seq sequences: sequence i has rows q_start[i] .. q_start[i+1] - 1
+ * (q_start[n_seq + 1] ascending, within [0, n_tokens]), which are its last
+ * positions: row q_start[i+1] - 1 is position kv_len[i] - 1.  Its position p
+ * lies in block table[i * table_width + p / block] at row p % block; entries
+ * outside [0, n_blocks) are missing blocks, as are positions past the table.
+ * n_tokens: rows of the row tensors.  max_kv: no bound, only how long
+ * contexts are expected to get (0: table_width * block), from which the
+ * attention chooses how far it splits them. */
+typedef struct {
+  const int* table;
+  const int* q_start;
+  const int* kv_len;
+  int n_seq, table_width, n_tokens, max_kv;
+} megakernel_kv8_batch;
+
+/* RMSNorm of every head of q and k with its gain (bf16 [head_dim]), then the
+ * rotate-half rotation by pos[t] * inv_freq[i] (fp32 [head_dim / 2]; the
+ * product is formed exactly).  n_q heads of q, n_kv of k; q and k have one
+ * type, q_out and k_out one type, bf16 or fp32; an output may be its own
+ * input.  The arithmetic is fp32, rounded once. */
+int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* k, const void* q_gain,
+                               const void* k_gain, const float* inv_freq, const int* pos, const megakernel_rows* q_out,
+                               const megakernel_rows* k_out, int n_tokens, int n_q, int n_kv, int head_dim, float eps,
+                               void* stream);
+
+/* Quantise rows of K and V (n_kv heads, bf16 or fp32, one type) into their
+ * blocks.  Per block, head and K / V: the scale is the smallest power of two
+ * s >= 2^-126 with |x| <= 448 s for the new rows, or the block's own scale
+ * where it is larger and older rows are in the block; codes are x / s rounded
+ * to nearest even.  Where the scale grows, the older rows' codes are rounded
+ * again from their values.  Infinities do not count for the scale and become
+ * +-448 s; NaN stays NaN.  Rows whose block is missing or whose position is
+ * negative are dropped.  Other rows of a block are left as they were.  Rows
+ * given to one block by two sequences of a call are a race; blocks that
+ * nothing is appended to may be shared. */
+int megakernel_op_kv8_append(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                             const megakernel_rows* k, const megakernel_rows* v, void* stream);
+
+/* The values of rows that the cache holds (bf16 or fp32; exact in both, down
+ * to their smallest normal number).  Rows whose block is missing or whose
+ * position is negative are zeros; rows of no sequence are left alone. */
+int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                           const megakernel_rows* k_out, const megakernel_rows* v_out, void* stream);
+
+/* Causal attention of each sequence's rows over its blocks: row at position
+ * p sees positions 0 .. p, without those whose block is missing;
+ * out = sum_j softmax_j(scale * q . k_j) v_j, zeros for a row that sees
+ * nothing.  Query head h reads KV head h / (n_q / n_kv).  q and out bf16; the
+ * scores, the softmax and the sums are fp32, the weights are rounded to bf16
+ * for the product with V.  workspace: megakernel_op_kv8_workspace_bytes(...)
+ * bytes (NULL where that is 0), 16-byte aligned, without an initial value;
+ * calls that may overlap in time need one each. */
+long long megakernel_op_kv8_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, int n_q);
+int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                const megakernel_rows* q, const megakernel_rows* out, int n_q, float scale,
+                                void* workspace, long long workspace_bytes, void* stream);
+
 /* Self-test of the hand-off primitive that replaces the reference's grid
  * barrier (src/barriers.cuh:38-73): one workgroup per CU runs `rounds`
  * all-gather rounds of tagged words (full tags and 4-bit packed pairs,

@@ -88,6 +88,14 @@ SIGNATURES = {
     "megakernel_op_lmhead_argmax_noalloc": (c_int, [c_void_p, c_ll, c_int, c_int, c_int, c_void_p, c_int,
                                                     c_void_p, c_void_p, c_int, c_int]),
     "megakernel_op_last_ms": (c_float, []),
+    # paged 8-bit KV cache (the structs of megakernel.h by address)
+    "megakernel_op_qk_norm_rope": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                           c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p]),
+    "megakernel_op_kv8_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "megakernel_op_kv8_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "megakernel_op_kv8_workspace_bytes": (c_ll, [c_void_p, c_void_p, c_int]),
+    "megakernel_op_kv8_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_ll,
+                                            c_void_p]),
     # self-test
     "megakernel_selftest_dataflow": (c_int, [c_int, P_int, P_float]),
 }

@@ -1,0 +1,246 @@
+"""Operators of a paged 8-bit KV cache over the library's
+``megakernel_op_qk_norm_rope`` and ``megakernel_op_kv8_*`` entry points.
+
+What a server keeps next to the model: a pool of blocks that sequences share
+(:class:`Cache`), the sequences' block tables and lengths (:class:`Batch`),
+and the operators that take one layer from its QKV rows to its attention
+output: :func:`qk_norm_rope`, :func:`append`, :func:`attention`; :func:`read`
+gives rows of the cache back.  The reference has one contiguous bf16 cache
+(/root/reference/src/kv_cache.cuh:11-32) and these steps only inside its
+kernel (/root/reference/src/attention.cuh).
+
+Tensors are torch tensors on one GPU and belong to the caller, outputs
+included; nothing is copied, and no call waits.  Work is enqueued on torch's
+current stream of that GPU, so tensors that another stream wrote need that
+stream waited for, as with torch's own operators.  Calls can be captured into
+a graph: a replay reads lengths and tables anew, while sizes stay fixed.
+
+    cache = kv8.Cache(k, v, k_scale, v_scale)      # or kv8.Cache.empty(...)
+    batch = kv8.Batch(table, q_start, kv_len, n_tokens)
+    kv8.qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q, k)
+    kv8.append(cache, batch, k, v)
+    kv8.attention(cache, batch, q, out)
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}  # MK_TYPE_F32, MK_TYPE_BF16
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong),
+                ("type", ctypes.c_int)]
+
+
+class _CCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_blocks", ctypes.c_int), ("block", ctypes.c_int),
+                ("n_kv", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class _CBatch(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("n_seq", ctypes.c_int), ("table_width", ctypes.c_int), ("n_tokens", ctypes.c_int),
+                ("max_kv", ctypes.c_int)]
+
+
+def _whole(t, dtype, shape, name: str):
+    """A contiguous GPU tensor of one type; None in `shape` is any size."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on the GPU, not on {t.device}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple('any' if n is None else n for n in shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _same_gpu(device, **tensors):
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _rows(t, tokens: int, heads: int, dim: int, device, name: str) -> _Rows:
+    """Rows [tokens][heads][dim] with any token and head stride."""
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{name} must be bfloat16 or float32, not {t.dtype}")
+    if t.shape != (tokens, heads, dim):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(tokens, heads, dim)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    st, sh, sd = t.stride()
+    if sd != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous (stride {sd})")
+    return _Rows(t.data_ptr(), st if tokens > 1 else 0, sh if heads > 1 else 0, _TYPES[t.dtype])
+
+
+def _call(fn, device, *args):
+    """Enqueue on the current stream of `device`; raises what the library reports."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        lib = _lib.load()
+        _lib.check(lib, rc, fn.__name__.replace("megakernel_", ""))
+
+
+class Cache:
+    """A pool of blocks of one layer: e4m3 codes ``k`` [n_blocks][n_kv][block][head_dim]
+    and ``v`` [n_blocks][n_kv][head_dim][block] (uint8), and their power-of-two
+    scales [n_blocks][n_kv] (float32).  ``block`` is 16, 32, 64 or 128
+    positions, ``head_dim`` 64 or 128.  Blocks need no initial value.
+    """
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _whole(k, torch.uint8, (None, None, None, None), "k")
+        n_blocks, n_kv, block, head_dim = k.shape
+        _whole(v, torch.uint8, (n_blocks, n_kv, head_dim, block), "v")
+        _whole(k_scale, torch.float32, (n_blocks, n_kv), "k_scale")
+        _whole(v_scale, torch.float32, (n_blocks, n_kv), "v_scale")
+        _same_gpu(k.device, v=v, k_scale=k_scale, v_scale=v_scale)
+        if block not in (16, 32, 64, 128) or head_dim not in (64, 128):
+            raise ValueError(f"blocks of {block} positions (16, 32, 64 or 128), head_dim {head_dim} (64 or 128)")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_blocks, self.n_kv, self.block, self.head_dim, self.device = n_blocks, n_kv, block, head_dim, k.device
+        self._c = _CCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, block, n_kv,
+                          head_dim)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, n_blocks: int, n_kv: int, head_dim: int, block: int = 32, device="cuda") -> "Cache":
+        codes = [torch.empty(s, dtype=torch.uint8, device=device)
+                 for s in ((n_blocks, n_kv, block, head_dim), (n_blocks, n_kv, head_dim, block))]
+        return cls(*codes, *(torch.empty((n_blocks, n_kv), dtype=torch.float32, device=device) for _ in range(2)))
+
+
+class Batch:
+    """Rows of several sequences.  Sequence i has rows q_start[i] ..
+    q_start[i + 1] - 1 of the row tensors, and these are the newest of its
+    kv_len[i] positions.  ``table`` [n_seq][width] names its blocks in order;
+    entries outside the pool (-1, say) are missing blocks: attention leaves
+    their positions out, :func:`append` drops their rows, :func:`read` gives
+    zeros.  All three are int32 tensors on the GPU and are read when a call
+    runs, so they may change between calls and replays.
+
+    ``n_tokens`` is the row tensors' first size.  ``max_kv`` only says how long
+    contexts are expected to get, from which :func:`attention` chooses how far
+    to split them; longer ones are right all the same.
+    """
+
+    def __init__(self, table, q_start, kv_len, n_tokens: int, max_kv: int = 0):
+        _whole(kv_len, torch.int32, (None,), "kv_len")
+        n_seq = kv_len.shape[0]
+        _whole(table, torch.int32, (n_seq, None), "table")
+        _whole(q_start, torch.int32, (n_seq + 1,), "q_start")
+        _same_gpu(kv_len.device, table=table, q_start=q_start)
+        if n_tokens < 0 or max_kv < 0 or table.shape[1] < 1:
+            raise ValueError(f"n_tokens {n_tokens} and max_kv {max_kv} (at least 0), table width {table.shape[1]} (at least 1)")
+        self.table, self.q_start, self.kv_len = table, q_start, kv_len
+        self.n_seq, self.n_tokens, self.max_kv, self.device = n_seq, int(n_tokens), int(max_kv), kv_len.device
+        # of no sequence there are no addresses to hand over, and nothing to do
+        self._c = _CBatch(table.data_ptr() or 16, q_start.data_ptr(), kv_len.data_ptr() or 16, n_seq, table.shape[1],
+                          self.n_tokens, self.max_kv)
+        self._ref = ctypes.byref(self._c)
+        self._need: dict[tuple, int] = {}
+
+
+def qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q_out, k_out, eps: float = 1e-6):
+    """RMSNorm of every head of q [T][n_q][D] and k [T][n_kv][D] with its gain
+    (bf16 [D]), then the rotate-half rotation by ``pos[t] * inv_freq[i]``
+    (int32 [T], float32 [D/2]), into q_out and k_out.  D is 64 or 128; inputs
+    and outputs are bf16 or fp32 with any token and head strides, so the rows
+    may lie in a packed QKV tensor, and an output may be its own input."""
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q and k are [tokens][heads][head_dim], not {tuple(q.shape)} and {tuple(k.shape)}")
+    if not q.is_cuda:
+        raise ValueError(f"q must be on the GPU, not on {q.device}")
+    tokens, n_q, dim = q.shape
+    n_kv, device = k.shape[1], q.device
+    _whole(q_gain, torch.bfloat16, (dim,), "q_gain")
+    _whole(k_gain, torch.bfloat16, (dim,), "k_gain")
+    _whole(inv_freq, torch.float32, (dim // 2,), "inv_freq")
+    _whole(pos, torch.int32, (tokens,), "pos")
+    _same_gpu(device, q_gain=q_gain, k_gain=k_gain, inv_freq=inv_freq, pos=pos)
+    rows = [_rows(t, tokens, h, dim, device, name) for t, h, name in
+            ((q, n_q, "q"), (k, n_kv, "k"), (q_out, n_q, "q_out"), (k_out, n_kv, "k_out"))]
+    if tokens == 0:
+        return
+    a, b, c, d = (ctypes.byref(r) for r in rows)
+    _call(_lib.load().megakernel_op_qk_norm_rope, device, a, b, q_gain.data_ptr(), k_gain.data_ptr(),
+          inv_freq.data_ptr(), pos.data_ptr(), c, d, tokens, n_q, n_kv, dim, eps)
+
+
+def _pair(cache: Cache, batch: Batch, k, v, names):
+    _same_gpu(cache.device, batch=batch)
+    r = [_rows(t, batch.n_tokens, cache.n_kv, cache.head_dim, cache.device, n) for t, n in zip((k, v), names)]
+    return ctypes.byref(r[0]), ctypes.byref(r[1])
+
+
+def append(cache: Cache, batch: Batch, k, v):
+    """Quantise rows k, v [n_tokens][n_kv][head_dim] (bf16 or fp32) into their
+    blocks.  A block and head has one scale, the smallest power of two that
+    fits its rows into e4m3; rows that a block already holds are rounded again
+    where a new row makes its scale grow.  Two sequences of one call may not
+    append to the same block."""
+    a, b = _pair(cache, batch, k, v, ("k", "v"))
+    if batch.n_seq and batch.n_tokens:
+        _call(_lib.load().megakernel_op_kv8_append, cache.device, cache._ref, batch._ref, a, b)
+
+
+def read(cache: Cache, batch: Batch, k_out, v_out):
+    """The values of the batch's rows into k_out, v_out [n_tokens][n_kv][head_dim]
+    (bf16 or fp32, exact in both).  ``q_start`` of a batch whose rows are whole
+    contexts is their lengths' running sum."""
+    a, b = _pair(cache, batch, k_out, v_out, ("k_out", "v_out"))
+    if batch.n_seq and batch.n_tokens:
+        _call(_lib.load().megakernel_op_kv8_read, cache.device, cache._ref, batch._ref, a, b)
+
+
+def workspace_bytes(cache: Cache, batch: Batch, n_q: int) -> int:
+    """Bytes of :func:`attention`'s workspace for these sizes (0: none)."""
+    key = (cache.n_kv, cache.head_dim, cache.block, n_q)
+    need = batch._need.get(key)
+    if need is None:
+        lib = _lib.load()
+        need = _lib.check(lib, lib.megakernel_op_kv8_workspace_bytes(cache._ref, batch._ref, n_q), "op_kv8_workspace_bytes")
+        batch._need[key] = need
+    return need
+
+
+def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, workspace=None):
+    """Causal attention of q [n_tokens][n_q][head_dim] (bf16) over the cache
+    into out: each row sees its sequence's positions up to its own, its own
+    among them.  Query head h reads KV head h / (n_q / n_kv); rows that see
+    nothing are zeros.  ``scale`` is 1 / sqrt(head_dim) unless given.
+    ``workspace`` is a uint8 tensor of :func:`workspace_bytes`, one for each
+    call that may run at the same time; without one, a call takes its own from
+    torch's allocator."""
+    if q.dim() != 3:
+        raise ValueError(f"q is [tokens][heads][head_dim], not {tuple(q.shape)}")
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise ValueError(f"q and out must be bfloat16, not {q.dtype} and {out.dtype}")
+    device, n_q = cache.device, q.shape[1]
+    _same_gpu(device, batch=batch)
+    a = _rows(q, batch.n_tokens, n_q, cache.head_dim, device, "q")
+    b = _rows(out, batch.n_tokens, n_q, cache.head_dim, device, "out")
+    need = workspace_bytes(cache, batch, n_q)
+    if not batch.n_seq or not batch.n_tokens:
+        return
+    if workspace is None:
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    else:
+        _whole(workspace, torch.uint8, (None,), "workspace")
+        _same_gpu(device, workspace=workspace)
+    _call(_lib.load().megakernel_op_kv8_attention, device, cache._ref, batch._ref, ctypes.byref(a), ctypes.byref(b), n_q,
+          cache.head_dim ** -0.5 if scale is None else scale, workspace.data_ptr() if workspace is not None else None,
+          workspace.numel() if workspace is not None else 0)
