@@ -15,8 +15,6 @@
 namespace mk {
 namespace kv8 {
 
-constexpr int kMaxSplits = 128;
-
 static bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 static int type_size(int type) { return type == MK_TYPE_F32 ? 4 : type == MK_TYPE_BF16 ? 2 : 0; }
@@ -137,23 +135,81 @@ static long long block_items(const megakernel_kv8_batch* b, int block) {
   return n < m ? n : m;
 }
 // Most tiles of `rows` query rows.
-static long long row_tiles(const megakernel_kv8_batch* b, int group, int rows) {
+static long long most_row_tiles(const megakernel_kv8_batch* b, int group, int rows) {
   const long long n = b->n_tokens, m = n * group / rows + b->n_seq, each = n * ((group + rows - 1) / rows);
   return each < m ? each : m;
 }
 
-static int max_splits(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q) {
-  const long long wg = row_tiles(b, n_q / c->n_kv, ROWS) * c->n_kv;
-  if (wg < 1) return 1;
-  const long long kv = b->max_kv ? b->max_kv : (long long)b->table_width * c->block;
-  const long long tiles = (kv + TILE - 1) / TILE, want = (1024 + wg - 1) / wg, can = (tiles + 3) / 4;
-  const long long s = want < can ? want : can;
-  return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+// How the attention of a batch is launched.
+struct Plan {
+  bool use[2];                   // attn_rows, attn_tile
+  int few;                       // as in Attn
+  int waves;                     // of attn_rows's workgroups
+  int lr[2], target[2], least[2];
+  long long items[2], slots[2];  // most items, and partials, per KV head
+};
+
+// Lengths are on the device, so what is chosen here goes by the sizes that
+// the host has: rows, sequences, and how long contexts may get (max_kv).
+// Every choice is right for any lengths.
+static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q) {
+  Plan p{};
+  const int group = n_q / c->n_kv;
+  const bool d64 = c->head_dim == 64;
+  const long long rows = (long long)b->n_tokens * group;
+  const long long kv = b->max_kv ? b->max_kv : (long long)b->table_width * c->block, steps = (kv + TILE - 1) / TILE;
+  // Which kernel takes a sequence.  attn_rows reads a context once for every
+  // 16 rows but starts fast; attn_tile has the rate for large products and
+  // takes 15 us more to get there.  Rows x steps of a KV head at which they
+  // were even, 8 heads at 2,100 and 16,000 positions: 128 Ki for head_dim 64
+  // (512 rows at 16,000: 45 / 46 us; 1,024 at 2,100: 18 / 30), 48 Ki for 128
+  // (256 rows at 16,000: 55 / 46; 512: 80 / 64; 512 at 2,100: 17 / 31).  Many
+  // sequences share the chip, so their rows count together.
+  const long long even = (d64 ? 8 << 17 : 8 * 49152) / ((long long)b->n_seq * c->n_kv * steps + 1);
+  const int few = (int)(even < 64 ? 64 : even > 1024 ? 1024 : even);
+  if (b->n_seq == 1) p.use[rows > few] = true;
+  else if (rows <= few || rows <= 32ll * b->n_seq) p.use[FEW] = true;
+  else p.use[FEW] = p.use[MANY] = true;
+  p.few = !p.use[MANY] ? 0x7fffffff : !p.use[FEW] ? 0 : few;
+  p.lr[FEW] = 4, p.lr[MANY] = 7;
+  p.least[FEW] = 8, p.least[MANY] = 4;
+  p.waves = 8;
+  if (p.use[FEW]) {
+    long long tiles = most_row_tiles(b, group, ROWS);
+    const long long most = (long long)b->n_seq * ((few + ROWS - 1) / ROWS);
+    if (p.use[MANY] && tiles > most) tiles = most;
+    // Splitting costs a second kernel and a second start (5 us), and saves
+    // steps on a CU that has neighbours idle: worth it from about 40 steps of
+    // 8 KB or 16 of 16 KB on one sequence (us unsplit / split: head_dim 64,
+    // 2,600 positions 9.8 / 9.9, 4,096 12.5 / 9.8; 128: 1,024 positions 9.7 /
+    // 12.3, 2,048 14.2 / 14.0, 4,096 23.0 / 14.0), later the more CUs are
+    // busy anyway (16 sequences of 4,096, head_dim 64: 15.5 / 19.9).  Split
+    // work goes to workgroups of four waves, two for every CU; whole contexts
+    // to eight waves (one sequence of 1,024: 7.0 us with four, 6.6 with eight).
+    const long long units = tiles * c->n_kv;
+    if (units < 256 && steps * (256 - units) > 256 * (d64 ? 40 : 16)) {
+      p.target[FEW] = (512 + c->n_kv - 1) / c->n_kv;
+      p.waves = 4;
+    }
+    p.items[FEW] = tiles + p.target[FEW];
+    p.slots[FEW] = 2ll * p.target[FEW];
+  }
+  if (p.use[MANY]) {
+    // two workgroups fit a CU: split contexts where the row tiles do not fill them
+    const long long tiles = most_row_tiles(b, group, TILE_ROWS), sure = rows / TILE_ROWS;
+    if (steps > p.least[MANY] && sure * c->n_kv < 512) p.target[MANY] = (512 + c->n_kv - 1) / c->n_kv;
+    p.items[MANY] = tiles + p.target[MANY];
+    p.slots[MANY] = 2ll * p.target[MANY];
+  }
+  return p;
 }
 
-static long long workspace(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q) {
-  const int s = max_splits(c, b, n_q);
-  return s == 1 ? 0 : (long long)b->n_tokens * n_q * s * (c->head_dim + 2) * 4;
+static long long part_floats(const Plan& p, int k, int n_kv, int head_dim) { return p.slots[k] * n_kv * head_dim << p.lr[k]; }
+static long long part_bytes(const Plan& p, int k, int n_kv, int head_dim) {
+  return part_floats(p, k, n_kv, head_dim) * 4 + (p.slots[k] * n_kv << p.lr[k]) * 8;
+}
+static long long workspace(const Plan& p, int n_kv, int head_dim) {
+  return part_bytes(p, FEW, n_kv, head_dim) + part_bytes(p, MANY, n_kv, head_dim);
 }
 
 static bool heads_ok(const char* op, int n_q, int n_kv) {
@@ -296,7 +352,7 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
 long long megakernel_op_kv8_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, int n_q) {
   const char* op = "op_kv8_workspace_bytes";
   if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !heads_ok(op, n_q, cache->n_kv)) return -1;
-  return workspace(cache, batch, n_q);
+  return workspace(plan(cache, batch, n_q), cache->n_kv, cache->head_dim);
 }
 
 int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
@@ -315,33 +371,48 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
     set_err("%s: scale=%g must be positive and finite", op, scale);
     return -1;
   }
-  const long long need = workspace(cache, batch, n_q);
+  const Plan pl = plan(cache, batch, n_q);
+  const long long need = workspace(pl, cache->n_kv, cache->head_dim);
   if (need && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < need)) {
     set_err("%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", op, need, d_workspace ? workspace_bytes : 0);
     return -1;
   }
-  const int group = n_q / cache->n_kv;
-  const long long groups = row_tiles(batch, group, ROWS) * cache->n_kv;
-  if (groups == 0) return 0;
+  if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
   Attn p;
   p.c = cache_of(cache);
   p.b = batch_of(batch);
   p.q = rows_of(q);
   p.out = rows_of(out);
   p.n_q = n_q;
-  p.group = group;
+  p.group = n_q / cache->n_kv;
   p.scale = scale * 1.4426950408889634f;
-  p.part = static_cast<float*>(d_workspace);
-  p.max_splits = max_splits(cache, batch, n_q);
-  p.min_tiles = 4;
-  if (!grid_ok(op, groups * p.max_splits)) return -1;
-  const dim3 g((unsigned)groups, (unsigned)p.max_splits);
+  p.few = pl.few;
+  char* ws = static_cast<char*>(d_workspace);
+  for (int k = 0; k < 2; ++k) {
+    Deal& d = p.d[k];
+    d.lr = pl.lr[k], d.target = pl.target[k], d.least = pl.least[k], d.items = (int)pl.items[k];
+    d.part = reinterpret_cast<float*>(ws);
+    d.ml = reinterpret_cast<float2*>(d.part + part_floats(pl, k, cache->n_kv, cache->head_dim));
+    ws += part_bytes(pl, k, cache->n_kv, cache->head_dim);
+  }
+  const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv, joins = (long long)batch->n_tokens * n_q;
+  if (!grid_ok(op, few * 2) || !grid_ok(op, many) || !grid_ok(op, joins)) return -1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->head_dim == 64) hipLaunchKernelGGL(attn_rows<64>, g, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(attn_rows<128>, g, dim3(256), 0, st, p);
-  if (p.max_splits > 1) {
-    if (cache->head_dim == 64) hipLaunchKernelGGL(attn_join<64>, dim3((unsigned)groups), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(attn_join<128>, dim3((unsigned)groups), dim3(256), 0, st, p);
+  const bool d64 = cache->head_dim == 64;
+  auto go = [&](auto kern, long long groups, int threads) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(threads), 0, st, p);
+  };
+  if (pl.use[MANY]) d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
+  if (pl.use[FEW]) {
+    if (pl.waves == 4) d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
+    else d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
+  }
+  // a workgroup for every row, or where rows are many a wave for four (verify of
+  // 1,152 rows 41.0 / 43.6 us in all, a prompt of 16,384 336 / 315)
+  if (need && joins <= 4096) d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
+  else if (need) {
+    const long long waves = (long long)batch->n_tokens * ((n_q + 3) / 4);
+    d64 ? go(attn_join_waves<64, 4>, (waves + 3) / 4, 256) : go(attn_join_waves<128, 4>, (waves + 3) / 4, 256);
   }
   return launched(op);
 }

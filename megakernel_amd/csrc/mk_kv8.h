@@ -68,31 +68,45 @@ __device__ __forceinline__ Seq seq_at(const Batch& b, int i, int lb) {
   return s;
 }
 
+// Sum over the lanes up to and with this one (DPP: no step through LDS).
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 -> 1, 2 -> 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // rows 0, 1 -> 2, 3
+  return x;
+}
+
 // Work items are dealt to the sequences in order, count(seq) each; finds the
 // sequence of item `it` and the item's number within it.  A wave looks at 64
-// sequences at a time (the whole wave must call it).  False past the last.
+// sequences at a time (the whole wave must call it), each lane at one, so a
+// workgroup waits for one round of loads.  False past the last.
 template <class Count>
 __device__ __forceinline__ bool find_item(const Batch& b, int lb, int it, Count count, Seq& s, int& within) {
   const int l = (int)(threadIdx.x & (kWave - 1u));
   int before = 0;
   for (int base = 0; base < b.n_seq; base += kWave) {
+    Seq q{};
     int c = 0;
-    if (base + l < b.n_seq) c = count(seq_at(b, base + l, lb));
-    int sum = c;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int o = __shfl_up(sum, d);
-      if (l >= d) sum += o;
+    if (base + l < b.n_seq) {
+      q = seq_at(b, base + l, lb);
+      c = count(q);
     }
+    const int sum = wave_prefix(c);
     const unsigned long long hit = __ballot(before + sum > it);
     if (hit) {
-      const int f = __ffsll((long long)hit) - 1;
-      within = it - before - (__shfl(sum, f) - __shfl(c, f));
-      s = seq_at(b, __builtin_amdgcn_readfirstlane(base + f), lb);
-      within = __builtin_amdgcn_readfirstlane(within);
+      const int f = __builtin_amdgcn_readfirstlane(__ffsll((long long)hit) - 1);
+      s.i = base + f;
+      s.row0 = __builtin_amdgcn_readlane(q.row0, f);
+      s.rows = __builtin_amdgcn_readlane(q.rows, f);
+      s.pos0 = __builtin_amdgcn_readlane(q.pos0, f);
+      s.len = __builtin_amdgcn_readlane(q.len, f);
+      within = it - before - (__builtin_amdgcn_readlane(sum, f) - __builtin_amdgcn_readlane(c, f));
       return true;
     }
-    before += __shfl(sum, kWave - 1);
+    before += __builtin_amdgcn_readlane(sum, kWave - 1);
   }
   return false;
 }
@@ -397,60 +411,242 @@ __global__ __launch_bounds__(256) void read_back(Cache c, Batch b, Rows kr, Rows
 // --------------------------------------------------------------- attention
 // Query rows of one KV head: row r of a sequence is token r / G, query head
 // r % G of the group of G that share the KV head.
+// How the work of one kernel is dealt out: row tiles of 2^lr rows, and where
+// contexts are split the steps of positions of all row tiles in about
+// `target` items per KV head, of at least `least` steps each; target 0 for no
+// splits.  Partials: outputs [slot][head][row][D] and maxima and sums
+// [slot][head][row].
+struct Deal {
+  int lr, target, least, items;
+  float* part;
+  float2* ml;
+};
+
+enum Kind : int { FEW = 0, MANY = 1 };  // attn_rows, attn_tile
+
 struct Attn {
   Cache c;
   Batch b;
   Rows q, out;
   int n_q, group;
-  float scale;      // softmax scale * log2(e)
-  float* part;      // partials of the splits (null: one split)
-  int max_splits, min_tiles;
+  float scale;  // softmax scale * log2(e)
+  int few;      // sequences of up to so many query rows are attn_rows's, the others attn_tile's
+  Deal d[2];
 };
 
-constexpr int ROWS = 16;  // query rows of a row tile (the matrix columns)
-constexpr int TILE = 64;  // positions of a step
+constexpr int ROWS = 16;        // query rows of attn_rows's tile (the matrix columns)
+constexpr int TILE_ROWS = 128;  // and of attn_tile's
+constexpr int TILE = 64;        // positions of a step
 
-// Splits of a row tile that sees `tiles` steps of positions: as many as the
-// launch has, with at least min_tiles steps in each.
-__device__ __forceinline__ int splits_for(int tiles, int max_splits, int min_tiles) {
-  return min(max((tiles + min_tiles - 1) / min_tiles, 1), max_splits);
+// Row tile rt of a sequence: its rows, and the positions [0, any) that some
+// row of it sees, [0, all) that every row sees.
+struct RowTile {
+  int n_rows, any, all;
+};
+__device__ __forceinline__ RowTile row_tile(const Seq& s, int G, int rt, int rows) {
+  const long long r0 = (long long)rt * rows, left = (long long)s.rows * G - r0;
+  RowTile t;
+  t.n_rows = (int)min(left, (long long)rows);
+  t.all = min(max(s.pos0 + (int)(r0 / G) + 1, 0), s.len);
+  t.any = min(max(s.pos0 + (int)((r0 + t.n_rows - 1) / G) + 1, 0), s.len);
+  return t;
 }
-// Floats of one row's partial: D outputs, then the maximum and the sum.
-template <int D>
-__device__ __forceinline__ float* part_at(float* part, long long row, int max_splits, int s) {
-  return part + (row * max_splits + s) * (D + 2);
+__device__ __forceinline__ int row_tiles(const Seq& s, int G, int lr) {
+  return (int)(((long long)s.rows * G + (1 << lr) - 1) >> lr);
 }
+
+// Most splits of one row tile (attn_join gives each a thread).
+constexpr int kMaxSplits = 256;
+
+// A row tile and one of the splits of its positions.
+struct Item {
+  Seq s;
+  int rt, split, ns;  // row tile, split, splits of this sequence's row tiles
+  int slot;           // of the tile's first partial, if ns > 1
+  int kind;
+};
+
+// Steps of a sequence's longest row tile.
+__device__ __forceinline__ int most_steps(const Seq& s) { return (min(max(s.pos0 + s.rows, 0), s.len) + TILE - 1) / TILE; }
+
+__device__ __forceinline__ int kind_of(const Attn& p, const Seq& s) { return (long long)s.rows * p.group > p.few; }
+
+// Lane l's sequence of the 64 from `base` on, no rows past the last.
+__device__ __forceinline__ Seq lane_seq(const Attn& p, int base) {
+  const int i = base + (int)(threadIdx.x & (kWave - 1u));
+  return i < p.b.n_seq ? seq_at(p.b, i, p.c.lb) : Seq{};
+}
+
+// Steps of an item: the target-th part of all steps of the kernel's row tiles.
+// `first` holds the first 64 sequences.
+__device__ __forceinline__ int steps_per_item(const Attn& p, int kind, const Seq& first) {
+  const Deal& d = p.d[kind];
+  if (!d.target) return 0x7fffffff;
+  long long total = 0;
+  for (int base = 0; base < p.b.n_seq; base += kWave) {
+    const Seq q = base ? lane_seq(p, base) : first;
+    const long long w = kind_of(p, q) == kind ? (long long)row_tiles(q, p.group, d.lr) * most_steps(q) : 0;
+    // 64 lanes' sum in two halves that stay inside 32 bits
+    const int lo = wave_prefix((int)(w & 0xffffff)), hi = wave_prefix((int)min(w >> 24, 0x1ffffffll));
+    total += ((long long)__builtin_amdgcn_readlane(hi, 63) << 24) + __builtin_amdgcn_readlane(lo, 63);
+  }
+  return (int)min(max((total + d.target - 1) / d.target, (long long)d.least), 0x7fffffffll);
+}
+
+// Where sequences are of unlike length, equal splits of each would leave most
+// of the chip waiting for the longest.  Every workgroup therefore adds up the
+// steps of all sequences (their lengths are on the device alone), takes the
+// `target`-th part of that as the steps of an item, and deals the items out:
+// a sequence of k row tiles and n steps gets k * ceil(n / part) of them.
+// There are at most target + (row tiles) items, and 2 * target partials: a
+// sequence that is split at all has more than one part.
+// Finds item `it` of a kernel, or with kind -1 the item that holds row `it`
+// of all sequences' rows (r.rt is then the row's token within its sequence).
+template <int KIND>
+__device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
+  const int G = p.group;
+  const Seq first = lane_seq(p, 0);
+  const int per0 = KIND != MANY ? steps_per_item(p, FEW, first) : 0, per1 = KIND != FEW ? steps_per_item(p, MANY, first) : 0;
+  int before = 0, slots0 = 0, slots1 = 0;
+  for (int base = 0; base < p.b.n_seq; base += kWave) {
+    const Seq q = base ? lane_seq(p, base) : first;
+    const int kind = kind_of(p, q);
+    int c = 0, s0 = 0, s1 = 0, ns = 1;
+    if (KIND < 0 || kind == KIND) {
+      const int per = kind ? per1 : per0;
+      const int rt = row_tiles(q, G, kind ? p.d[1].lr : p.d[0].lr), n = most_steps(q);
+      ns = min(max(n / per + (n % per != 0), 1), kMaxSplits);
+      const int sl = ns > 1 ? rt * ns : 0;
+      s0 = kind ? 0 : sl;
+      s1 = kind ? sl : 0;
+      c = KIND < 0 ? q.rows : rt * ns;
+    }
+    const int sum = wave_prefix(c), sum0 = KIND != MANY ? wave_prefix(s0) : 0, sum1 = KIND != FEW ? wave_prefix(s1) : 0;
+    const unsigned long long hit = __ballot(before + sum > it);
+    if (hit) {
+      const int f = __builtin_amdgcn_readfirstlane(__ffsll((long long)hit) - 1);
+      r.s.i = base + f;
+      r.s.row0 = __builtin_amdgcn_readlane(q.row0, f);
+      r.s.rows = __builtin_amdgcn_readlane(q.rows, f);
+      r.s.pos0 = __builtin_amdgcn_readlane(q.pos0, f);
+      r.s.len = __builtin_amdgcn_readlane(q.len, f);
+      r.ns = __builtin_amdgcn_readlane(ns, f);
+      r.kind = __builtin_amdgcn_readlane(kind, f);
+      const int within = it - before - (__builtin_amdgcn_readlane(sum, f) - __builtin_amdgcn_readlane(c, f));
+      r.slot = r.kind ? slots1 + __builtin_amdgcn_readlane(sum1 - s1, f) : slots0 + __builtin_amdgcn_readlane(sum0 - s0, f);
+      if (KIND < 0) {
+        r.rt = within;
+        r.split = 0;
+      } else {
+        r.rt = within / r.ns;
+        r.split = within % r.ns;
+        r.slot += r.rt * r.ns;
+      }
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(sum, kWave - 1);
+    slots0 += __builtin_amdgcn_readlane(sum0, kWave - 1);
+    slots1 += __builtin_amdgcn_readlane(sum1, kWave - 1);
+  }
+  return false;
+}
+
+template <bool V>
+struct Bool {
+  static constexpr bool value = V;
+};
 
 // Codes of the value NaN (0x7f, 0xff) in four bytes: 0x80 in each such byte.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-template <int D>
-__global__ __launch_bounds__(256) void attn_rows(Attn p) {
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi, float s) {
+  return __builtin_bit_cast(bf16x8, fp8x8_to_bf16x8_scaled(u32x2{lo, hi}, s));
+}
+
+// Block ids of the positions whose K, and whose V, a lane loads in a step.
+struct Ids {
+  int k, v;
+};
+
+// Few query rows: one row tile per workgroup (and split), whose W waves take
+// the steps in turn, codes straight from the cache to registers.  The bound
+// is the cache's bytes: 16 columns of the matrix instructions are there
+// anyway.  A step's K codes make way for the next step's as soon as the
+// scores are there, its V codes after the second product, so a wave has
+// loads in flight all the time without a second set of registers.
+//
+// Positions are dealt so that no value ever changes lanes: a K load's lane
+// (c, g) holds dimensions 16g.. of position 16(c/4) + 4t + c%4 of the step, so
+// the score tile t comes out with lane (c, g) holding positions
+// 16g + 4t + (0..3) of query row c -- the 16 positions whose V codes of one
+// dimension are the lane's 16-byte V load, which makes the weights the B
+// operand as they stand.
+template <int D, int W>
+__global__ __launch_bounds__(W* kWave) void attn_rows(Attn p) {
   constexpr int KH = D / 64, DT = D / 16;  // 64-dimension halves of K, 16-dimension tiles of V
-  __shared__ float lm[4][ROWS], ls[4][ROWS];
-  __shared__ float lo[4][ROWS][D + 1];
-  const int lb = p.c.lb, G = p.group;
+  __shared__ float lm[W][ROWS], ls[W][ROWS];
+  __shared__ float lo[W][ROWS][D + 4];
+  const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
   const int head = (int)(blockIdx.x % (unsigned)p.c.n_kv);
-  Seq s;
-  int rt;
-  if (!find_item(p.b, lb, (int)(blockIdx.x / (unsigned)p.c.n_kv),
-                 [&](const Seq& x) { return (int)(((long long)x.rows * G + ROWS - 1) / ROWS); }, s, rt))
-    return;
+  Item it;
+  if (!find_split<FEW>(p, (int)(blockIdx.x / (unsigned)p.c.n_kv), it)) return;
+  const Seq& s = it.s;
   const int l = (int)(threadIdx.x & 63u), wv = wave_id();
   const int c = l & 15, g = l >> 4;  // this lane's query row; its 16 positions of a step
-  const int r0 = rt * ROWS, r = r0 + c;
-  const int n_rows = (int)min((long long)s.rows * G - r0, (long long)ROWS);
-  const bool mine = c < n_rows;
-  const int tok = (mine ? r : r0) / G, hd = head * G + (mine ? r : r0) % G;
-  // positions that this row sees: [0, see)
-  const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;
-  const int see_all = min(max(s.pos0 + r0 / G + 1, 0), s.len);                     // seen by every row
-  const int see_any = min(max(s.pos0 + (r0 + n_rows - 1) / G + 1, 0), s.len);  // seen by some row
-  const int tiles = (see_any + TILE - 1) / TILE;
-  const int ns = splits_for(tiles, p.max_splits, p.min_tiles), sp = (int)blockIdx.y;
-  if (sp >= ns) return;
-  const int t0 = (int)((long long)tiles * sp / ns), t1 = (int)((long long)tiles * (sp + 1) / ns);
+  const RowTile rows = row_tile(s, G, it.rt, ROWS);
+  const int r0 = it.rt * ROWS, tiles = (rows.any + TILE - 1) / TILE;
+  const int t0 = (int)((long long)tiles * it.split / it.ns), t1 = (int)((long long)tiles * (it.split + 1) / it.ns);
+  const bool mine = c < rows.n_rows;
+  const int rr = mine ? r0 + c : r0, tok = rr / G, hd = head * G + rr % G;
+  const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
 
+  // Table entries of a step, loaded a step before the codes they lead to and
+  // judged only there: the loads are waited for in the order of their issue,
+  // so an entry asked for behind codes would arrive behind them.
+  const int* row = p.b.table + (long long)s.i * p.b.width;
+  const auto ids = [&](int t) {
+    const int top = min((t1 * TILE - 1) >> lb, p.b.width - 1);  // the last entry that this item may need
+    return Ids{row[min((t * TILE + 16 * (c >> 2)) >> lb, top)], row[min((t * TILE + 16 * g) >> lb, top)]};
+  };
+  const auto there = [&](int id, int pos) { return pos < s.len && id >= 0 && id < p.c.n_blocks; };
+  const unsigned bytes = (unsigned)(p.c.n_kv * D) << lb;  // of K or V of one block, all heads
+  const uint8_t *kb = p.c.k + ((long long)head * D << lb), *vb = p.c.v + ((long long)head * D << lb);
+  const float *ksb = p.c.ks + head, *vsb = p.c.vs + head;
+  u32x4 kw[4][KH], vw[DT];
+  float ks = 1.f, vs = 1.f;
+  bool gone = true;  // the lane's 16 positions of V and the scores are missing
+  const auto load_k = [&](int t, int id) {
+    const int pk = t * TILE + 16 * (c >> 2);
+    // block 0 in a missing block's place, masked later
+    const unsigned ik = there(id, pk) ? (unsigned)id : 0u;
+    const uint8_t* kp = kb + ((unsigned long long)ik * bytes + (unsigned)(((pk & off) + (c & 3)) * D + 16 * g));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < KH; ++h) kw[i][h] = *reinterpret_cast<const u32x4*>(kp + 4 * i * D + 64 * h);
+    ks = ksb[(unsigned long long)ik * (unsigned)p.c.n_kv];
+  };
+  const auto load_v = [&](int t, int id) {
+    const int pv = t * TILE + 16 * g;
+    gone = !there(id, pv);
+    const unsigned iv = gone ? 0u : (unsigned)id;
+    const uint8_t* vp = vb + ((unsigned long long)iv * bytes + (unsigned)((c << lb) + (pv & off)));
+    // block 0 may never have been written: its scale must not turn 0 into NaN
+    vs = vsb[(unsigned long long)iv * (unsigned)p.c.n_kv];
+    vs = gone ? 1.f : vs;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + ((16 * d) << lb));
+  };
+
+  const int begin = t0 + wv;
+  Ids next{-1, -1}, after{-1, -1};
+  if (begin < t1) {
+    next = ids(begin);
+    after = ids(begin + W);
+  }
   bf16x8 qv[2 * KH];
   {
     const uint16_t* qp = static_cast<const uint16_t*>(p.q.p) + (s.row0 + tok) * p.q.ts + hd * p.q.hs;
@@ -464,50 +660,41 @@ __global__ __launch_bounds__(256) void attn_rows(Attn p) {
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, sum = 0.f;
-  const int a = c >> 2, bb = c & 3;  // a K load's lane holds position 16a + 4t + bb of the step
 
-  for (int t = t0 + wv; t < t1; t += 4) {
-    const int pk = t * TILE + 16 * a, pv = t * TILE + 16 * g;
-    int ik = pk < s.len ? block_id(p.b, s.i, pk >> lb, p.c.n_blocks) : -1;
-    int iv = pv < s.len ? block_id(p.b, s.i, pv >> lb, p.c.n_blocks) : -1;
-    const bool gone = iv < 0;
-    ik = max(ik, 0);  // a missing block's place is taken by block 0, masked below
-    iv = max(iv, 0);
-    const uint8_t* kp = p.c.k + (((long long)ik * p.c.n_kv + head) * D << lb) + (long long)((pk & ((1 << lb) - 1)) + bb) * D + 16 * g;
-    const uint8_t* vp = p.c.v + (((long long)iv * p.c.n_kv + head) * D << lb) + ((long long)c << lb) + (pv & ((1 << lb) - 1));
-    const float ks = p.c.ks[(long long)ik * p.c.n_kv + head];
-    // block 0 may never have been written: its scale must not turn 0 into NaN
-    const float vs = gone ? 1.f : p.c.vs[(long long)iv * p.c.n_kv + head];
-    u32x4 kw[4][KH], vw[DT];
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int h = 0; h < KH; ++h) kw[x][h] = *reinterpret_cast<const u32x4*>(kp + 4 * x * D + 64 * h);
-#pragma unroll
-    for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + ((long long)(16 * d) << lb));
-
+  // Both are waited for here: left to itself, the second would be asked for
+  // behind the first codes, and the loop's waits be for everything.
+  asm volatile("" : "+v"(next.k), "+v"(next.v), "+v"(after.k), "+v"(after.v));
+  if (begin < t1) {
+    load_k(begin, next.k);
+    load_v(begin, next.v);
+    next = after;
+  }
+  // The last step is code of its own: behind loads that may not have been
+  // issued, every wait would have to be for all of them.
+  const auto step = [&](int t, auto more) {
+    const int pv = t * TILE + 16 * g;
     f32x4 sc[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i) {
+      sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < KH; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const u32x4 k8 = fp8x8_to_bf16x8_scaled(u32x2{kw[x][h][2 * e], kw[x][h][2 * e + 1]}, ks);
-          sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k8), qv[2 * h + e], sc[x], 0, 0, 0);
-        }
+        for (int e = 0; e < 2; ++e)
+          sc[i] = mfma16(codes_bf16(kw[i][h][2 * e], kw[i][h][2 * e + 1], ks), qv[2 * h + e], sc[i]);
     }
-    // scores of positions pv + 4x + i of row c
-    const bool masked = (t + 1) * TILE > see_all || __any(gone);
-    if (masked) {
+    if constexpr (more.value) {
+      after = ids(t + 2 * W);
+      load_k(t + W, next.k);
+    }
+    // scores of positions pv + 4i + j of row c
+    if ((t + 1) * TILE > rows.all || __any(gone)) {
+      // opaque: a branch for the few steps that need it, not its selects in every step
+      const int lim = opaque_v(gone ? 0 : see - pv);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool vis = !gone && pv + 4 * x + i < see;
-          sc[x][i] = vis ? sc[x][i] : -INFINITY;
-        }
+        for (int j = 0; j < 4; ++j) sc[i][j] = 4 * i + j < lim ? sc[i][j] : -INFINITY;
       // A NaN in V must not reach the rows that do not see it (0 * NaN): it
       // is taken out here, and put into the rows that do see it.
       uint32_t bad = 0;
@@ -515,12 +702,12 @@ __global__ __launch_bounds__(256) void attn_rows(Attn p) {
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) bad |= nan_bytes(vw[d][i]);
-      if (__any(bad)) {
+      if (__builtin_expect(__any(bad), 0)) {
         bf16x8 seen[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) seen[e][i] = (__bf16)((!gone && pv + 8 * e + i < see) ? 1.f : 0.f);
+          for (int i = 0; i < 8; ++i) seen[e][i] = (__bf16)(8 * e + i < lim ? 1.f : 0.f);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           f32x4 hit = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -528,13 +715,11 @@ __global__ __launch_bounds__(256) void attn_rows(Attn p) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t n = nan_bytes(vw[d][i]) >> 7;  // 1 in each NaN byte
-            is[i] = n * 0x38u;                            // e4m3 of 1
+            is[i] = n * 0x38u;                             // e4m3 of 1
             vw[d][i] &= ~(n * 0xffu);
           }
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(bf16x8, fp8x8_to_bf16x8_scaled(u32x2{is[2 * e], is[2 * e + 1]}, 1.f)), seen[e], hit, 0, 0, 0);
+          for (int e = 0; e < 2; ++e) hit = mfma16(codes_bf16(is[2 * e], is[2 * e + 1], 1.f), seen[e], hit);
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[d][i] = hit[i] > 0.f ? NAN : o[d][i];
         }
@@ -542,24 +727,26 @@ __global__ __launch_bounds__(256) void attn_rows(Attn p) {
     }
     float mt = sc[0][0];
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[x][i]);
+      for (int j = 0; j < 4; ++j) mt = fmaxf(mt, sc[i][j]);
     mt = max_xor32(max_xor16(mt)) * p.scale;
-    const float mn = fmaxf(m, mt), mref = mn == -INFINITY ? 0.f : mn;
-    const float al = __builtin_amdgcn_exp2f(m - mref);
-    m = mn;
-    float pr[16], add = 0.f;
+    if (__any(mt > m)) {  // some row's maximum grows: its sums so far take the new one
+      const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      sum *= al;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+      for (int d = 0; d < DT; ++d) o[d] *= al;
+    }
+    const float mref = m == -INFINITY ? 0.f : m;
+    float pr[16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pr[4 * x + i] = __builtin_amdgcn_exp2f(fmaf(sc[x][i], p.scale, -mref));
-        add += pr[4 * x + i];
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pr[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], p.scale, -mref));
+        sum += pr[4 * i + j];
       }
-    sum = sum * al + add;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] *= al;
     bf16x8 pb[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -572,85 +759,413 @@ __global__ __launch_bounds__(256) void attn_rows(Attn p) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const u32x4 v8 = fp8x8_to_bf16x8_scaled(u32x2{vw[d][2 * e], vw[d][2 * e + 1]}, vs);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v8), pb[e], o[d], 0, 0, 0);
-      }
+      for (int e = 0; e < 2; ++e) o[d] = mfma16(codes_bf16(vw[d][2 * e], vw[d][2 * e + 1], vs), pb[e], o[d]);
+    if constexpr (more.value) {
+      load_v(t + W, next.v);
+      next = after;
+    }
+  };
+  if (begin < t1) {
+    int t = begin;
+    for (; t + W < t1; t += W) step(t, Bool<true>{});
+    step(t, Bool<false>{});
   }
+
   sum = sum_xor32(sum_xor16(sum));
 
-  // join the four waves: o[d][i] is dimension 16d + 4g + i of row c
-  if (g == 0) lm[wv][c] = m, ls[wv][c] = sum;
+  // join the waves: o[d][i] is dimension 16d + 4g + i of row c
+  if (mine) {
+    if (g == 0) lm[wv][c] = m, ls[wv][c] = sum;
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lo[wv][c][16 * d + 4 * g + i] = o[d][i];
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&lo[wv][c][16 * d + 4 * g]) = o[d];
+  }
   __syncthreads();
-  const int row = (int)threadIdx.x / 16, q16 = (int)threadIdx.x % 16;
-  if (row >= n_rows) return;
-  float mm = lm[0][row];
+  for (int i = (int)threadIdx.x; i < rows.n_rows * (D / 4); i += W * kWave) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float mm = lm[0][row];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) mm = fmaxf(mm, lm[w][row]);
-  const float mref = mm == -INFINITY ? 0.f : mm;
-  float wt[4], tot = 0.f;
+    for (int w = 1; w < W; ++w) mm = fmaxf(mm, lm[w][row]);
+    const float mref = mm == -INFINITY ? 0.f : mm;
+    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+    float tot = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    wt[w] = __builtin_amdgcn_exp2f(lm[w][row] - mref);
-    tot += wt[w] * ls[w][row];
-  }
-  const int tk = (r0 + row) / G, oh = head * G + (r0 + row) % G;
-  const float inv = ns == 1 ? (tot > 0.f || tot != tot ? 1.f / tot : 0.f) : 1.f;
-  float y[D / 16];
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const int d = q16 * (D / 16) + i;
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) v += wt[w] * lo[w][row][d];
-    y[i] = v * inv;
-  }
-  if (ns == 1) {
-    uint16_t* op = static_cast<uint16_t*>(p.out.p) + (s.row0 + tk) * p.out.ts + oh * p.out.hs + q16 * (D / 16);
-#pragma unroll
-    for (int i = 0; i < D / 16; i += 2)
-      *reinterpret_cast<uint32_t*>(op + i) = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{y[i], y[i + 1]}, bf16x2));
-  } else {
-    float* pp = part_at<D>(p.part, (long long)(s.row0 + tk) * p.n_q + oh, p.max_splits, sp);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) pp[q16 * (D / 16) + i] = y[i];
-    if (q16 == 0) pp[D] = mm, pp[D + 1] = tot;
+    for (int w = 0; w < W; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lm[w][row] - mref);
+      tot += f * ls[w][row];
+      v += f * *reinterpret_cast<const f32x4*>(&lo[w][row][d]);
+    }
+    const int tk = (r0 + row) / G, oh = head * G + (r0 + row) % G;
+    if (it.ns == 1) {
+      v *= tot > 0.f || tot != tot ? 1.f / tot : 0.f;
+      uint16_t* op = static_cast<uint16_t*>(p.out.p) + (s.row0 + tk) * p.out.ts + oh * p.out.hs + d;
+      u32x2 w;
+      w.x = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, bf16x2));
+      w.y = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, bf16x2));
+      *reinterpret_cast<u32x2*>(op) = w;
+    } else {
+      const long long at = ((long long)(it.slot + it.split) * p.c.n_kv + head) * ROWS + row;
+      *reinterpret_cast<f32x4*>(p.d[FEW].part + at * D + d) = v;
+      if (d == 0) p.d[FEW].ml[at] = make_float2(mm, tot);
+    }
   }
 }
 
-// Joins the splits of every row that has more than one, in the splits' order.
+// Many query rows.  128 rows per workgroup, 32 to each of its four waves, on
+// v_mfma_f32_32x32x16_bf16; a step's 64 positions are turned from codes to
+// bf16 once and staged in LDS for all four (two buffers, one barrier a step;
+// the next step's codes are in flight meanwhile).  Rows of LDS are padded by
+// 16 bytes, which spreads the eight lanes that a 16-byte read serves at once
+// over all banks.  K rows lie in LDS in the order that makes a lane's 16
+// scores of 32 positions two runs of eight positions, 8h + 16m of half-wave h,
+// the B operand of the second product as they stand.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void attn_tile(Attn p) {
+  constexpr int KC = D / 16, DB = D / 32;            // 16-dimension pieces of a K row, 32-dimension blocks of V
+  constexpr int KS = D + 8, VS = TILE + 8;           // LDS row strides
+  constexpr int NL = D * TILE / (256 * 16);          // 16-byte loads per thread of K, and of V
+  __shared__ __align__(16) uint16_t kl[2][TILE * KS];
+  __shared__ __align__(16) uint16_t vl[2][D * VS];
+  __shared__ unsigned long long nans[2][D];  // positions of a step whose V is NaN, by dimension
+  __shared__ int bad[2];                     // 1 + the step in the buffer, if nans has any
+  const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
+  const int head = (int)(blockIdx.x % (unsigned)p.c.n_kv);
+  Item it;
+  // the last items first: a prompt's last row tiles have the most positions
+  if (!find_split<MANY>(p, p.d[MANY].items - 1 - (int)(blockIdx.x / (unsigned)p.c.n_kv), it)) return;
+  const Seq& s = it.s;
+  const int l = (int)(threadIdx.x & 63u), wv = wave_id(), tid = (int)threadIdx.x;
+  const int c = l & 31, h = l >> 5;
+  const RowTile rows = row_tile(s, G, it.rt, TILE_ROWS);
+  const int r0 = it.rt * TILE_ROWS, tiles = (rows.any + TILE - 1) / TILE;
+  const int t0 = (int)((long long)tiles * it.split / it.ns), t1 = (int)((long long)tiles * (it.split + 1) / it.ns);
+  const bool mine = 32 * wv + c < rows.n_rows;
+  const int rr = mine ? r0 + 32 * wv + c : r0, tok = rr / G, hd = head * G + rr % G;
+  const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
+  // every row of the wave sees [0, all)
+  const int all = min(max(s.pos0 + (r0 + min(32 * wv, rows.n_rows - 1)) / G + 1, 0), s.len);
+
+  bf16x8 qv[KC];
+  {
+    const uint16_t* qp = static_cast<const uint16_t*>(p.q.p) + (s.row0 + tok) * p.q.ts + hd * p.q.hs + 8 * h;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) qv[k] = *reinterpret_cast<const bf16x8*>(qp + 16 * k);
+  }
+  // this thread's share of the staging: 16 dimensions of position kt + .., 16
+  // positions of dimension vd + ..
+  const int kt = tid / KC, kd = tid % KC * 16, vd = tid / 4, vp = tid % 4 * 16;
+  const int* row = p.b.table + (long long)s.i * p.b.width;
+  const int top = min(max(t1 * TILE - 1, 0) >> lb, p.b.width - 1);
+  const unsigned bytes = (unsigned)(p.c.n_kv * D) << lb;  // of K or V of one block, all heads
+  const uint8_t *kb = p.c.k + ((long long)head * D << lb), *vb = p.c.v + ((long long)head * D << lb);
+  const float *ksb = p.c.ks + head, *vsb = p.c.vs + head;
+  const auto there = [&](int id, int pos) { return pos < s.len && id >= 0 && id < p.c.n_blocks; };
+  int idk[NL], idv;
+  const auto ids = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) idk[i] = row[min((t * TILE + kt + i * (256 / KC)) >> lb, top)];
+    idv = row[min((t * TILE + vp) >> lb, top)];
+  };
+  u32x4 kw[NL], vw[NL];
+  float ks[NL], vs;
+  unsigned gone_next = 0;  // the loaded step's runs of 16 positions that are missing
+  const auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int pos = t * TILE + kt + i * (256 / KC);
+      const bool ok = there(idk[i], pos);
+      const unsigned id = ok ? (unsigned)idk[i] : 0u;
+      kw[i] = *reinterpret_cast<const u32x4*>(kb + ((unsigned long long)id * bytes + (unsigned)((pos & off) * D + kd)));
+      ks[i] = ksb[(unsigned long long)id * (unsigned)p.c.n_kv];
+    }
+    const int pos = t * TILE + vp;
+    const bool ok = there(idv, pos);
+    gone_next = (unsigned)__ballot(!ok) & 15u;
+    const unsigned id = ok ? (unsigned)idv : 0u;
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      vw[i] = *reinterpret_cast<const u32x4*>(vb + ((unsigned long long)id * bytes + (unsigned)(((vd + i * 64) << lb) + (pos & off))));
+    vs = vsb[(unsigned long long)id * (unsigned)p.c.n_kv];
+    // What no row may see is zero in V.  K needs nothing: its scores are
+    // replaced.
+    if ((t + 1) * TILE > s.len || !ok) {
+      const int n = ok ? s.len - pos : 0;  // positions of the 16 that exist
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int left = n - 4 * j;
+          vw[i][j] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        }
+      vs = ok ? vs : 1.f;
+    }
+  };
+  const auto stage = [&](int t, int buf) {
+    if ((t + 1) * TILE > rows.all) {
+      // Rows differ in what they see, and a NaN in V must not reach those that
+      // do not see it (0 * NaN): it is taken out and its place noted.
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        uint32_t at = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t n = nan_bytes(vw[i][j]) >> 7;  // 1 in each NaN byte
+          at |= n * 0x10204080u >> 28 << (4 * j);
+          vw[i][j] &= ~(n * 0xffu);
+        }
+        reinterpret_cast<uint16_t*>(&nans[buf][vd + i * 64])[vp / 16] = (uint16_t)at;
+        any |= at;
+      }
+      if (any) bad[buf] = t + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int j = kt + i * (256 / KC);
+      // position 32a + 16m + 8h + 4b + e goes to row 32a + 16m + 8b + 4h + e
+      const int r = (j & ~12) | (j & 8) >> 1 | (j & 4) << 1;
+      u32x4* w = reinterpret_cast<u32x4*>(&kl[buf][r * KS + kd]);
+      w[0] = fp8x8_to_bf16x8_scaled(u32x2{kw[i][0], kw[i][1]}, ks[i]);
+      w[1] = fp8x8_to_bf16x8_scaled(u32x2{kw[i][2], kw[i][3]}, ks[i]);
+      u32x4* x = reinterpret_cast<u32x4*>(&vl[buf][(vd + i * 64) * VS + vp]);
+      x[0] = fp8x8_to_bf16x8_scaled(u32x2{vw[i][0], vw[i][1]}, vs);
+      x[1] = fp8x8_to_bf16x8_scaled(u32x2{vw[i][2], vw[i][3]}, vs);
+    }
+  };
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -INFINITY, sum = 0.f;
+  if (tid < 2) bad[tid] = 0;
+  if (t0 < t1) {
+    ids(t0);
+    load(t0);
+    ids(t0 + 1);
+  }
+  // q is waited for here: inside the loop the wait would stand in every step,
+  // behind the next step's codes
+#pragma unroll
+  for (int k = 0; k < KC; ++k) asm volatile("" : "+v"(qv[k]));
+  __syncthreads();
+  if (t0 < t1) stage(t0, t0 & 1);
+  __syncthreads();
+
+  for (int t = t0; t < t1; ++t) {
+    const int buf = t & 1;
+    const unsigned gone = gone_next;
+    if (t + 1 < t1) {
+      load(t + 1);
+      ids(t + 2);
+    }
+    f32x16 sc[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[a][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KC; ++k)
+        sc[a] = mfma32(*reinterpret_cast<const bf16x8*>(&kl[buf][(32 * a + c) * KS + 16 * k + 8 * h]), qv[k], sc[a]);
+    }
+    // score i of half a: position 32a + 16(i/8) + 8h + i%8 of the step
+    const bool masked = (t + 1) * TILE > all || gone;
+    if (masked) {
+      // opaque: a branch for the few steps that need it, not its 64 selects in every step
+      const int lim = opaque_v(see - t * TILE - 8 * h);
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sc[a][i] = 32 * a + 16 * (i / 8) + i % 8 < lim && !(gone >> (2 * a + i / 8) & 1) ? sc[a][i] : -INFINITY;
+    }
+    float mt = sc[0][0];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[a][i]);
+    mt = max_xor32(mt) * p.scale;
+    if (__any(mt > m)) {  // some row's maximum grows: its sums so far take the new one
+      const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      sum *= al;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] *= al;
+    }
+    const float mref = m == -INFINITY ? 0.f : m;
+    bf16x8 pb[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], p.scale, -mref));
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], p.scale, -mref));
+        sum += x + y;
+        const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
+        pb[a][i / 8][i % 8] = w[0];
+        pb[a][i / 8][i % 8 + 1] = w[1];
+      }
+    if (__builtin_expect((t + 1) * TILE > rows.all && bad[buf] == t + 1, 0)) {
+      // the NaN that stage() took out of V, put into the rows that see them
+      const int n = min(max(see - t * TILE, 0), TILE);
+      unsigned long long seen = n < 64 ? (1ull << n) - 1ull : ~0ull;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) seen &= gone >> i & 1 ? ~(0xffffull << (16 * i)) : ~0ull;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (nans[buf][32 * d + 8 * (i / 4) + 4 * h + i % 4] & seen) o[d][i] = NAN;
+    }
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+          o[d] = mfma32(*reinterpret_cast<const bf16x8*>(&vl[buf][(32 * d + c) * VS + 32 * a + 16 * i + 8 * h]), pb[a][i], o[d]);
+    if (t + 1 < t1) stage(t + 1, buf ^ 1);
+    __syncthreads();
+  }
+  sum = sum_xor32(sum);
+  if (!mine) return;
+  // o[d][4b + j] is dimension 32d + 8b + 4h + j of row c
+  if (it.ns == 1) {
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    uint16_t* op = static_cast<uint16_t*>(p.out.p) + (s.row0 + tok) * p.out.ts + hd * p.out.hs + 4 * h;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        u32x2 w;
+        w.x = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{o[d][4 * b] * inv, o[d][4 * b + 1] * inv}, bf16x2));
+        w.y = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{o[d][4 * b + 2] * inv, o[d][4 * b + 3] * inv}, bf16x2));
+        *reinterpret_cast<u32x2*>(op + 32 * d + 8 * b) = w;
+      }
+  } else {
+    const long long at = ((long long)(it.slot + it.split) * p.c.n_kv + head) * TILE_ROWS + 32 * wv + c;
+    float* pp = p.d[MANY].part + at * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        *reinterpret_cast<f32x4*>(pp + 32 * d + 8 * b) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+    if (h == 0) p.d[MANY].ml[at] = make_float2(m, sum);
+  }
+}
+
+// Where a row's partials are.
+struct Parts {
+  const float* part;  // the first split's outputs
+  const float2* ml;
+  long long stride;   // rows from one split to the next
+};
+template <int D>
+__device__ __forceinline__ Parts parts_of(const Attn& p, const Item& it, int oh) {
+  const Deal& d = p.d[it.kind];
+  const long long r = (long long)it.rt * p.group + oh % p.group, rt = r >> d.lr;
+  Parts x;
+  x.stride = (long long)p.c.n_kv << d.lr;
+  const long long at = (((it.slot + rt * it.ns) * p.c.n_kv + oh / p.group) << d.lr) + r - (rt << d.lr);
+  x.part = d.part + at * D;
+  x.ml = d.ml + at;
+  return x;
+}
+__device__ __forceinline__ void put_row4(const Rows& out, long long e, f32x4 a, float tot) {
+  a *= tot > 0.f || tot != tot ? 1.f / tot : 0.f;
+  u32x2 w;
+  w.x = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a[0], a[1]}, bf16x2));
+  w.y = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a[2], a[3]}, bf16x2));
+  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out.p) + e) = w;
+}
+
+// Joins the splits of the rows that have more than one; D/4 lanes read a
+// partial, the order of the sums is fixed.  Many rows: a wave takes HEADS
+// rows of one token after the other.
+template <int D, int HEADS>
+__global__ __launch_bounds__(256) void attn_join_waves(Attn p) {
+  constexpr int LPP = D / 4, NG = kWave / LPP, PER = 8;  // lanes per partial, partials at once, loads in flight
+  const int l = (int)(threadIdx.x & 63u), per_token = (p.n_q + HEADS - 1) / HEADS;
+  const int w = (int)blockIdx.x * 4 + wave_id();
+  Item it;
+  if (!find_split<-1>(p, w / per_token, it) || it.ns == 1) return;
+  const int ns = it.ns, ln = l % LPP, grp = l / LPP, h0 = w % per_token * HEADS;
+  for (int oh = h0; oh < min(h0 + HEADS, p.n_q); ++oh) {
+    const Parts x = parts_of<D>(p, it, oh);
+    float mm = -INFINITY;
+    for (int z = l; z < ns; z += kWave) mm = fmaxf(mm, x.ml[z * x.stride].x);
+    mm = wave_max(mm);
+    const float mref = mm == -INFINITY ? 0.f : mm;
+    float tot = 0.f;
+    f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int z0 = grp; z0 < ns; z0 += PER * NG) {
+      f32x4 v[PER];
+      float2 q[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int z = z0 + i * NG;
+        q[i] = z < ns ? x.ml[z * x.stride] : make_float2(-INFINITY, 0.f);
+        v[i] = z < ns ? *reinterpret_cast<const f32x4*>(x.part + z * x.stride * D + 4 * ln) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float f = __builtin_amdgcn_exp2f(q[i].x - mref);
+        tot += f * q[i].y;
+        a += f * v[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (NG == 4) a[i] = sum_xor16(a[i]);
+      a[i] = sum_xor32(a[i]);
+    }
+    if (NG == 4) tot = sum_xor16(tot);
+    tot = sum_xor32(tot);
+    if (grp == 0) put_row4(p.out, (it.s.row0 + it.rt) * p.out.ts + oh * p.out.hs + 4 * ln, a, tot);
+  }
+}
+
+// Few rows: a workgroup for each, all its partials in flight together.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join(Attn p) {
-  const int lb = p.c.lb, G = p.group;
-  const int head = (int)(blockIdx.x % (unsigned)p.c.n_kv);
-  Seq s;
-  int rt;
-  if (!find_item(p.b, lb, (int)(blockIdx.x / (unsigned)p.c.n_kv),
-                 [&](const Seq& x) { return (int)(((long long)x.rows * G + ROWS - 1) / ROWS); }, s, rt))
-    return;
-  const int r0 = rt * ROWS, n_rows = (int)min((long long)s.rows * G - r0, (long long)ROWS);
-  const int see_any = min(max(s.pos0 + (r0 + n_rows - 1) / G + 1, 0), s.len);
-  const int ns = splits_for((see_any + TILE - 1) / TILE, p.max_splits, p.min_tiles);
+  constexpr int LPP = D / 4, NG = 256 / LPP, PER = 4;  // lanes per partial, groups, partials in flight per group
+  __shared__ float lw[kMaxSplits], red1[4];
+  __shared__ f32x4 red[NG][LPP];
+  const int oh = (int)(blockIdx.x % (unsigned)p.n_q);
+  Item it;
+  if (!find_split<-1>(p, (int)(blockIdx.x / (unsigned)p.n_q), it)) return;
+  const int ns = it.ns;
   if (ns == 1) return;
-  for (int i = (int)threadIdx.x; i < n_rows * D; i += 256) {
-    const int row = i / D, d = i % D, tk = (r0 + row) / G, oh = head * G + (r0 + row) % G;
-    const float* pp = part_at<D>(p.part, (long long)(s.row0 + tk) * p.n_q + oh, p.max_splits, 0);
-    float mm = -INFINITY;
-    for (int z = 0; z < ns; ++z) mm = fmaxf(mm, pp[z * (D + 2) + D]);
-    const float mref = mm == -INFINITY ? 0.f : mm;
-    float v = 0.f, tot = 0.f;
-    for (int z = 0; z < ns; ++z) {
-      const float w = __builtin_amdgcn_exp2f(pp[z * (D + 2) + D] - mref);
-      v += w * pp[z * (D + 2) + d];
-      tot += w * pp[z * (D + 2) + D + 1];
-    }
-    const float y = tot > 0.f || tot != tot ? v / tot : 0.f;
-    static_cast<uint16_t*>(p.out.p)[(s.row0 + tk) * p.out.ts + oh * p.out.hs + d] =
-        __builtin_bit_cast(uint16_t, (__bf16)y);
+  const Parts x = parts_of<D>(p, it, oh);
+  const int ln = (int)threadIdx.x % LPP, grp = (int)threadIdx.x / LPP, tz = (int)threadIdx.x;
+  f32x4 v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int z = grp + i * NG;
+    v[i] = z < ns ? *reinterpret_cast<const f32x4*>(x.part + z * x.stride * D + 4 * ln) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float2 q = tz < ns ? x.ml[tz * x.stride] : make_float2(-INFINITY, 0.f);
+  const float mm = block_max<4>(q.x, red1);
+  const float w = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(q.x - mm);
+  lw[tz] = w;
+  const float tot = block_sum<4>(w * q.y, red1);
+  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < PER; ++i) a += lw[grp + i * NG] * v[i];
+  for (int z = grp + PER * NG; z < ns; z += NG) a += lw[z] * *reinterpret_cast<const f32x4*>(x.part + z * x.stride * D + 4 * ln);
+  red[grp][ln] = a;
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int i = 1; i < NG; ++i) a += red[i][ln];
+    put_row4(p.out, (it.s.row0 + it.rt) * p.out.ts + oh * p.out.hs + 4 * ln, a, tot);
   }
 }
 

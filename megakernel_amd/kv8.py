@@ -24,17 +24,24 @@ a graph: a replay reads lengths and tables anew, while sizes stay fixed.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
 
 from . import _lib
 
-_TYPES = {torch.float32: 0, torch.bfloat16: 1}  # MK_TYPE_F32, MK_TYPE_BF16
+_TYPES = {torch.bfloat16: 1, torch.float32: 0}  # MK_TYPE_BF16, MK_TYPE_F32
+_BF16 = {torch.bfloat16: 1}
 
 
 class _Rows(ctypes.Structure):
     _fields_ = [("p", ctypes.c_void_p), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong),
                 ("type", ctypes.c_int)]
+
+
+# one _Rows as bytes, in a third of the structure's time
+_pack_rows = struct.Struct("@Pqqi0P").pack
 
 
 class _CCache(ctypes.Structure):
@@ -49,10 +56,15 @@ class _CBatch(ctypes.Structure):
                 ("max_kv", ctypes.c_int)]
 
 
-def _whole(t, dtype, shape, name: str):
-    """A contiguous GPU tensor of one type; None in `shape` is any size."""
+def _whole(t, dtype, shape, device: int, name: str):
+    """A contiguous tensor of one type and shape on GPU `device`; None in
+    `shape` is any size."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return
     if not t.is_cuda:
         raise ValueError(f"{name} must be on the GPU, not on {t.device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
     if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
@@ -61,36 +73,39 @@ def _whole(t, dtype, shape, name: str):
         raise ValueError(f"{name} must be contiguous")
 
 
-def _same_gpu(device, **tensors):
-    for name, t in tensors.items():
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
+def _rows(t, shape, device: int, name: str, types=_TYPES) -> bytes:
+    """Rows [tokens][heads][dim] with any token and head stride, as a
+    megakernel_rows."""
+    typ = types.get(t.dtype)
+    if typ is None or t.shape != shape or t.get_device() != device or t.stride(2) != 1:
+        if typ is None:
+            raise ValueError(f"{name} must be {' or '.join(str(x)[6:] for x in types)}, not {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+        if t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+        raise ValueError(f"the last dimension of {name} must be contiguous (stride {t.stride(2)})")
+    # of a single token or head, the stride says nothing
+    return _pack_rows(t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0, typ)
 
 
-def _rows(t, tokens: int, heads: int, dim: int, device, name: str) -> _Rows:
-    """Rows [tokens][heads][dim] with any token and head stride."""
-    if t.dtype not in _TYPES:
-        raise ValueError(f"{name} must be bfloat16 or float32, not {t.dtype}")
-    if t.shape != (tokens, heads, dim):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(tokens, heads, dim)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    st, sh, sd = t.stride()
-    if sd != 1:
-        raise ValueError(f"the last dimension of {name} must be contiguous (stride {sd})")
-    return _Rows(t.data_ptr(), st if tokens > 1 else 0, sh if heads > 1 else 0, _TYPES[t.dtype])
+_library = None
 
 
-def _call(fn, device, *args):
-    """Enqueue on the current stream of `device`; raises what the library reports."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call(name: str, device: int, *args):
+    """Enqueue on the current stream of GPU `device`; raises what the library reports."""
+    global _library
+    if _library is None:
+        _library = _lib.load()
+    fn = getattr(_library, name)
+    # the handle of torch.cuda.current_stream(device), without the object around it
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, _raw_stream(device))
     if rc:
-        lib = _lib.load()
-        _lib.check(lib, rc, fn.__name__.replace("megakernel_", ""))
+        _lib.check(_library, rc, name[11:])
 
 
 class Cache:
@@ -101,16 +116,16 @@ class Cache:
     """
 
     def __init__(self, k, v, k_scale, v_scale):
-        _whole(k, torch.uint8, (None, None, None, None), "k")
+        device = k.get_device()
+        _whole(k, torch.uint8, (None, None, None, None), device, "k")
         n_blocks, n_kv, block, head_dim = k.shape
-        _whole(v, torch.uint8, (n_blocks, n_kv, head_dim, block), "v")
-        _whole(k_scale, torch.float32, (n_blocks, n_kv), "k_scale")
-        _whole(v_scale, torch.float32, (n_blocks, n_kv), "v_scale")
-        _same_gpu(k.device, v=v, k_scale=k_scale, v_scale=v_scale)
+        _whole(v, torch.uint8, (n_blocks, n_kv, head_dim, block), device, "v")
+        _whole(k_scale, torch.float32, (n_blocks, n_kv), device, "k_scale")
+        _whole(v_scale, torch.float32, (n_blocks, n_kv), device, "v_scale")
         if block not in (16, 32, 64, 128) or head_dim not in (64, 128):
             raise ValueError(f"blocks of {block} positions (16, 32, 64 or 128), head_dim {head_dim} (64 or 128)")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_blocks, self.n_kv, self.block, self.head_dim, self.device = n_blocks, n_kv, block, head_dim, k.device
+        self.n_blocks, self.n_kv, self.block, self.head_dim, self.device = n_blocks, n_kv, block, head_dim, device
         self._c = _CCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_blocks, block, n_kv,
                           head_dim)
         self._ref = ctypes.byref(self._c)
@@ -137,15 +152,15 @@ class Batch:
     """
 
     def __init__(self, table, q_start, kv_len, n_tokens: int, max_kv: int = 0):
-        _whole(kv_len, torch.int32, (None,), "kv_len")
+        device = kv_len.get_device()
+        _whole(kv_len, torch.int32, (None,), device, "kv_len")
         n_seq = kv_len.shape[0]
-        _whole(table, torch.int32, (n_seq, None), "table")
-        _whole(q_start, torch.int32, (n_seq + 1,), "q_start")
-        _same_gpu(kv_len.device, table=table, q_start=q_start)
+        _whole(table, torch.int32, (n_seq, None), device, "table")
+        _whole(q_start, torch.int32, (n_seq + 1,), device, "q_start")
         if n_tokens < 0 or max_kv < 0 or table.shape[1] < 1:
             raise ValueError(f"n_tokens {n_tokens} and max_kv {max_kv} (at least 0), table width {table.shape[1]} (at least 1)")
         self.table, self.q_start, self.kv_len = table, q_start, kv_len
-        self.n_seq, self.n_tokens, self.max_kv, self.device = n_seq, int(n_tokens), int(max_kv), kv_len.device
+        self.n_seq, self.n_tokens, self.max_kv, self.device = n_seq, int(n_tokens), int(max_kv), device
         # of no sequence there are no addresses to hand over, and nothing to do
         self._c = _CBatch(table.data_ptr() or 16, q_start.data_ptr(), kv_len.data_ptr() or 16, n_seq, table.shape[1],
                           self.n_tokens, self.max_kv)
@@ -161,28 +176,25 @@ def qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q_out, k_out, eps: float =
     may lie in a packed QKV tensor, and an output may be its own input."""
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k are [tokens][heads][head_dim], not {tuple(q.shape)} and {tuple(k.shape)}")
-    if not q.is_cuda:
-        raise ValueError(f"q must be on the GPU, not on {q.device}")
+    device = q.get_device()
     tokens, n_q, dim = q.shape
-    n_kv, device = k.shape[1], q.device
-    _whole(q_gain, torch.bfloat16, (dim,), "q_gain")
-    _whole(k_gain, torch.bfloat16, (dim,), "k_gain")
-    _whole(inv_freq, torch.float32, (dim // 2,), "inv_freq")
-    _whole(pos, torch.int32, (tokens,), "pos")
-    _same_gpu(device, q_gain=q_gain, k_gain=k_gain, inv_freq=inv_freq, pos=pos)
-    rows = [_rows(t, tokens, h, dim, device, name) for t, h, name in
-            ((q, n_q, "q"), (k, n_kv, "k"), (q_out, n_q, "q_out"), (k_out, n_kv, "k_out"))]
+    n_kv = k.shape[1]
+    _whole(pos, torch.int32, (tokens,), device, "pos")
+    _whole(q_gain, torch.bfloat16, (dim,), device, "q_gain")
+    _whole(k_gain, torch.bfloat16, (dim,), device, "k_gain")
+    _whole(inv_freq, torch.float32, (dim // 2,), device, "inv_freq")
+    qs, ks = (tokens, n_q, dim), (tokens, n_kv, dim)
+    rows = (_rows(q, qs, device, "q"), _rows(k, ks, device, "k"), _rows(q_out, qs, device, "q_out"),
+            _rows(k_out, ks, device, "k_out"))
     if tokens == 0:
         return
-    a, b, c, d = (ctypes.byref(r) for r in rows)
-    _call(_lib.load().megakernel_op_qk_norm_rope, device, a, b, q_gain.data_ptr(), k_gain.data_ptr(),
-          inv_freq.data_ptr(), pos.data_ptr(), c, d, tokens, n_q, n_kv, dim, eps)
+    _call("megakernel_op_qk_norm_rope", device, rows[0], rows[1], q_gain.data_ptr(), k_gain.data_ptr(),
+          inv_freq.data_ptr(), pos.data_ptr(), rows[2], rows[3], tokens, n_q, n_kv, dim, eps)
 
 
-def _pair(cache: Cache, batch: Batch, k, v, names):
-    _same_gpu(cache.device, batch=batch)
-    r = [_rows(t, batch.n_tokens, cache.n_kv, cache.head_dim, cache.device, n) for t, n in zip((k, v), names)]
-    return ctypes.byref(r[0]), ctypes.byref(r[1])
+def _one_gpu(cache: Cache, batch: Batch):
+    if cache.device != batch.device:
+        raise ValueError(f"the batch is on cuda:{batch.device}, not on cuda:{cache.device}")
 
 
 def append(cache: Cache, batch: Batch, k, v):
@@ -191,18 +203,22 @@ def append(cache: Cache, batch: Batch, k, v):
     fits its rows into e4m3; rows that a block already holds are rounded again
     where a new row makes its scale grow.  Two sequences of one call may not
     append to the same block."""
-    a, b = _pair(cache, batch, k, v, ("k", "v"))
+    _one_gpu(cache, batch)
+    shape = (batch.n_tokens, cache.n_kv, cache.head_dim)
+    a, b = _rows(k, shape, cache.device, "k"), _rows(v, shape, cache.device, "v")
     if batch.n_seq and batch.n_tokens:
-        _call(_lib.load().megakernel_op_kv8_append, cache.device, cache._ref, batch._ref, a, b)
+        _call("megakernel_op_kv8_append", cache.device, cache._ref, batch._ref, a, b)
 
 
 def read(cache: Cache, batch: Batch, k_out, v_out):
     """The values of the batch's rows into k_out, v_out [n_tokens][n_kv][head_dim]
     (bf16 or fp32, exact in both).  ``q_start`` of a batch whose rows are whole
     contexts is their lengths' running sum."""
-    a, b = _pair(cache, batch, k_out, v_out, ("k_out", "v_out"))
+    _one_gpu(cache, batch)
+    shape = (batch.n_tokens, cache.n_kv, cache.head_dim)
+    a, b = _rows(k_out, shape, cache.device, "k_out"), _rows(v_out, shape, cache.device, "v_out")
     if batch.n_seq and batch.n_tokens:
-        _call(_lib.load().megakernel_op_kv8_read, cache.device, cache._ref, batch._ref, a, b)
+        _call("megakernel_op_kv8_read", cache.device, cache._ref, batch._ref, a, b)
 
 
 def workspace_bytes(cache: Cache, batch: Batch, n_q: int) -> int:
@@ -226,21 +242,19 @@ def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, wo
     torch's allocator."""
     if q.dim() != 3:
         raise ValueError(f"q is [tokens][heads][head_dim], not {tuple(q.shape)}")
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
-        raise ValueError(f"q and out must be bfloat16, not {q.dtype} and {out.dtype}")
+    _one_gpu(cache, batch)
     device, n_q = cache.device, q.shape[1]
-    _same_gpu(device, batch=batch)
-    a = _rows(q, batch.n_tokens, n_q, cache.head_dim, device, "q")
-    b = _rows(out, batch.n_tokens, n_q, cache.head_dim, device, "out")
+    shape = (batch.n_tokens, n_q, cache.head_dim)
+    a, b = _rows(q, shape, device, "q", _BF16), _rows(out, shape, device, "out", _BF16)
     need = workspace_bytes(cache, batch, n_q)
     if not batch.n_seq or not batch.n_tokens:
         return
-    if workspace is None:
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    else:
-        _whole(workspace, torch.uint8, (None,), "workspace")
-        _same_gpu(device, workspace=workspace)
-    _call(_lib.load().megakernel_op_kv8_attention, device, cache._ref, batch._ref, ctypes.byref(a), ctypes.byref(b), n_q,
-          cache.head_dim ** -0.5 if scale is None else scale, workspace.data_ptr() if workspace is not None else None,
-          workspace.numel() if workspace is not None else 0)
+    at = size = None
+    if workspace is not None:
+        _whole(workspace, torch.uint8, (None,), device, "workspace")
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    if workspace is not None:
+        at, size = workspace.data_ptr(), workspace.numel()
+    _call("megakernel_op_kv8_attention", device, cache._ref, batch._ref, a, b, n_q,
+          cache.head_dim ** -0.5 if scale is None else scale, at, size or 0)
