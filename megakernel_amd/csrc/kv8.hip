@@ -220,19 +220,19 @@ static bool heads_ok(const char* op, int n_q, int n_kv) {
   return true;
 }
 
+// Pieces of 4 rows x 8 dimensions of one block and head.
+static int block_pieces(const megakernel_kv8_cache* c) { return c->block / 4 * (c->head_dim / 8); }
+
 template <int D>
-static void launch_append(int passes, bool f32, dim3 g, hipStream_t st, Cache c, Batch b, Rows k, Rows v) {
+static void launch_append(int pieces, bool f32, dim3 g, hipStream_t st, Cache c, Batch b, Rows k, Rows v) {
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, g, dim3(256), 0, st, c, b, k, v); };
-  if constexpr (D == 64) {
-    if (passes == 1) return f32 ? go(append<D, 1, true>) : go(append<D, 1, false>);
-    if (passes == 2) return f32 ? go(append<D, 2, true>) : go(append<D, 2, false>);
-    return f32 ? go(append<D, 4, true>) : go(append<D, 4, false>);
-  } else {
-    if (passes == 1) return f32 ? go(append<D, 1, true>) : go(append<D, 1, false>);
-    if (passes == 2) return f32 ? go(append<D, 2, true>) : go(append<D, 2, false>);
-    if (passes == 4) return f32 ? go(append<D, 4, true>) : go(append<D, 4, false>);
-    return f32 ? go(append<D, 8, true>) : go(append<D, 8, false>);
-  }
+  if constexpr (D == 64)
+    if (pieces == 32) return f32 ? go(append<D, 32, 1, true>) : go(append<D, 32, 1, false>);
+  if (pieces == 64) return f32 ? go(append<D, 64, 1, true>) : go(append<D, 64, 1, false>);
+  if (pieces == 128) return f32 ? go(append<D, 128, 1, true>) : go(append<D, 128, 1, false>);
+  if constexpr (D == 128)
+    if (pieces == 512) return f32 ? go(append<D, 256, 2, true>) : go(append<D, 256, 2, false>);
+  return f32 ? go(append<D, 256, 1, true>) : go(append<D, 256, 1, false>);
 }
 
 }  // namespace kv8
@@ -311,15 +311,15 @@ int megakernel_op_kv8_append(const megakernel_kv8_cache* cache, const megakernel
     set_err("%s: k and v must have one type (%d, %d)", op, k->type, v->type);
     return -1;
   }
-  const long long groups = block_items(batch, cache->block) * cache->n_kv;
+  const int pieces = block_pieces(cache), heads = pieces < 256 ? 256 / pieces : 1;
+  const long long groups = block_items(batch, cache->block) * ((cache->n_kv + heads - 1) / heads);
   if (groups == 0) return 0;
-  if (!grid_ok(op, 2 * groups)) return -1;
-  const dim3 g((unsigned)groups, 2);
-  const int rpp = 2048 / cache->head_dim, passes = (cache->block + rpp - 1) / rpp;
+  if (!grid_ok(op, groups)) return -1;
+  const dim3 g((unsigned)groups);
   const bool f32 = k->type == MK_TYPE_F32;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->head_dim == 64) launch_append<64>(passes, f32, g, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v));
-  else launch_append<128>(passes, f32, g, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v));
+  if (cache->head_dim == 64) launch_append<64>(pieces, f32, g, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v));
+  else launch_append<128>(pieces, f32, g, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v));
   return launched(op);
 }
 
@@ -336,14 +336,19 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
     set_err("%s: k_out and v_out must have one type (%d, %d)", op, k_out->type, v_out->type);
     return -1;
   }
-  const long long groups = block_items(batch, cache->block) * cache->n_kv;
-  if (groups == 0) return 0;
-  if (!grid_ok(op, 2 * groups)) return -1;
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)groups, 2), dim3(256), 0, static_cast<hipStream_t>(stream), cache_of(cache),
-                       batch_of(batch), rows_of(k_out), rows_of(v_out));
-  };
+  const long long items = block_items(batch, cache->block);
+  // a piece for every thread, and several where that is more workgroups than run at once
   const bool f32 = k_out->type == MK_TYPE_F32;
+  const int pieces = block_pieces(cache) * (f32 ? 2 : 1);
+  int heads = pieces < 256 ? 256 / pieces : 1;
+  while (heads < cache->n_kv && items * cache->n_kv > 2048ll * heads) heads *= 2;
+  const long long groups = items * ((cache->n_kv + heads - 1) / heads);
+  if (groups == 0) return 0;
+  if (!grid_ok(op, groups)) return -1;
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, static_cast<hipStream_t>(stream), cache_of(cache),
+                       batch_of(batch), rows_of(k_out), rows_of(v_out), heads);
+  };
   if (cache->head_dim == 64) f32 ? go(read_back<64, true>) : go(read_back<64, false>);
   else f32 ? go(read_back<128, true>) : go(read_back<128, false>);
   return launched(op);

@@ -215,14 +215,15 @@ __device__ __forceinline__ int scale_exp(float amax) {
   return max(e, -126);
 }
 
-// Codes of four values that were divided by the scale: nearest, ties to even;
-// beyond 448 (infinities alone) saturated; NaN stays NaN.
+// Codes of four values that were divided by the scale: nearest, ties to even.
+// Finite values are within 448.
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-  const auto cl = [](float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); };
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a), cl(b), 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(cl(c), cl(d), w, true);
-  return (uint32_t)w;
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
+// Infinities to +-448; NaN stays.
+__device__ __forceinline__ float saturate(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
+
 // Four codes re-rounded after multiplying by a power of two of at most one.
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
@@ -230,136 +231,222 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   return encode4(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
 }
 
-// x * 2^-e for e in [-126, 120], exactly: two factors where one would leave
-// fp32's range.
-struct Unscale {
-  float f, g;
+// A block's rows are dealt to threads in pieces of 4 rows x W dimensions (8;
+// 4 where rows are written in fp32): in K a piece is W consecutive bytes of 4
+// rows, in V 4 consecutive bytes of W dimensions, so neither layout needs a
+// transposition through LDS, and in the rows it is 16 consecutive bytes (32
+// of fp32 input).  A wave holds 32 rows x 8W dimensions (16 rows x 16W of the
+// smallest block), where 64 consecutive bytes of K, 32 of V and 128 of a row
+// are touched at once.
+struct Piece {
+  int row, dim;
 };
-__device__ __forceinline__ Unscale unscale(int e) {
-  const int h = -e / 2;
-  return Unscale{ldexpf(1.f, h), ldexpf(1.f, -e - h)};
+template <int D, int W>
+__device__ __forceinline__ Piece piece_at(int u, int lb) {
+  // u: row quad (3 bits, 2 for blocks of 16), dimension group (the rest of 6 bits, if there are so many), then the rest
+  constexpr int gb = (D == 64 ? 6 : 7) - (W == 8 ? 3 : 2);  // log2 of the groups of W dimensions
+  const int qb = min(lb - 2, 3), ob = min(6 - qb, gb);
+  const int hi = u >> (qb + ob), qh = lb - 2 - qb;  // row quads beyond the first 8
+  return Piece{((u & ((1 << qb) - 1)) | (hi & ((1 << qh) - 1)) << qb) * 4, ((u >> qb & ((1 << ob) - 1)) | hi >> qh << ob) * W};
 }
 
-// One workgroup per (block that rows go to, head, K or V).  A thread holds 8
-// dimensions of one row per pass; all rows of the block stay in registers
-// between the maximum and the rounding, so the input is read once.
-template <int D, int PASSES, bool SRC32>
+// Eight elements of a row as they were loaded (once, so past the caches).
+template <bool F32>
+struct Raw8 {
+  u32x4 w[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, long long e) {
+    const u32x4* q = F32 ? reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + e)
+                         : reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + e);
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = __builtin_nontemporal_load(q + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i) w[i] = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (F32) return __uint_as_float(w[e >> 2][e & 3]);
+    else return e & 1 ? bf16_hi(w[0][e >> 1]) : bf16_lo(w[0][e >> 1]);
+  }
+  // Largest magnitude so far, as bits (whose order is that of the values,
+  // infinities above and NaN above those): of one fp32, or of two bf16 side
+  // by side.
+  __device__ __forceinline__ void top(uint32_t& m) const {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (F32) m = max(m, w[i][j] & 0x7fffffffu);
+        else
+          m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                     __builtin_bit_cast(u16x2, w[i][j] & 0x7fff7fffu)));
+      }
+  }
+  static __device__ __forceinline__ float top_value(uint32_t m) {
+    return __uint_as_float(F32 ? m : max(m & 0xffff0000u, m << 16));
+  }
+};
+
+// One team of T threads per block that rows go to and head, K and V both; a
+// workgroup holds 256 / T heads.  The rows stay in registers between the
+// maximum and the rounding, so the input is read once.
+template <int D, int T, int PASSES, bool SRC32>
 __global__ __launch_bounds__(256) void append(Cache c, Batch b, Rows kr, Rows vr) {
-  constexpr int TPR = D / 8, RPP = 256 / TPR;  // threads per row, rows per pass
-  constexpr int MAXB = PASSES * RPP < 128 ? PASSES * RPP : 128;
-  __shared__ float red[4];
-  __shared__ __align__(16) uint8_t tile[D * MAXB];
+  constexpr int HEADS = 256 / T;
+  __shared__ float red[4][2];
   Seq s;
   int within;
-  const int head = (int)(blockIdx.x % (unsigned)c.n_kv);
-  if (!find_item(b, c.lb, (int)(blockIdx.x / (unsigned)c.n_kv), [&](const Seq& q) { return blocks_touched(q, c.lb); },
-                 s, within))
-    return;
-  const bool is_v = blockIdx.y != 0;
+  const unsigned sets = (unsigned)((c.n_kv + HEADS - 1) / HEADS);
+  if (!find_item(b, c.lb, (int)(blockIdx.x / sets), [&](const Seq& q) { return blocks_touched(q, c.lb); }, s, within)) return;
+  const int tid = (int)threadIdx.x, head = (int)(blockIdx.x % sets) * HEADS + tid / T;
   const int B = 1 << c.lb, j = (max(s.pos0, 0) >> c.lb) + within;
   const int id = block_id(b, s.i, j, c.n_blocks);
   if (id < 0) return;
+  const bool on = head < c.n_kv;
   const int p0 = j << c.lb;
-  const int r0 = max(max(s.pos0, 0) - p0, 0);                 // first new row of the block
-  const int r1 = min(min(s.pos0 + s.rows, s.len) - p0, B);    // end of its new rows
-  const Rows& src = is_v ? vr : kr;
-  const int tr = (int)threadIdx.x / TPR, d0 = (int)threadIdx.x % TPR * 8;
-  float f[PASSES][8];
-  float amax = 0.f;
+  const int r0 = max(max(s.pos0, 0) - p0, 0);               // first new row of the block
+  const int r1 = min(min(s.pos0 + s.rows, s.len) - p0, B);  // end of its new rows
+  const long long at = (long long)id * c.n_kv + head;
+  float old_k = 0.f, old_v = 0.f;
+  if (r0 > 0 && on) old_k = c.ks[at], old_v = c.vs[at];
+  Raw8<SRC32> kr8[PASSES][4], vr8[PASSES][4];
+  uint32_t vold[PASSES][8];  // V's dwords, where a piece has rows that stay
+  uint32_t ktop = 0, vtop = 0;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int r = p * RPP + tr;
+    const Piece pc = piece_at<D, 8>(tid % T + p * T, c.lb);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[p][i] = 0.f;
-    if (r >= r0 && r < r1) {
-      load8<SRC32>(src.p, (s.row0 + (long long)(p0 + r - s.pos0)) * src.ts + head * src.hs + d0, f[p]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = fabsf(f[p][i]);
-      if (x < INFINITY) amax = fmaxf(amax, x);  // the scale is that of the finite values
-    }
-  }
-  amax = block_max<4>(amax, red);
-  float* sp = (is_v ? c.vs : c.ks) + (long long)id * c.n_kv + head;
-  int e = scale_exp(amax);
-  float ratio = 1.f;  // old scale / new scale
-  if (r0 > 0) {
-    const float old = *sp;
-    const int eo = old > 0.f ? max(min(ilogbf(old), 127), -126) : -126;
-    ratio = eo < e ? ldexpf(1.f, eo - e) : 1.f;
-    e = max(e, eo);
-  }
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) *sp = ldexpf(1.f, e);
-  const Unscale u = unscale(e);
-  uint8_t* dst = (is_v ? c.v : c.k) + ((long long)id * c.n_kv + head) * ((long long)D << c.lb);
-  if (!is_v) {
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int r = p * RPP + tr;
-      u32x2* w = reinterpret_cast<u32x2*>(dst + (long long)r * D + d0);
-      if (r >= r0 && r < r1) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = f[p][i] * u.f * u.g;
-        *w = u32x2{encode4(x[0], x[1], x[2], x[3]), encode4(x[4], x[5], x[6], x[7])};
-      } else if (r < r0 && ratio < 1.f) {
-        const u32x2 o = *w;
-        *w = u32x2{rescale4(o.x, ratio), rescale4(o.y, ratio)};
+    for (int i = 0; i < 4; ++i) {
+      const int r = pc.row + i;
+      const long long row = s.row0 + (long long)(p0 + r - s.pos0);
+      kr8[p][i].zero();
+      vr8[p][i].zero();
+      if (on && r >= r0 && r < r1) {
+        kr8[p][i].load(kr.p, row * kr.ts + head * kr.hs + pc.dim);
+        vr8[p][i].load(vr.p, row * vr.ts + head * vr.hs + pc.dim);
       }
     }
-    return;
-  }
-  // V: the codes turn in LDS to [D][B]; 16 rows of one dimension make a piece
+    if (on && pc.row < r1 && (pc.row < r0 || pc.row + 4 > r1)) {
 #pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const int r = p * RPP + tr;
-    if (r >= r0 && r < r1) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = f[p][i] * u.f * u.g;
-      const uint32_t w[2] = {encode4(x[0], x[1], x[2], x[3]), encode4(x[4], x[5], x[6], x[7])};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) tile[(d0 + i) * B + r] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+      for (int e = 0; e < 8; ++e)
+        vold[p][e] = *reinterpret_cast<const uint32_t*>(c.v + ((at * D + pc.dim + e) << c.lb) + pc.row);
     }
   }
-  __syncthreads();
-  const int c0 = ratio < 1.f ? 0 : r0 >> 4, c1 = (r1 + 15) >> 4;  // pieces that change
-  const int n = D * (c1 - c0);
-  for (int i = (int)threadIdx.x; i < n; i += 256) {
-    const int d = i / (c1 - c0), pc = c0 + i % (c1 - c0);
-    u32x4* w = reinterpret_cast<u32x4*>(dst + (long long)d * B + pc * 16);
-    u32x4 x = *reinterpret_cast<const u32x4*>(tile + d * B + pc * 16);
-    if (pc * 16 < r0 || pc * 16 + 16 > r1) {  // some rows of the piece are old, or not written yet
-      const u32x4 o = *w;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t os = ratio < 1.f ? rescale4(o[q], ratio) : o[q];
-        uint32_t m_new = 0, m_old = 0;
+  for (int p = 0; p < PASSES; ++p)
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const int r = pc * 16 + 4 * q + z;
-          if (r >= r0 && r < r1) m_new |= 0xffu << (8 * z);
-          if (r < r0) m_old |= 0xffu << (8 * z);
+    for (int i = 0; i < 4; ++i) {
+      kr8[p][i].top(ktop);
+      vr8[p][i].top(vtop);
+    }
+  float kmax = Raw8<SRC32>::top_value(ktop), vmax = Raw8<SRC32>::top_value(vtop);
+  const bool odd = __any(!(kmax < INFINITY) || !(vmax < INFINITY));  // some value is no finite number
+  if (__builtin_expect(odd, 0)) {                                    // the scale is that of the finite values
+    kmax = vmax = 0.f;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = fabsf(kr8[p][i].get(e)), y = fabsf(vr8[p][i].get(e));
+          kmax = fmaxf(kmax, x < INFINITY ? x : 0.f);
+          vmax = fmaxf(vmax, y < INFINITY ? y : 0.f);
         }
-        x[q] = (x[q] & m_new) | (os & m_old) | (o[q] & ~(m_new | m_old));
+  }
+  kmax = max_xor16(group_max<16>(kmax));
+  vmax = max_xor16(group_max<16>(vmax));
+  if constexpr (T >= 64) {
+    kmax = max_xor32(kmax);
+    vmax = max_xor32(vmax);
+  }
+  if constexpr (T > 64) {
+    if (tid % 64 == 0) red[tid / 64][0] = kmax, red[tid / 64][1] = vmax;
+    __syncthreads();
+    const int w = tid / T * (T / 64);
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) kmax = fmaxf(kmax, red[w + i][0]), vmax = fmaxf(vmax, red[w + i][1]);
+  }
+  if (!on) return;
+  // the block's scale, and old scale / new scale
+  const auto settle = [&](float amax, float old, float& ratio) {
+    int e = scale_exp(amax);
+    ratio = 1.f;
+    if (r0 > 0) {
+      const int eo = old > 0.f ? max(min(ilogbf(old), 127), -126) : -126;
+      if (eo < e) ratio = ldexpf(1.f, eo - e);
+      e = max(e, eo);
+    }
+    return e;
+  };
+  float kratio, vratio;
+  const int ke = settle(kmax, old_k, kratio), ve = settle(vmax, old_v, vratio);
+  if (tid % T == 0) {  // the team's old scales were read before its maxima met
+    c.ks[at] = ldexpf(1.f, ke);
+    c.vs[at] = ldexpf(1.f, ve);
+  }
+  const float ku = ldexpf(1.f, -ke), vu = ldexpf(1.f, -ve);
+  uint8_t *kd = c.k + (at * D << c.lb), *vd = c.v + (at * D << c.lb);
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const Piece pc = piece_at<D, 8>(tid % T + p * T, c.lb);
+    if (pc.row >= r1) continue;
+    const auto code4 = [&](float x, float y, float z, float w) {
+      if (__builtin_expect(odd, 0)) x = saturate(x), y = saturate(y), z = saturate(z), w = saturate(w);
+      return encode4(x, y, z, w);
+    };
+    uint32_t keep = 0, older = 0;  // bytes of V's dwords that stay as they are; those of older rows
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = pc.row + i;
+      u32x2* w = reinterpret_cast<u32x2*>(kd + (long long)r * D + pc.dim);
+      if (r >= r0 && r < r1) {
+        const Raw8<SRC32>& x = kr8[p][i];
+        *w = u32x2{code4(x.get(0) * ku, x.get(1) * ku, x.get(2) * ku, x.get(3) * ku),
+                   code4(x.get(4) * ku, x.get(5) * ku, x.get(6) * ku, x.get(7) * ku)};
+      } else {
+        keep |= 0xffu << (8 * i);
+        if (r < r0) {
+          older |= 0xffu << (8 * i);
+          if (kratio < 1.f) *w = u32x2{rescale4(w->x, kratio), rescale4(w->y, kratio)};
+        }
       }
     }
-    *w = x;
+    if (keep == 0xffffffffu && !(older && vratio < 1.f)) continue;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t x = code4(vr8[p][0].get(e) * vu, vr8[p][1].get(e) * vu, vr8[p][2].get(e) * vu, vr8[p][3].get(e) * vu);
+      if (keep) {
+        const uint32_t o = vold[p][e], os = vratio < 1.f ? rescale4(o, vratio) : o;
+        x = (x & ~keep) | (os & older) | (o & keep & ~older);
+      }
+      *reinterpret_cast<uint32_t*>(vd + ((long long)(pc.dim + e) << c.lb) + pc.row) = x;
+    }
   }
 }
 
 // --------------------------------------------------------------- read back
-// One workgroup per (block, head, K or V), as the append.  Rows of missing
-// blocks, and rows before position 0, are written as zeros.
-__device__ __forceinline__ void decode8(u32x2 w, float s, float (&f)[8]) {
+// Rows of missing blocks, and rows before position 0, are written as zeros.
+__device__ __forceinline__ void decode4(uint32_t w, float s, float* f) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  f[0] = lo[0] * s, f[1] = lo[1] * s, f[2] = hi[0] * s, f[3] = hi[1] * s;
+}
+// 16 bytes of a row: 8 bf16 or 4 fp32.  Past the caches: nothing here reads
+// them again, and as ordinary stores they pushed out codes that were still to
+// be read (16 contexts of 512 to 4,096 into fp32, 377 MB: 94 us, now 67,
+// 5.6 TB/s).
+template <bool F32>
+__device__ __forceinline__ void put16(void* p, long long e, const float* f) {
+  u32x4 w;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
-    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
-    f[4 * i] = lo[0] * s, f[4 * i + 1] = lo[1] * s, f[4 * i + 2] = hi[0] * s, f[4 * i + 3] = hi[1] * s;
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (F32) w[i] = __float_as_uint(f[i]);
+    else w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{f[2 * i], f[2 * i + 1]}, bf16x2));
   }
+  u32x4* q = F32 ? reinterpret_cast<u32x4*>(static_cast<float*>(p) + e) : reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + e);
+  __builtin_nontemporal_store(w, q);
 }
 
 // The blocks of every row of a sequence, from position pos0 (rounded down to
@@ -368,43 +455,70 @@ __device__ __forceinline__ int blocks_spanned(const Seq& s, int lb) {
   return s.rows > 0 ? ((s.pos0 + s.rows - 1) >> lb) - (s.pos0 >> lb) + 1 : 0;
 }
 
+// Bytes 0..3 of the result: byte i of a, b, c, d.
+__device__ __forceinline__ uint32_t gather4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, (uint32_t)i | (uint32_t)(4 + i) << 8);
+  const uint32_t hi = __builtin_amdgcn_perm(d, c, (uint32_t)i | (uint32_t)(4 + i) << 8);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+
+// A workgroup takes `heads` heads of one block; a thread a piece at a time.
 template <int D, bool DST32>
-__global__ __launch_bounds__(256) void read_back(Cache c, Batch b, Rows kr, Rows vr) {
-  constexpr int TPR = D / 8, RPP = 256 / TPR;
-  __shared__ __align__(16) uint8_t tile[D * 128];
+__global__ __launch_bounds__(256) void read_back(Cache c, Batch b, Rows kr, Rows vr, int heads) {
   Seq s;
   int within;
-  const int head = (int)(blockIdx.x % (unsigned)c.n_kv);
-  if (!find_item(b, c.lb, (int)(blockIdx.x / (unsigned)c.n_kv), [&](const Seq& q) { return blocks_spanned(q, c.lb); },
-                 s, within))
-    return;
-  const bool is_v = blockIdx.y != 0;
-  const int B = 1 << c.lb, j = (s.pos0 >> c.lb) + within;
+  const unsigned sets = (unsigned)((c.n_kv + heads - 1) / heads);
+  if (!find_item(b, c.lb, (int)(blockIdx.x / sets), [&](const Seq& q) { return blocks_spanned(q, c.lb); }, s, within)) return;
+  const int B = 1 << c.lb, j = (s.pos0 >> c.lb) + within, h0 = (int)(blockIdx.x % sets) * heads;
   const int id = block_id(b, s.i, j, c.n_blocks);
   const int p0 = j * B, r0 = max(s.pos0 - p0, 0), r1 = min(s.pos0 + s.rows - p0, B);
-  const int live = min(max(s.len - p0, 0), B);  // rows of the block that hold positions
-  const Rows& dst = is_v ? vr : kr;
-  const long long off = ((long long)id * c.n_kv + head) * ((long long)D << c.lb);
-  const float sc = id >= 0 ? (is_v ? c.vs : c.ks)[(long long)id * c.n_kv + head] : 0.f;
-  if (is_v && id >= 0) {
-    for (int i = (int)threadIdx.x; i < D * B / 16; i += 256)
-      reinterpret_cast<u32x4*>(tile)[i] = reinterpret_cast<const u32x4*>(c.v + off)[i];
-  }
-  __syncthreads();
-  const int tr = (int)threadIdx.x / TPR, d0 = (int)threadIdx.x % TPR * 8;
-  for (int r = r0 + tr; r < r1; r += RPP) {
-    u32x2 w = u32x2{0, 0};
-    if (id >= 0 && r < live) {
-      if (is_v) {
+  const int live = id >= 0 ? min(max(s.len - p0, 0), B) : 0;  // rows of the block that hold positions
+  constexpr int W = DST32 ? 4 : 8, ND = W / 4;
+  const int lu = c.lb - 2 + (D == 64 ? 6 : 7) - (W == 8 ? 3 : 2);  // log2 of a head's pieces
+  const int n = min(heads, c.n_kv - h0) << lu;
+  for (int u = (int)threadIdx.x; u < n; u += 256) {
+    const int head = h0 + (u >> lu);
+    const Piece pc = piece_at<D, W>(u & ((1 << lu) - 1), c.lb);
+    if (pc.row + 4 <= r0 || pc.row >= r1) continue;
+    uint32_t kw[4][ND], vw[W];
+    float ks = 0.f, vs = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)tile[(d0 + i) * B + r] << (8 * (i & 3));
-      } else {
-        w = *reinterpret_cast<const u32x2*>(c.k + off + (long long)r * D + d0);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < ND; ++j) kw[i][j] = 0;
+#pragma unroll
+    for (int e = 0; e < W; ++e) vw[e] = 0;
+    if (pc.row < live) {  // the whole piece lies in the block; rows past `live` are dropped below
+      const long long at = (long long)id * c.n_kv + head;
+      const uint8_t *kp = c.k + (at * D << c.lb) + pc.row * D + pc.dim, *vp = c.v + (at * D << c.lb) + (pc.dim << c.lb) + pc.row;
+      ks = c.ks[at], vs = c.vs[at];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (W == 8) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(kp + i * D);
+          kw[i][0] = x.x, kw[i][ND - 1] = x.y;
+        } else {
+          kw[i][0] = *reinterpret_cast<const uint32_t*>(kp + i * D);
+        }
       }
+#pragma unroll
+      for (int e = 0; e < W; ++e) vw[e] = *reinterpret_cast<const uint32_t*>(vp + (e << c.lb));
     }
-    float f[8];
-    decode8(w, sc, f);
-    store8<DST32>(dst.p, (s.row0 + (long long)(p0 + r - s.pos0)) * dst.ts + head * dst.hs + d0, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = pc.row + i;
+      if (r < r0 || r >= r1) continue;
+      const bool is = r < live;
+      const long long row = s.row0 + (long long)(p0 + r - s.pos0);
+      float f[W];
+#pragma unroll
+      for (int j = 0; j < ND; ++j) decode4(is ? kw[i][j] : 0u, is ? ks : 0.f, f + 4 * j);
+      put16<DST32>(kr.p, row * kr.ts + head * kr.hs + pc.dim, f);
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+        decode4(is ? gather4(vw[4 * j], vw[4 * j + 1], vw[4 * j + 2], vw[4 * j + 3], i) : 0u, is ? vs : 0.f, f + 4 * j);
+      put16<DST32>(vr.p, row * vr.ts + head * vr.hs + pc.dim, f);
+    }
   }
 }
 
