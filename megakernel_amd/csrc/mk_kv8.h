@@ -670,6 +670,13 @@ struct Bool {
   static constexpr bool value = V;
 };
 
+// Weights are exp2(score - reference), where the reference is a row's maximum
+// so far, or up to 2^RISE less: sums take a new reference (a product for each
+// output held) only where the maximum has risen by more.  Weights of up to 2^8
+// lose nothing in bf16 and fp32, and a rise of some maximum of a wave's rows is
+// the rule for the first hundred steps.
+constexpr float RISE = 8.f;
+
 // Codes of the value NaN (0x7f, 0xff) in four bytes: 0x80 in each such byte.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -845,7 +852,7 @@ __global__ __launch_bounds__(W* kWave) void attn_rows(Attn p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) mt = fmaxf(mt, sc[i][j]);
     mt = max_xor32(max_xor16(mt)) * p.scale;
-    if (__any(mt > m)) {  // some row's maximum grows: its sums so far take the new one
+    if (__any(mt > m + RISE)) {
       const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       sum *= al;
@@ -938,14 +945,21 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void attn_tile(Attn p) {
-  constexpr int KC = D / 16, DB = D / 32;            // 16-dimension pieces of a K row, 32-dimension blocks of V
-  constexpr int KS = D + 8, VS = TILE + 8;           // LDS row strides
-  constexpr int NL = D * TILE / (256 * 16);          // 16-byte loads per thread of K, and of V
-  __shared__ __align__(16) uint16_t kl[2][TILE * KS];
-  __shared__ __align__(16) uint16_t vl[2][D * VS];
-  __shared__ unsigned long long nans[2][D];  // positions of a step whose V is NaN, by dimension
-  __shared__ int bad[2];                     // 1 + the step in the buffer, if nans has any
+struct TileLds {
+  static constexpr int KS = D + 8, VS = TILE + 8;  // row strides
+  uint16_t k[2][TILE * KS];
+  uint16_t v[2][D * VS];
+  unsigned long long nans[2][D];  // positions of a step whose V is NaN, by dimension
+  int bad[2];                     // 1 + the step in the buffer, if nans has any
+};
+
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_tile(Attn p) {
+  constexpr int KC = D / 16, DB = D / 32;    // 16-dimension pieces of a K row, 32-dimension blocks of V
+  constexpr int NL = D * TILE / (256 * 16);  // 16-byte loads per thread of K, and of V
+  typedef TileLds<D> Lds;
+  constexpr int KS = Lds::KS, VS = Lds::VS;
+  __shared__ __align__(16) Lds lds;
   const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
   const int head = (int)(blockIdx.x % (unsigned)p.c.n_kv);
   Item it;
@@ -957,6 +971,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile(Attn p) {
   const RowTile rows = row_tile(s, G, it.rt, TILE_ROWS);
   const int r0 = it.rt * TILE_ROWS, tiles = (rows.any + TILE - 1) / TILE;
   const int t0 = (int)((long long)tiles * it.split / it.ns), t1 = (int)((long long)tiles * (it.split + 1) / it.ns);
+  const int n = t1 - t0, end = min(s.len, t1 * TILE);
   const bool mine = 32 * wv + c < rows.n_rows;
   const int rr = mine ? r0 + 32 * wv + c : r0, tok = rr / G, hd = head * G + rr % G;
   const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
@@ -969,129 +984,170 @@ __global__ __launch_bounds__(256, 2) void attn_tile(Attn p) {
 #pragma unroll
     for (int k = 0; k < KC; ++k) qv[k] = *reinterpret_cast<const bf16x8*>(qp + 16 * k);
   }
-  // this thread's share of the staging: 16 dimensions of position kt + .., 16
-  // positions of dimension vd + ..
-  const int kt = tid / KC, kd = tid % KC * 16, vd = tid / 4, vp = tid % 4 * 16;
-  const int* row = p.b.table + (long long)s.i * p.b.width;
-  const int top = min(max(t1 * TILE - 1, 0) >> lb, p.b.width - 1);
+  // The staging is dealt so that what a wave loads at once lies in one run of
+  // 16 positions: one block, one scale, an address that is the wave's but for
+  // an offset that never changes.  K: positions kt + 256 / KC * i of a step,
+  // 16 dimensions; V: run wv, dimensions l and l + 64.
+  const int kt = tid / KC;
+  const unsigned ko = (unsigned)((kt & 15) * D + tid % KC * 16), vo = (unsigned)(l << lb);
   const unsigned bytes = (unsigned)(p.c.n_kv * D) << lb;  // of K or V of one block, all heads
   const uint8_t *kb = p.c.k + ((long long)head * D << lb), *vb = p.c.v + ((long long)head * D << lb);
   const float *ksb = p.c.ks + head, *vsb = p.c.vs + head;
-  const auto there = [&](int id, int pos) { return pos < s.len && id >= 0 && id < p.c.n_blocks; };
-  int idk[NL], idv;
-  const auto ids = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) idk[i] = row[min((t * TILE + kt + i * (256 / KC)) >> lb, top)];
-    idv = row[min((t * TILE + vp) >> lb, top)];
+  // Block ids of 16 steps, a run of 16 positions to each lane, and of the next
+  // 16 in the other of two; a bit for each run that is there.
+  const int* row = p.b.table + (long long)s.i * p.b.width;
+  const int top = min(max(end - 1, 0) >> lb, p.b.width - 1);
+  int tab0 = 0, tab1 = 0;
+  unsigned long long ok0 = 0, ok1 = 0;
+  const auto first_of = [&](int k) { return (t0 + k) * TILE; };
+  const auto window = [&](int w) {  // looks up the runs of steps 16w .. 16w + 15
+    const int pos = first_of(16 * w) + 16 * l;
+    return row[min(pos >> lb, top)];
   };
+  const auto judge = [&](int w, int& tab) {  // which of them are there; the others' place is taken by block 0
+    const bool ok = first_of(16 * w) + 16 * l < end && tab >= 0 && tab < p.c.n_blocks;
+    tab = ok ? tab : 0;
+    return __ballot(ok);
+  };
+  const auto id_of = [&](int k, int run) {
+    const int at = (k & 15) * 4 + run;
+    return (unsigned)__builtin_amdgcn_readlane(k & 16 ? tab1 : tab0, at);
+  };
+  const auto gone_of = [&](int k) { return ~(unsigned)((k & 16 ? ok1 : ok0) >> ((k & 15) * 4)) & 15u; };
   u32x4 kw[NL], vw[NL];
   float ks[NL], vs;
-  unsigned gone_next = 0;  // the loaded step's runs of 16 positions that are missing
-  const auto load = [&](int t) {
+  const auto load_k = [&](int k) {
+    const int first = first_of(k);
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int pos = t * TILE + kt + i * (256 / KC);
-      const bool ok = there(idk[i], pos);
-      const unsigned id = ok ? (unsigned)idk[i] : 0u;
-      kw[i] = *reinterpret_cast<const u32x4*>(kb + ((unsigned long long)id * bytes + (unsigned)((pos & off) * D + kd)));
+      const int run = (wv * (256 / KC / 4) + i * (256 / KC)) >> 4;
+      const unsigned id = id_of(k, run);
+      const uint8_t* base = kb + ((unsigned long long)id * bytes + (unsigned)(((first + 16 * run) & off & ~15) * D));
+      kw[i] = *reinterpret_cast<const u32x4*>(base + ko);
       ks[i] = ksb[(unsigned long long)id * (unsigned)p.c.n_kv];
     }
-    const int pos = t * TILE + vp;
-    const bool ok = there(idv, pos);
-    gone_next = (unsigned)__ballot(!ok) & 15u;
-    const unsigned id = ok ? (unsigned)idv : 0u;
+  };
+  const auto load_v = [&](int k) {
+    const unsigned id = id_of(k, wv);
+    const uint8_t* base = vb + ((unsigned long long)id * bytes + (unsigned)((first_of(k) + 16 * wv) & off));
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      vw[i] = *reinterpret_cast<const u32x4*>(vb + ((unsigned long long)id * bytes + (unsigned)(((vd + i * 64) << lb) + (pos & off))));
+    for (int i = 0; i < NL; ++i) vw[i] = *reinterpret_cast<const u32x4*>(base + (64u << lb) * i + vo);
     vs = vsb[(unsigned long long)id * (unsigned)p.c.n_kv];
-    // What no row may see is zero in V.  K needs nothing: its scores are
-    // replaced.
-    if ((t + 1) * TILE > s.len || !ok) {
-      const int n = ok ? s.len - pos : 0;  // positions of the 16 that exist
+  };
+  const auto stage_k = [&](int k) {
 #pragma unroll
-      for (int i = 0; i < NL; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int left = n - 4 * j;
-          vw[i][j] &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-        }
-      vs = ok ? vs : 1.f;
+    for (int i = 0; i < NL; ++i) {
+      const int j = kt + i * (256 / KC);
+      // position 32a + 16m + 8h + 4b + e goes to row 32a + 16m + 8b + 4h + e
+      const int r = (j & ~12) | (j & 8) >> 1 | (j & 4) << 1;
+      u32x4* w = reinterpret_cast<u32x4*>(&lds.k[k & 1][r * KS + tid % KC * 16]);
+      w[0] = fp8x8_to_bf16x8_scaled(u32x2{kw[i][0], kw[i][1]}, ks[i]);
+      w[1] = fp8x8_to_bf16x8_scaled(u32x2{kw[i][2], kw[i][3]}, ks[i]);
     }
   };
-  const auto stage = [&](int t, int buf) {
-    if ((t + 1) * TILE > rows.all) {
-      // Rows differ in what they see, and a NaN in V must not reach those that
-      // do not see it (0 * NaN): it is taken out and its place noted.
+  const auto stage_v = [&](int k) {
+    const int first = first_of(k);
+    if (first + TILE > rows.all || gone_of(k)) {
+      const int left = gone_of(k) >> wv & 1 ? 0 : opaque_v(end - first - 16 * wv);  // of the run's 16 positions
+      // What no row may see is zero.  Where rows differ in what they see, a
+      // NaN must not reach those that do not see it (0 * NaN): it is taken
+      // out and its place noted.
       uint32_t any = 0;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         uint32_t at = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t n = nan_bytes(vw[i][j]) >> 7;  // 1 in each NaN byte
-          at |= n * 0x10204080u >> 28 << (4 * j);
-          vw[i][j] &= ~(n * 0xffu);
+          const int y = left - 4 * j;
+          vw[i][j] &= y >= 4 ? 0xffffffffu : y <= 0 ? 0u : (1u << (8 * y)) - 1u;
+          const uint32_t nn = nan_bytes(vw[i][j]) >> 7;  // 1 in each NaN byte
+          at |= nn * 0x10204080u >> 28 << (4 * j);
+          vw[i][j] &= ~(nn * 0xffu);
         }
-        reinterpret_cast<uint16_t*>(&nans[buf][vd + i * 64])[vp / 16] = (uint16_t)at;
+        reinterpret_cast<uint16_t*>(&lds.nans[k & 1][l + i * 64])[wv] = (uint16_t)at;
         any |= at;
       }
-      if (any) bad[buf] = t + 1;
+      if (any) lds.bad[k & 1] = k + 1;
+      vs = left <= 0 ? 1.f : vs;  // block 0's scale may be anything
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int j = kt + i * (256 / KC);
-      // position 32a + 16m + 8h + 4b + e goes to row 32a + 16m + 8b + 4h + e
-      const int r = (j & ~12) | (j & 8) >> 1 | (j & 4) << 1;
-      u32x4* w = reinterpret_cast<u32x4*>(&kl[buf][r * KS + kd]);
-      w[0] = fp8x8_to_bf16x8_scaled(u32x2{kw[i][0], kw[i][1]}, ks[i]);
-      w[1] = fp8x8_to_bf16x8_scaled(u32x2{kw[i][2], kw[i][3]}, ks[i]);
-      u32x4* x = reinterpret_cast<u32x4*>(&vl[buf][(vd + i * 64) * VS + vp]);
+      u32x4* x = reinterpret_cast<u32x4*>(&lds.v[k & 1][(l + i * 64) * VS + 16 * wv]);
       x[0] = fp8x8_to_bf16x8_scaled(u32x2{vw[i][0], vw[i][1]}, vs);
       x[1] = fp8x8_to_bf16x8_scaled(u32x2{vw[i][2], vw[i][3]}, vs);
     }
   };
 
-  f32x16 o[DB];
+  f32x16 o[DB], sc[2];
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m = -INFINITY, sum = 0.f;
-  if (tid < 2) bad[tid] = 0;
-  if (t0 < t1) {
-    ids(t0);
-    load(t0);
-    ids(t0 + 1);
+  // Both halves in turn: a product that adds to the one before it waits twice
+  // as long as the unit takes.
+  const auto scores = [&](int k) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[a][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KC; ++j)
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+        sc[a] = mfma32(*reinterpret_cast<const bf16x8*>(&lds.k[k & 1][(32 * a + c) * KS + 16 * j + 8 * h]), qv[j], sc[a]);
+  };
+
+  // Step k's scores are there when its turn comes; its turn is: V of step
+  // k + 1 to bf16, the weights, step k + 1's scores, the product with V, K of
+  // step k + 2 to bf16.  What is staged was asked for a turn before.
+  if (tid < 2) lds.bad[tid] = 0;
+  if (n > 0) {
+    tab0 = window(0);
+    tab1 = window(1);
+    ok0 = judge(0, tab0);
+    ok1 = judge(1, tab1);
+    load_k(0);
+    load_v(0);
   }
   // q is waited for here: inside the loop the wait would stand in every step,
   // behind the next step's codes
 #pragma unroll
   for (int k = 0; k < KC; ++k) asm volatile("" : "+v"(qv[k]));
   __syncthreads();
-  if (t0 < t1) stage(t0, t0 & 1);
+  if (n > 0) {
+    stage_k(0);
+    load_k(1);
+    stage_v(0);
+  }
+  __syncthreads();
+  if (n > 0) {
+    scores(0);
+    stage_k(1);
+    load_k(2);
+    load_v(1);
+  }
   __syncthreads();
 
-  for (int t = t0; t < t1; ++t) {
-    const int buf = t & 1;
-    const unsigned gone = gone_next;
-    if (t + 1 < t1) {
-      load(t + 1);
-      ids(t + 2);
+  for (int k = 0; k < n; ++k) {
+    const int first = first_of(k), buf = k & 1;
+    const unsigned gone = gone_of(k);
+    // window w + 1, looked up and judged during window w, in the place of w - 1
+    if ((k & 15) == 12 && k > 16) {
+      if (k & 16) ok0 = judge((k >> 4) + 1, tab0);
+      else ok1 = judge((k >> 4) + 1, tab1);
     }
-    f32x16 sc[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[a][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KC; ++k)
-        sc[a] = mfma32(*reinterpret_cast<const bf16x8*>(&kl[buf][(32 * a + c) * KS + 16 * k + 8 * h]), qv[k], sc[a]);
+    stage_v(k + 1);
+    load_v(k + 2);
+    if ((k & 15) == 1 && k > 16) {
+      const int x = window((k >> 4) + 1);
+      if (k & 16) tab0 = x;
+      else tab1 = x;
     }
     // score i of half a: position 32a + 16(i/8) + 8h + i%8 of the step
-    const bool masked = (t + 1) * TILE > all || gone;
-    if (masked) {
+    if (first + TILE > all || gone) {
       // opaque: a branch for the few steps that need it, not its 64 selects in every step
-      const int lim = opaque_v(see - t * TILE - 8 * h);
+      const int lim = opaque_v(see - first - 8 * h);
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -1104,7 +1160,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile(Attn p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[a][i]);
     mt = max_xor32(mt) * p.scale;
-    if (__any(mt > m)) {  // some row's maximum grows: its sums so far take the new one
+    if (__any(mt > m + RISE)) {
       const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       sum *= al;
@@ -1114,38 +1170,45 @@ __global__ __launch_bounds__(256, 2) void attn_tile(Attn p) {
         for (int i = 0; i < 16; ++i) o[d][i] *= al;
     }
     const float mref = m == -INFINITY ? 0.f : m;
-    bf16x8 pb[2][2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], p.scale, -mref));
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], p.scale, -mref));
-        sum += x + y;
-        const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
-        pb[a][i / 8][i % 8] = w[0];
-        pb[a][i / 8][i % 8 + 1] = w[1];
-      }
-    if (__builtin_expect((t + 1) * TILE > rows.all && bad[buf] == t + 1, 0)) {
-      // the NaN that stage() took out of V, put into the rows that see them
-      const int n = min(max(see - t * TILE, 0), TILE);
-      unsigned long long seen = n < 64 ? (1ull << n) - 1ull : ~0ull;
+    if (__builtin_expect(first + TILE > rows.all && lds.bad[buf] == k + 1, 0)) {
+      // the NaN that stage_v() took out, put into the rows that see them
+      const int x = min(max(see - first, 0), TILE);
+      unsigned long long seen = x < 64 ? (1ull << x) - 1ull : ~0ull;
 #pragma unroll
       for (int i = 0; i < 4; ++i) seen &= gone >> i & 1 ? ~(0xffffull << (16 * i)) : ~0ull;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (nans[buf][32 * d + 8 * (i / 4) + 4 * h + i % 4] & seen) o[d][i] = NAN;
+          if (lds.nans[buf][32 * d + 8 * (i / 4) + 4 * h + i % 4] & seen) o[d][i] = NAN;
     }
+    const bf16x2 one = bf16x2{(__bf16)1.f, (__bf16)1.f};
+    bf16x8 pb[2][2];
+    const auto weights = [&](int a) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+      for (int i = 0; i < 16; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], p.scale, -mref));
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], p.scale, -mref));
+        const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
+        sum = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum, false);  // of the weights as V's product has them
+        pb[a][i / 8][i % 8] = w[0];
+        pb[a][i / 8][i % 8 + 1] = w[1];
+      }
+    };
+    const auto add_v = [&](int a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int d = 0; d < DB; ++d)
-          o[d] = mfma32(*reinterpret_cast<const bf16x8*>(&vl[buf][(32 * d + c) * VS + 32 * a + 16 * i + 8 * h]), pb[a][i], o[d]);
-    if (t + 1 < t1) stage(t + 1, buf ^ 1);
+          o[d] = mfma32(*reinterpret_cast<const bf16x8*>(&lds.v[buf][(32 * d + c) * VS + 32 * a + 16 * i + 8 * h]), pb[a][i], o[d]);
+    };
+    weights(0);
+    weights(1);
+    scores(k + 1);  // of the last step, of nothing: not used
+    add_v(0);
+    add_v(1);
+    stage_k(k + 2);
+    load_k(k + 3);
     __syncthreads();
   }
   sum = sum_xor32(sum);
