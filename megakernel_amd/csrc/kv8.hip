@@ -166,10 +166,13 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
   // (256 rows at 16,000: 55 / 46; 512: 80 / 64; 512 at 2,100: 17 / 31).  Many
   // sequences share the chip, so their rows count together.
   const long long even = (d64 ? 8 << 17 : 8 * 49152) / ((long long)b->n_seq * c->n_kv * steps + 1);
-  const int few = (int)(even < 64 ? 64 : even > 1024 ? 1024 : even);
+  int few = (int)(even < 64 ? 64 : even > 1024 ? 1024 : even);
   if (b->n_seq == 1) p.use[rows > few] = true;
   else if (rows <= few || rows <= 32ll * b->n_seq) p.use[FEW] = true;
-  else p.use[FEW] = p.use[MANY] = true;
+  else {  // both, and a workgroup for every row tile that may be there: not too many that are not
+    p.use[FEW] = p.use[MANY] = true;
+    if (few > 128) few = 128;
+  }
   p.few = !p.use[MANY] ? 0x7fffffff : !p.use[FEW] ? 0 : few;
   p.lr[FEW] = 4, p.lr[MANY] = 7;
   p.least[FEW] = 8, p.least[MANY] = 4;
@@ -401,17 +404,16 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
     ws += part_bytes(pl, k, cache->n_kv, cache->head_dim);
   }
   const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv, joins = (long long)batch->n_tokens * n_q;
-  if (!grid_ok(op, few * 2) || !grid_ok(op, many) || !grid_ok(op, joins)) return -1;
+  if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
   auto go = [&](auto kern, long long groups, int threads) {
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(threads), 0, st, p);
   };
-  if (pl.use[MANY]) d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
-  if (pl.use[FEW]) {
-    if (pl.waves == 4) d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
-    else d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
-  }
+  if (pl.use[FEW] && pl.use[MANY]) d64 ? go(attn_both<64>, many + few, 256) : go(attn_both<128>, many + few, 256);
+  else if (pl.use[MANY]) d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
+  else if (pl.waves == 4) d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
+  else d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
   // a workgroup for every row, or where rows are many a wave for four (verify of
   // 1,152 rows 41.0 / 43.6 us in all, a prompt of 16,384 336 / 315)
   if (need && joins <= 4096) d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);

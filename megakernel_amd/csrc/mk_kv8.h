@@ -706,14 +706,21 @@ struct Ids {
 // dimension are the lane's 16-byte V load, which makes the weights the B
 // operand as they stand.
 template <int D, int W>
-__global__ __launch_bounds__(W* kWave) void attn_rows(Attn p) {
+struct RowsLds {
+  float lo[W][ROWS][D + 4];
+  float lm[W][ROWS], ls[W][ROWS];
+};
+
+template <int D, int W>
+__device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   constexpr int KH = D / 64, DT = D / 16;  // 64-dimension halves of K, 16-dimension tiles of V
-  __shared__ float lm[W][ROWS], ls[W][ROWS];
-  __shared__ float lo[W][ROWS][D + 4];
+  RowsLds<D, W>& lds = *static_cast<RowsLds<D, W>*>(smem);
+  auto &lm = lds.lm, &ls = lds.ls;
+  auto& lo = lds.lo;
   const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
-  const int head = (int)(blockIdx.x % (unsigned)p.c.n_kv);
+  const int head = item % p.c.n_kv;
   Item it;
-  if (!find_split<FEW>(p, (int)(blockIdx.x / (unsigned)p.c.n_kv), it)) return;
+  if (!find_split<FEW>(p, item / p.c.n_kv, it)) return;
   const Seq& s = it.s;
   const int l = (int)(threadIdx.x & 63u), wv = wave_id();
   const int c = l & 15, g = l >> 4;  // this lane's query row; its 16 positions of a step
@@ -954,17 +961,17 @@ struct TileLds {
 };
 
 template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_tile(Attn p) {
+__device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   constexpr int KC = D / 16, DB = D / 32;    // 16-dimension pieces of a K row, 32-dimension blocks of V
   constexpr int NL = D * TILE / (256 * 16);  // 16-byte loads per thread of K, and of V
   typedef TileLds<D> Lds;
   constexpr int KS = Lds::KS, VS = Lds::VS;
-  __shared__ __align__(16) Lds lds;
+  Lds& lds = *static_cast<Lds*>(smem);
   const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
-  const int head = (int)(blockIdx.x % (unsigned)p.c.n_kv);
+  const int head = item % p.c.n_kv;
   Item it;
   // the last items first: a prompt's last row tiles have the most positions
-  if (!find_split<MANY>(p, p.d[MANY].items - 1 - (int)(blockIdx.x / (unsigned)p.c.n_kv), it)) return;
+  if (!find_split<MANY>(p, p.d[MANY].items - 1 - item / p.c.n_kv, it)) return;
   const Seq& s = it.s;
   const int l = (int)(threadIdx.x & 63u), wv = wave_id(), tid = (int)threadIdx.x;
   const int c = l & 31, h = l >> 5;
@@ -1236,6 +1243,29 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_tile(Attn p) {
         *reinterpret_cast<f32x4*>(pp + 32 * d + 8 * b) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
     if (h == 0) p.d[MANY].ml[at] = make_float2(m, sum);
   }
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(W* kWave) void attn_rows(Attn p) {
+  __shared__ __align__(16) RowsLds<D, W> lds;
+  rows_item<D, W>(p, (int)blockIdx.x, &lds);
+}
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_tile(Attn p) {
+  __shared__ __align__(16) TileLds<D> lds;
+  tile_item<D>(p, (int)blockIdx.x, &lds);
+}
+// Batches with sequences of both kinds: one launch, so that neither waits for
+// the other's last workgroup; the tiles first, they take longest.
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_both(Attn p) {
+  __shared__ __align__(16) union {
+    TileLds<D> t;
+    RowsLds<D, 4> r;
+  } lds;
+  const int many = p.d[MANY].items * p.c.n_kv;
+  if ((int)blockIdx.x < many) tile_item<D>(p, (int)blockIdx.x, &lds);
+  else rows_item<D, 4>(p, (int)blockIdx.x - many, &lds);
 }
 
 // Where a row's partials are.

@@ -77,16 +77,17 @@ def _rows(t, shape, device: int, name: str, types=_TYPES) -> bytes:
     """Rows [tokens][heads][dim] with any token and head stride, as a
     megakernel_rows."""
     typ = types.get(t.dtype)
-    if typ is None or t.shape != shape or t.get_device() != device or t.stride(2) != 1:
+    if typ is None or t.shape != shape or t.get_device() != device:
         if typ is None:
             raise ValueError(f"{name} must be {' or '.join(str(x)[6:] for x in types)}, not {t.dtype}")
         if t.shape != shape:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
-        if t.get_device() != device:
-            raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
-        raise ValueError(f"the last dimension of {name} must be contiguous (stride {t.stride(2)})")
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+    token, head, last = t.stride()
+    if last != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous (stride {last})")
     # of a single token or head, the stride says nothing
-    return _pack_rows(t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0, typ)
+    return _pack_rows(t.data_ptr(), token if shape[0] > 1 else 0, head if shape[1] > 1 else 0, typ)
 
 
 _library = None
