@@ -484,9 +484,9 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
  * to nearest even.  Where the scale grows, the older rows' codes are rounded
  * again from their values.  Infinities do not count for the scale and become
  * +-448 s; NaN stays NaN.  Rows whose block is missing or whose position is
- * negative are dropped.  Other rows of a block are left as they were.  Rows
- * given to one block by two sequences of a call are a race; blocks that
- * nothing is appended to may be shared. */
+ * negative are dropped.  Other rows of a block are left as they were.  A block
+ * that a call appends to may stand in one table entry only, of one sequence;
+ * blocks that nothing is appended to may be shared. */
 int megakernel_op_kv8_append(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                              const megakernel_rows* k, const megakernel_rows* v, void* stream);
 
@@ -503,7 +503,8 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
  * scores, the softmax and the sums are fp32, the weights are rounded to bf16
  * for the product with V.  workspace: megakernel_op_kv8_workspace_bytes(...)
  * bytes (NULL where that is 0), 16-byte aligned, without an initial value;
- * calls that may overlap in time need one each. */
+ * calls that may overlap in time need one each.  out may not overlap q or the
+ * cache.  n_tokens * (n_q / n_kv) is at most 2^30. */
 long long megakernel_op_kv8_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, int n_q);
 int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                                 const megakernel_rows* q, const megakernel_rows* out, int n_q, float scale,

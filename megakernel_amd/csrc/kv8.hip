@@ -375,6 +375,10 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
     set_err("%s: out must not be q", op);
     return -1;
   }
+  if ((long long)batch->n_tokens * (n_q / cache->n_kv) > (1ll << 30)) {
+    set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows", op, batch->n_tokens, n_q / cache->n_kv);
+    return -1;
+  }
   if (!(scale > 0.f && scale < INFINITY)) {
     set_err("%s: scale=%g must be positive and finite", op, scale);
     return -1;
@@ -403,7 +407,11 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
     d.ml = reinterpret_cast<float2*>(d.part + part_floats(pl, k, cache->n_kv, cache->head_dim));
     ws += part_bytes(pl, k, cache->n_kv, cache->head_dim);
   }
-  const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv, joins = (long long)batch->n_tokens * n_q;
+  const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv;
+  // tokens whose rows may have splits to join
+  long long tokens = batch->n_tokens;
+  if (!pl.target[MANY] && pl.use[MANY] && tokens > (long long)batch->n_seq * (pl.few / p.group)) tokens = (long long)batch->n_seq * (pl.few / p.group);
+  const long long joins = tokens * n_q;
   if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
@@ -418,7 +426,7 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   // 1,152 rows 41.0 / 43.6 us in all, a prompt of 16,384 336 / 315)
   if (need && joins <= 4096) d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
   else if (need) {
-    const long long waves = (long long)batch->n_tokens * ((n_q + 3) / 4);
+    const long long waves = tokens * ((n_q + 3) / 4);
     d64 ? go(attn_join_waves<64, 4>, (waves + 3) / 4, 256) : go(attn_join_waves<128, 4>, (waves + 3) / 4, 256);
   }
   return launched(op);

@@ -614,8 +614,9 @@ __device__ __forceinline__ int steps_per_item(const Attn& p, int kind, const Seq
 // a sequence of k row tiles and n steps gets k * ceil(n / part) of them.
 // There are at most target + (row tiles) items, and 2 * target partials: a
 // sequence that is split at all has more than one part.
-// Finds item `it` of a kernel, or with kind -1 the item that holds row `it`
-// of all sequences' rows (r.rt is then the row's token within its sequence).
+// Finds item `it` of a kernel, or with kind -1 the item that holds token `it`
+// of all tokens of kernels that split (r.rt is then the token's number within
+// its sequence).
 template <int KIND>
 __device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
   const int G = p.group;
@@ -626,7 +627,7 @@ __device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
     const Seq q = base ? lane_seq(p, base) : first;
     const int kind = kind_of(p, q);
     int c = 0, s0 = 0, s1 = 0, ns = 1;
-    if (KIND < 0 || kind == KIND) {
+    if (KIND < 0 ? (kind ? p.d[1].target : p.d[0].target) != 0 : kind == KIND) {
       const int per = kind ? per1 : per0;
       const int rt = row_tiles(q, G, kind ? p.d[1].lr : p.d[0].lr), n = most_steps(q);
       ns = min(max(n / per + (n % per != 0), 1), kMaxSplits);
@@ -1177,7 +1178,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
         for (int i = 0; i < 16; ++i) o[d][i] *= al;
     }
     const float mref = m == -INFINITY ? 0.f : m;
-    if (__builtin_expect(first + TILE > rows.all && lds.bad[buf] == k + 1, 0)) {
+    if (__builtin_expect((first + TILE > rows.all || gone) && lds.bad[buf] == k + 1, 0)) {
       // the NaN that stage_v() took out, put into the rows that see them
       const int x = min(max(see - first, 0), TILE);
       unsigned long long seen = x < 64 ? (1ull << x) - 1ull : ~0ull;

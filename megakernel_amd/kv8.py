@@ -202,8 +202,8 @@ def append(cache: Cache, batch: Batch, k, v):
     """Quantise rows k, v [n_tokens][n_kv][head_dim] (bf16 or fp32) into their
     blocks.  A block and head has one scale, the smallest power of two that
     fits its rows into e4m3; rows that a block already holds are rounded again
-    where a new row makes its scale grow.  Two sequences of one call may not
-    append to the same block."""
+    where a new row makes its scale grow.  A block that a call appends to may
+    stand in one table entry only."""
     _one_gpu(cache, batch)
     shape = (batch.n_tokens, cache.n_kv, cache.head_dim)
     a, b = _rows(k, shape, cache.device, "k"), _rows(v, shape, cache.device, "v")

@@ -91,21 +91,22 @@ class Pool:
         group = q.shape[1] // self.n_kv
         size, reach = np.zeros(out.shape), np.zeros(out.shape[:2])
         for i in range(len(length)):
+            at = [(j, self.place(table[i], j)) for j in range(max(0, int(length[i])))]
+            there = [(j, *self.values(*a)) for j, a in at if a]
+            pos = np.array([x[0] for x in there])
+            keys, vals = (np.stack([x[k] for x in there]) if there else None for k in (1, 2))
             for t in range(start[i], start[i + 1]):
-                p = int(length[i]) - int(start[i + 1]) + t
-                at = [self.place(table[i], j) for j in range(max(0, p + 1))]
-                kv = [self.values(*a) for a in at if a]
+                n = int((pos <= int(length[i]) - int(start[i + 1]) + t).sum()) if there else 0
+                if n == 0:
+                    out[t] = 0.0
+                    continue
                 for h in range(q.shape[1]):
-                    if not kv:
-                        out[t, h] = 0.0
-                        continue
-                    k = np.stack([x[0][h // group] for x in kv])
-                    v = np.stack([x[1][h // group] for x in kv])
+                    k, v = keys[:n, h // group], vals[:n, h // group]
                     s = k @ q[t, h] * scale
                     w = np.exp(s - s.max())
                     w /= w.sum()
-                    out[t, h] = (w[:, None] * v).sum(0)
-                    size[t, h] = (w[:, None] * np.abs(v)).sum(0)
+                    out[t, h] = w @ v
+                    size[t, h] = w @ np.abs(v)
                     reach[t, h] = (np.abs(k) @ np.abs(q[t, h])).max() * scale
         return size, reach
 

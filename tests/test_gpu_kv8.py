@@ -524,3 +524,234 @@ def test_empty_batches():
     kv8.append(c.cache, c.batch, k, k)
     kv8.read(c.cache, c.batch, k, torch.empty_like(k))
     kv8.attention(c.cache, c.batch, q, torch.empty_like(q))
+
+
+# --------------------------------------- splits, both kernels, many sequences
+def _hint(c: Case, max_kv: int):
+    c.batch = kv8.Batch(c.batch.table, c.batch.q_start, c.batch.kv_len, c.tokens, max_kv)
+    return c
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("missing", [0.0, 0.2])
+def test_attention_splits(dim, missing):
+    """Contexts long enough that few rows are split, among short, empty and
+    ragged ones; the workspace is needed, and its initial value does not matter."""
+    for block, n_kv, group, lens, new in ((32, 1, 2, [4200], [1]), (16, 2, 3, [4100, 30, 2500, 0, 700], [1, 3, 7, 0, 2]),
+                                          (128, 1, 16, [5000, 4999], [2, 1])):
+        _say(f"attention splits D={dim} block {block} {lens} {new} missing {missing}")
+        c = Case(block, n_kv, dim, lens, new, seed=dim + block, missing=missing)
+        need = kv8.workspace_bytes(c.cache, c.batch, n_kv * group)
+        assert need > 0
+        ws = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")  # NaN, in any reading
+        _, out = _check_attention(c, n_kv * group, say=str(lens), workspace=ws)
+        c.rng = np.random.default_rng(5)
+        q = c.rows(n_kv * group, torch.bfloat16).cuda()
+        a, b = torch.empty_like(q), torch.empty_like(q)
+        kv8.attention(c.cache, c.batch, q, a, workspace=ws)
+        kv8.attention(c.cache, c.batch, q, b)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)  # the same sums in the same order
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hint", [64, 0])
+def test_attention_of_many_rows_over_many_steps(dim, hint):
+    """A prompt's last tokens over a context of more steps than a look-up of
+    block ids covers, whole (a hint that is far too short) and split."""
+    block, lens, new = 16, [2710], [131]
+    _say(f"attention many steps D={dim} hint {hint}")
+    c = _hint(Case(block, 1, dim, lens, new, seed=dim, missing=0.05), hint)
+    assert (kv8.workspace_bytes(c.cache, c.batch, 8) > 0) == (hint == 0)
+    _check_attention(c, 8)
+
+
+def test_attention_of_many_rows_joined_by_waves():
+    """More rows than a workgroup each."""
+    _say("attention joined by waves")
+    c = Case(64, 2, 64, [900], [300], seed=31)
+    assert kv8.workspace_bytes(c.cache, c.batch, 16) > 0 and c.tokens * 16 > 4096
+    _check_attention(c, 16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_a_mixed_batch(dim):
+    """Single tokens next to prompts, long and short contexts of each."""
+    lens, new = [4300, 600, 40, 1500, 0, 300, 2100], [1, 250, 40, 3, 0, 1, 90]
+    _say(f"attention mixed D={dim}")
+    for hint in (0, 64):
+        c = _hint(Case(32, 1, dim, lens, new, seed=33, missing=0.03, gap=2), hint)
+        _check_attention(c, 2, say=f"hint {hint}")
+
+
+def test_more_sequences_than_a_wave_has_lanes():
+    _say("150 sequences")
+    rng = np.random.default_rng(34)
+    lens = [int(x) for x in rng.integers(0, 90, 150)]
+    new = [min(n, int(x)) for n, x in zip(lens, rng.integers(0, 6, 150))]
+    lens[70], new[70], lens[130], new[130] = 700, 300, 2600, 1
+    c = Case(16, 2, 64, lens, new, seed=35, gap=1)
+    k, v = c.rows(2, torch.bfloat16), c.rows(2, torch.bfloat16)
+    c.pool.append(c.table, c.start, c.lens, _f64(k), _f64(v))
+    kv8.append(c.cache, c.batch, k.cuda(), v.cuda())
+    torch.cuda.synchronize()
+    c.same_pool()
+    _check_attention(c, 4)
+    want = [np.full((c.tokens, 2, 64), 7.0) for _ in range(2)]
+    c.pool.read(c.table, c.start, c.lens, *want)
+    got = [torch.full((c.tokens, 2, 64), 7.0, device="cuda") for _ in range(2)]
+    kv8.read(c.cache, c.batch, *got)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        np.testing.assert_array_equal(_f64(g), w)
+
+
+@pytest.mark.parametrize("n_tokens", [2, 40])
+def test_graphs_of_split_contexts(n_tokens):
+    """Two captured calls, each with the workspace it took, replayed in turn
+    and on two streams at once, against the eager call."""
+    _say(f"graphs of splits, {n_tokens} tokens")
+    cs = [Case(32, 2, 64, [4500], [n_tokens], seed=s) for s in (36, 37)]
+    qs = [c.rows(8, torch.bfloat16).cuda() for c in cs]
+    assert all(kv8.workspace_bytes(c.cache, c.batch, 8) > 0 for c in cs)
+    want, outs, graphs = [], [], []
+    for c, q in zip(cs, qs):
+        o = torch.empty_like(q)
+        kv8.attention(c.cache, c.batch, q, o)
+        torch.cuda.synchronize()
+        want.append(o.clone())
+        out = torch.empty_like(q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            kv8.attention(c.cache, c.batch, q, out)
+        outs.append(out)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in cs]
+    for step in range(6):
+        for s, g, o in zip(streams, graphs, outs):
+            with torch.cuda.stream(s):
+                o.fill_(float("nan"))
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w), f"replay {step}"
+        eager = torch.empty_like(qs[0])
+        kv8.attention(cs[0].cache, cs[0].batch, qs[0], eager)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0])
+
+
+def test_kv8_on_a_side_stream_behind_its_inputs():
+    """A stream that waits for the one that wrote the inputs, as with torch's own operators."""
+    _say("side stream")
+    c = Case(32, 2, 64, [4400], [1], seed=38)
+    q = c.rows(4, torch.bfloat16).cuda()
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    kv8.attention(c.cache, c.batch, q, want)
+    side = torch.cuda.Stream()
+    late = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    for _ in range(8):
+        late.zero_()
+        late.add_(q)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            kv8.attention(c.cache, c.batch, late, got)
+        torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+# Which kernel takes a sequence goes by its rows and by the context lengths
+# that a batch announces: announced as long, these go to the one for many rows
+# (split); announced as short, only where the rows are over 1,024.
+TILED = [
+    # block, n_kv, group, dim, lens, new
+    (16, 2, 3, 64, [90, 40, 17], [90, 33, 5]),
+    (64, 1, 2, 128, [150, 66, 3], [140, 1, 3]),
+    (128, 1, 1, 128, [257], [257]),
+    (32, 1, 8, 64, [300], [64]),
+    (32, 1, 16, 128, [300, 5, 80], [70, 1, 3]),
+    (16, 1, 16, 64, [100, 1100], [66, 33]),
+    (64, 2, 4, 64, [600, 0, 129], [300, 0, 129]),
+    (128, 1, 3, 64, [1, 500, 64], [1, 400, 64]),
+]
+
+
+@pytest.mark.parametrize("hint", [64, 1 << 20])
+@pytest.mark.parametrize("missing", [0.0, 0.3])
+@pytest.mark.parametrize("case", TILED, ids=[f"b{c[0]}h{c[1]}g{c[2]}d{c[3]}n{sum(c[5])}" for c in TILED])
+def test_attention_tiles(case, missing, hint):
+    block, n_kv, group, dim, lens, new = case
+    _say(f"attention tiles {case} missing {missing} hint {hint}")
+    c = _hint(Case(block, n_kv, dim, lens, new, seed=block * dim + sum(lens), missing=missing, gap=1), hint)
+    _check_attention(c, n_kv * group)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hint,group", [(1 << 20, 2), (64, 30)])
+def test_attention_tiles_never_see_what_they_may_not(dim, hint, group):
+    """As the rows' test: NaN in unused blocks, behind the last row, and in
+    positions that only some rows of a tile see."""
+    _say(f"attention tiles NaN D={dim} hint {hint}")
+    c = Case(16, 2, dim, [190, 33, 70], [140, 33, 40], seed=9, missing=0.2)
+    used = {int(b) for row, n in zip(c.table, c.lens) for j, b in enumerate(row) if j < -(-int(n) // 16) and 0 <= b < c.pool.n_blocks}
+    for b in range(c.pool.n_blocks):
+        if b not in used:
+            c.pool.k[b], c.pool.v[b] = 0x7F, 0xFF
+            c.pool.ks[b], c.pool.vs[b] = np.nan, np.inf
+    for row, n in zip(c.table, c.lens):
+        b, r = int(row[(n - 1) // 16]), int(n) % 16
+        if r and 0 <= b < c.pool.n_blocks:
+            c.pool.k[b, :, r:], c.pool.v[b, :, :, r:] = 0xFF, 0x7F
+    ks, vs = c.pool.ks.copy(), c.pool.vs.copy()
+
+    def check(nan_ok):
+        c.upload()
+        _hint(c, hint)
+        c.pool.vs[:] = np.where(np.isfinite(vs), vs, 0)  # the tolerance's, of what is seen
+        out = _check_attention(c, 2 * group, nan_ok=nan_ok)[1]
+        c.pool.ks[:], c.pool.vs[:] = ks, vs
+        return out
+
+    check(False)
+    at = next(p for p in range(100, 180) if c.pool.place(c.table[0], p))  # rows from at - 50 on see it
+    b, r = c.pool.place(c.table[0], at)
+    c.pool.v[b, 1, 5, r] = 0x7F
+    c.pool.v[b, 1, dim - 1, r] = 0xFF
+    b1, r1 = c.pool.place(c.table[1], next(p for p in range(3, 33) if c.pool.place(c.table[1], p)))
+    c.pool.v[b1, 0, 9, r1] = 0xFF
+    out = check(True)
+    assert torch.isnan(out[at - 50, 2 * group - 1, 5]) and torch.isnan(out[139, group, dim - 1])
+    assert not torch.isnan(out[: at - 50]).any() and not torch.isnan(out[:140, :group]).any()
+    c.pool.k[b, 0, r, 7] = 0x7F  # a NaN key makes the whole row NaN
+    out = check(True)
+    assert torch.isnan(out[at - 50 : 140, :group]).all() and not torch.isnan(out[: at - 50]).any()
+
+
+def test_attention_tiles_extremes():
+    _say("attention tiles extremes")
+    c = Case(32, 2, 64, [150, 80], [100, 20], seed=10)
+    for ke, ve, qs in ((9, 100, 3.0), (-100, -100, 1.0), (20, 0, 1e-3)):
+        c.pool.ks[:], c.pool.vs[:] = 2.0 ** ke, 2.0 ** ve
+        c.upload()
+        _hint(c, 1 << 20)
+        q = c.rows(4, torch.bfloat16, qs)
+        _check_attention(c, 4, scale=2.0 ** -10 if ke == 9 else None, q=q, say=f"{ke} {ve}")
+
+
+def test_attention_tiles_negative_positions_and_rising_maxima():
+    """Rows that see nothing in a tile of rows that do; keys that grow with the
+    position, so that the running maximum rises at every step."""
+    _say("attention tiles negative positions")
+    c = Case(16, 1, 64, [50, 700], [90, 300], seed=40)
+    for row, n in zip(c.table, c.lens):
+        for p in range(int(n)):
+            b, r = c.pool.place(row, p)
+            c.pool.k[b, :, r] = 0x38
+            c.pool.ks[b] = 2.0 ** (p // 16 // 4 - 8)
+    c.upload()
+    _hint(c, 1 << 20)
+    q = c.rows(3, torch.bfloat16, 0.5) + 0.25
+    _, out = _check_attention(c, 3, q=q)
+    assert torch.all(out[:40] == 0)

@@ -159,6 +159,7 @@ def test_other_refusals(clib):
     _refused(clib, att(c, b, r, far, 0, 1.0, None, 0, None), "n_q=0")
     _refused(clib, att(c, b, r, r, 8, 1.0, None, 0, None), "must not be q")
     _refused(clib, att(c, b, f32, far, 8, 1.0, None, 0, None), "bf16 only")
+    _refused(clib, att(_ref(_cache(n_kv=1)), _ref(_batch(n_tokens=1 << 27)), _ref(_r(ts=1024)), _ref(_r(2 * FAKE, ts=1024)), 16, 1.0, None, 0, None), "2^30")
     _refused(clib, att(c, b, r, _ref(_r(2 * FAKE, type=0)), 8, 1.0, None, 0, None), "bf16 only")
     for scale in (0.0, -1.0, float("inf"), float("nan")):
         _refused(clib, att(c, b, r, far, 8, scale, None, 0, None), "scale")
