@@ -459,7 +459,7 @@ typedef struct {
  * outside [0, n_blocks) are missing blocks, as are positions past the table.
  * n_tokens: rows of the row tensors.  max_kv: no bound, only how long
  * contexts are expected to get (0: table_width * block), from which the
- * attention chooses how far it splits them. */
+ * attention chooses its kernels and how far it splits them. */
 typedef struct {
   const int* table;
   const int* q_start;

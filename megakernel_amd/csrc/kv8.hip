@@ -158,49 +158,74 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
   const bool d64 = c->head_dim == 64;
   const long long rows = (long long)b->n_tokens * group;
   const long long kv = b->max_kv ? b->max_kv : (long long)b->table_width * c->block, steps = (kv + TILE - 1) / TILE;
-  // Which kernel takes a sequence.  attn_rows reads a context once for every
-  // 16 rows but starts fast; attn_tile has the rate for large products and
-  // takes 15 us more to get there.  Rows x steps of a KV head at which they
-  // were even, 8 heads at 2,100 and 16,000 positions: 128 Ki for head_dim 64
-  // (512 rows at 16,000: 45 / 46 us; 1,024 at 2,100: 18 / 30), 48 Ki for 128
-  // (256 rows at 16,000: 55 / 46; 512: 80 / 64; 512 at 2,100: 17 / 31).  Many
-  // sequences share the chip, so their rows count together.
-  const long long even = (d64 ? 8 << 17 : 8 * 49152) / ((long long)b->n_seq * c->n_kv * steps + 1);
-  int few = (int)(even < 64 ? 64 : even > 1024 ? 1024 : even);
-  if (b->n_seq == 1) p.use[rows > few] = true;
-  else if (rows <= few || rows <= 32ll * b->n_seq) p.use[FEW] = true;
-  else {  // both, and a workgroup for every row tile that may be there: not too many that are not
-    p.use[FEW] = p.use[MANY] = true;
-    if (few > 128) few = 128;
+  // Which kernel takes a batch.  attn_rows reads a context once for every 16
+  // rows but starts fast; attn_tile has two to three times the rate once its
+  // 128-row tiles fill the chip, and before that waits for its longest tile, or
+  // for the join of splits.  They are even at nearly as many rows as give every
+  // CU a tile (head_dim 128: two CUs of three), or at fewer that work longer.
+  // us of attn_rows / attn_tile, 8 KV heads: head_dim 64, 4,096 rows without a
+  // past in one sequence 37 / 41, in four 18 / 16, in 16 11 / 10, with 1,000
+  // positions before them in four 37 / 35; 2,048 rows after 4,000 53 / 57,
+  // 1,024 after 8,000 47 / 51, 512 after 16,000 44 / 51, 1,024 76 / 71; 128:
+  // 2,048 rows in one sequence 23 / 33, in two 16 / 21, in four 13 / 15, 4,096
+  // 58 / 57, 34 / 34, 29 / 23; 1,024 after 4,000 53 / 50, 2,048 103 / 75, 256
+  // after 8,000 38 / 35.
+  const long long cap = d64 ? 3584 : 2560, work = (d64 ? 7ll << 15 : 1ll << 16) / steps;
+  const long long even = (work < cap ? work : cap) * 8 / c->n_kv;
+  if (rows <= even || rows <= 16ll * b->n_seq) {
+    p.use[FEW] = true;
+    p.few = 0x7fffffff;
+  } else {
+    // In a batch that fills the chip a tile costs as much as about 64 rows in
+    // attn_rows (64 sequences, us of attn_rows / attn_tile: 64 rows each at
+    // 1,000 positions, head_dim 64 30 / 34, 128 62 / 52; 62 rows 29 / 34, 63 /
+    // 52; without a past 64 rows 14 / 10, 24 / 16; 62 rows of 128 24 / 15).
+    p.use[MANY] = true;
+    p.use[FEW] = b->n_seq > 1;
+    p.few = b->n_seq == 1 ? 0 : d64 ? 63 : 32;
   }
-  p.few = !p.use[MANY] ? 0x7fffffff : !p.use[FEW] ? 0 : few;
   p.lr[FEW] = 4, p.lr[MANY] = 7;
   p.least[FEW] = 8, p.least[MANY] = 4;
-  p.waves = 8;
   if (p.use[FEW]) {
     long long tiles = most_row_tiles(b, group, ROWS);
-    const long long most = (long long)b->n_seq * ((few + ROWS - 1) / ROWS);
-    if (p.use[MANY] && tiles > most) tiles = most;
+    const long long most = (long long)b->n_seq * ((p.few + ROWS - 1ll) / ROWS);
+    if (tiles > most) tiles = most;
     // Splitting costs a second kernel and a second start (5 us), and saves
     // steps on a CU that has neighbours idle: worth it from about 40 steps of
-    // 8 KB or 16 of 16 KB on one sequence (us unsplit / split: head_dim 64,
-    // 2,600 positions 9.8 / 9.9, 4,096 12.5 / 9.8; 128: 1,024 positions 9.7 /
-    // 12.3, 2,048 14.2 / 14.0, 4,096 23.0 / 14.0), later the more CUs are
-    // busy anyway (16 sequences of 4,096, head_dim 64: 15.5 / 19.9).  Split
-    // work goes to workgroups of four waves, two for every CU; whole contexts
-    // to eight waves (one sequence of 1,024: 7.0 us with four, 6.6 with eight).
+    // 8 KB or 16 of 16 KB on one sequence, later the more CUs are busy anyway
+    // (us unsplit / split; head_dim 64: one sequence of 1,024 positions 6.3 /
+    // 9.3, of 4,096 12.0 / 9.3, four of 2,048 8.3 / 9.5, 16 of 4,096 15.2 /
+    // 18.9; 128: 1,024 9.6 / 10.7, 4,096 23.3 / 10.8, four of 2,048 15.6 /
+    // 12.3, 16 of 4,096 37.4 / 32.6).  Split work goes to workgroups of four
+    // waves, two for every CU.
     const long long units = tiles * c->n_kv;
     if (units < 256 && steps * (256 - units) > 256 * (d64 ? 40 : 16)) {
       p.target[FEW] = (512 + c->n_kv - 1) / c->n_kv;
       p.waves = 4;
+    } else {
+      // Whole contexts: as many waves as the steps occupy, fewer where
+      // workgroups are many (us with 8 / 4 / 2 waves, head_dim 64; 256
+      // workgroups of 16 steps 8.0 / 8.9 / 12.7, of 64 16 / 20 / 34; 512 of 24
+      // 14.2 / 12.8 / 18.9, of 64 27 / 29 / 46; 1,024 of 4 14 / 10 / 8.5, of 16
+      // 19 / 13 / 15, of 64 53 / 50 / 52; 4,096 of 1 50 / 25 / 18).
+      const long long low = (rows / ROWS > b->n_seq ? rows / ROWS : b->n_seq) * c->n_kv;
+      p.waves = low >= 1024 ? (steps <= 8 ? 2 : 4) : steps <= (low > 256 ? 48 : 8) ? 4 : 8;
     }
     p.items[FEW] = tiles + p.target[FEW];
     p.slots[FEW] = 2ll * p.target[FEW];
   }
   if (p.use[MANY]) {
-    // two workgroups fit a CU: split contexts where the row tiles do not fill them
-    const long long tiles = most_row_tiles(b, group, TILE_ROWS), sure = rows / TILE_ROWS;
-    if (steps > p.least[MANY] && sure * c->n_kv < 512) p.target[MANY] = (512 + c->n_kv - 1) / c->n_kv;
+    long long tiles = most_row_tiles(b, group, TILE_ROWS);
+    const long long most = rows / TILE_ROWS + rows / (p.few + 1);  // of sequences with more rows than `few`
+    if (tiles > most) tiles = most;
+    // Two workgroups fit a CU.  Where the row tiles do not fill them, contexts
+    // are split if they are long: the partials' way through memory and the join
+    // cost 10 us and more for more rows (us unsplit / split, one sequence,
+    // head_dim 64: 1,024 tokens 23 / 32, after 1,000 positions 40 / 39, after
+    // 4,000 89 / 57; 2,048 tokens 41 / 54, 59 / 65, 109 / 102; 128: 31 / 37,
+    // 56 / 46, 122 / 75; 56 / 64, 82 / 80, 148 / 135).
+    const long long units = rows / TILE_ROWS * c->n_kv;
+    if (steps * (512 - units) > 5120 + 32 * units) p.target[MANY] = (512 + c->n_kv - 1) / c->n_kv;
     p.items[MANY] = tiles + p.target[MANY];
     p.slots[MANY] = 2ll * p.target[MANY];
   }
@@ -420,6 +445,7 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   };
   if (pl.use[FEW] && pl.use[MANY]) d64 ? go(attn_both<64>, many + few, 256) : go(attn_both<128>, many + few, 256);
   else if (pl.use[MANY]) d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
+  else if (pl.waves == 2) d64 ? go(attn_rows<64, 2>, few, 128) : go(attn_rows<128, 2>, few, 128);
   else if (pl.waves == 4) d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
   else d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
   // a workgroup for every row, or where rows are many a wave for four (verify of

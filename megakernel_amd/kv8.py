@@ -6,8 +6,8 @@ What a server keeps next to the model: a pool of blocks that sequences share
 and the operators that take one layer from its QKV rows to its attention
 output: :func:`qk_norm_rope`, :func:`append`, :func:`attention`; :func:`read`
 gives rows of the cache back.  The reference has one contiguous bf16 cache
-(/root/reference/src/kv_cache.cuh:11-32) and these steps only inside its
-kernel (/root/reference/src/attention.cuh).
+(src/kv_cache.cuh:11-32) and these steps only inside its
+kernel (src/attention.cuh).
 
 Tensors are torch tensors on one GPU and belong to the caller, outputs
 included; nothing is copied, and no call waits.  Work is enqueued on torch's
@@ -148,8 +148,8 @@ class Batch:
     runs, so they may change between calls and replays.
 
     ``n_tokens`` is the row tensors' first size.  ``max_kv`` only says how long
-    contexts are expected to get, from which :func:`attention` chooses how far
-    to split them; longer ones are right all the same.
+    contexts are expected to get, from which :func:`attention` chooses its kernels
+    and how far to split them; longer ones are right all the same.
     """
 
     def __init__(self, table, q_start, kv_len, n_tokens: int, max_kv: int = 0):

@@ -555,21 +555,22 @@ def test_attention_splits(dim, missing):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("hint", [64, 0])
-def test_attention_of_many_rows_over_many_steps(dim, hint):
+@pytest.mark.parametrize("hint,n_kv", [(64, 32), (1 << 20, 1)])
+def test_attention_of_many_rows_over_many_steps(dim, hint, n_kv):
     """A prompt's last tokens over a context of more steps than a look-up of
     block ids covers, whole (a hint that is far too short) and split."""
-    block, lens, new = 16, [2710], [131]
+    block, lens, new = 16, [2710 if n_kv == 1 else 1310], [131]
     _say(f"attention many steps D={dim} hint {hint}")
-    c = _hint(Case(block, 1, dim, lens, new, seed=dim, missing=0.05), hint)
-    assert (kv8.workspace_bytes(c.cache, c.batch, 8) > 0) == (hint == 0)
-    _check_attention(c, 8)
+    c = _hint(Case(block, n_kv, dim, lens, new, seed=dim, missing=0.05), hint)
+    assert (kv8.workspace_bytes(c.cache, c.batch, 8 * n_kv) > 0) == (hint != 64)
+    _check_attention(c, 8 * n_kv)
 
 
-def test_attention_of_many_rows_joined_by_waves():
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_many_rows_joined_by_waves(dim):
     """More rows than a workgroup each."""
-    _say("attention joined by waves")
-    c = Case(64, 2, 64, [900], [300], seed=31)
+    _say(f"attention joined by waves D={dim}")
+    c = _hint(Case(64, 2, dim, [900], [300], seed=31), 1 << 20)
     assert kv8.workspace_bytes(c.cache, c.batch, 16) > 0 and c.tokens * 16 > 4096
     _check_attention(c, 16)
 
@@ -579,7 +580,7 @@ def test_attention_of_a_mixed_batch(dim):
     """Single tokens next to prompts, long and short contexts of each."""
     lens, new = [4300, 600, 40, 1500, 0, 300, 2100], [1, 250, 40, 3, 0, 1, 90]
     _say(f"attention mixed D={dim}")
-    for hint in (0, 64):
+    for hint in (0, 64, 1 << 20):
         c = _hint(Case(32, 1, dim, lens, new, seed=33, missing=0.03, gap=2), hint)
         _check_attention(c, 2, say=f"hint {hint}")
 
@@ -606,12 +607,12 @@ def test_more_sequences_than_a_wave_has_lanes():
         np.testing.assert_array_equal(_f64(g), w)
 
 
-@pytest.mark.parametrize("n_tokens", [2, 40])
-def test_graphs_of_split_contexts(n_tokens):
+@pytest.mark.parametrize("n_tokens,hint", [(2, 0), (40, 0), (40, 1 << 20)])
+def test_graphs_of_split_contexts(n_tokens, hint):
     """Two captured calls, each with the workspace it took, replayed in turn
     and on two streams at once, against the eager call."""
     _say(f"graphs of splits, {n_tokens} tokens")
-    cs = [Case(32, 2, 64, [4500], [n_tokens], seed=s) for s in (36, 37)]
+    cs = [_hint(Case(32, 2, 64, [4500], [n_tokens], seed=s), hint) for s in (36, 37)]
     qs = [c.rows(8, torch.bfloat16).cuda() for c in cs]
     assert all(kv8.workspace_bytes(c.cache, c.batch, 8) > 0 for c in cs)
     want, outs, graphs = [], [], []
@@ -662,9 +663,9 @@ def test_kv8_on_a_side_stream_behind_its_inputs():
     assert torch.equal(got, want)
 
 
-# Which kernel takes a sequence goes by its rows and by the context lengths
-# that a batch announces: announced as long, these go to the one for many rows
-# (split); announced as short, only where the rows are over 1,024.
+# Which kernel takes a sequence goes by the batch's rows times KV heads and by
+# the context lengths that it announces: announced as long, these go to the one
+# for many rows (split); announced as short, to the one for few.
 TILED = [
     # block, n_kv, group, dim, lens, new
     (16, 2, 3, 64, [90, 40, 17], [90, 33, 5]),
@@ -688,8 +689,51 @@ def test_attention_tiles(case, missing, hint):
     _check_attention(c, n_kv * group)
 
 
+# Enough rows times KV heads for the kernel for many rows with short contexts.
+WHOLE = [
+    (16, 64, 3, 64, [90, 40, 17, 100], [90, 33, 5, 60]),
+    (64, 64, 2, 128, [170, 66, 3], [160, 1, 3]),
+    (128, 128, 1, 128, [257], [257]),
+    (32, 64, 8, 64, [300], [65]),
+    (16, 32, 16, 64, [100, 1100], [66, 33]),
+    (64, 64, 1, 64, [600, 0, 129], [500, 0, 129]),
+    (32, 128, 2, 64, [1, 500], [1, 129]),
+]
+
+
+@pytest.mark.parametrize("missing", [0.0, 0.3])
+@pytest.mark.parametrize("case", WHOLE, ids=[f"b{c[0]}h{c[1]}g{c[2]}d{c[3]}n{sum(c[5])}" for c in WHOLE])
+def test_attention_tiles_whole(case, missing):
+    block, n_kv, group, dim, lens, new = case
+    _say(f"attention whole tiles {case} missing {missing}")
+    c = _hint(Case(block, n_kv, dim, lens, new, seed=block * dim + sum(lens), missing=missing, gap=1), 64)
+    assert kv8.workspace_bytes(c.cache, c.batch, n_kv * group) == 0
+    _check_attention(c, n_kv * group)
+
+
+# The kernel for few rows has eight, four or two waves by the steps and by how
+# many row tiles there are.
+WAVES = [
+    (16, 2, 2, [1500, 900], [3, 9]),       # eight
+    (16, 2, 2, [300, 0, 90], [33, 0, 1]),  # four
+    (32, 128, 1, [120, 60], [100, 28]),   # two
+    (128, 128, 1, [900, 7], [121, 7]),    # two, and steps for all of them
+]
+
+
+@pytest.mark.parametrize("missing", [0.0, 0.3])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("hint,group", [(1 << 20, 2), (64, 30)])
+@pytest.mark.parametrize("case", WAVES, ids=[f"b{c[0]}h{c[1]}g{c[2]}n{sum(c[4])}" for c in WAVES])
+def test_attention_rows_by_waves(case, dim, missing):
+    block, n_kv, group, lens, new = case
+    _say(f"attention waves {case} D={dim} missing {missing}")
+    c = _hint(Case(block, n_kv, dim, lens, new, seed=dim + sum(lens), missing=missing, gap=1), 2 * 64 if block == 32 else max(lens) // 2)
+    assert kv8.workspace_bytes(c.cache, c.batch, n_kv * group) == 0
+    _check_attention(c, n_kv * group)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("hint,group", [(1 << 20, 2), (64, 30), (64, 78)])
 def test_attention_tiles_never_see_what_they_may_not(dim, hint, group):
     """As the rows' test: NaN in unused blocks, behind the last row, and in
     positions that only some rows of a tile see."""
