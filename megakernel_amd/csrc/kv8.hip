@@ -218,14 +218,16 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
     long long tiles = most_row_tiles(b, group, TILE_ROWS);
     const long long most = rows / TILE_ROWS + rows / (p.few + 1);  // of sequences with more rows than `few`
     if (tiles > most) tiles = most;
-    // Two workgroups fit a CU.  Where the row tiles do not fill them, contexts
-    // are split if they are long: the partials' way through memory and the join
-    // cost 10 us and more for more rows (us unsplit / split, one sequence,
+    // Three workgroups of head_dim 64 fit a CU, two of 128 (1,024 tokens at the
+    // end of 8,192 and 32,768 positions, us in 512 / 768 parts: 64 74, 217 /
+    // 68, 202; 128 100, 316 / 109, 326).  Where the row tiles do not fill them,
+    // contexts are split if they are long: the partials' way through memory and
+    // the join cost 10 us, more for more rows (us unsplit / split, one sequence,
     // head_dim 64: 1,024 tokens 23 / 32, after 1,000 positions 40 / 39, after
     // 4,000 89 / 57; 2,048 tokens 41 / 54, 59 / 65, 109 / 102; 128: 31 / 37,
     // 56 / 46, 122 / 75; 56 / 64, 82 / 80, 148 / 135).
     const long long units = rows / TILE_ROWS * c->n_kv;
-    if (steps * (512 - units) > 5120 + 32 * units) p.target[MANY] = (512 + c->n_kv - 1) / c->n_kv;
+    if (steps * (512 - units) > 5120 + 32 * units) p.target[MANY] = ((d64 ? 768 : 512) + c->n_kv - 1) / c->n_kv;
     p.items[MANY] = tiles + p.target[MANY];
     p.slots[MANY] = 2ll * p.target[MANY];
   }

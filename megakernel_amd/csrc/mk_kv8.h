@@ -159,7 +159,9 @@ __device__ __forceinline__ void store8(void* p, long long e, const float (&f)[8]
 // lane and the mean is a DPP sum.  The angle is a product of a 24-bit and a
 // 31-bit number, formed and reduced to a fraction of a turn in fp64 (fp32
 // would be off by 2^-24 of an angle of up to 1e5 radians); the sine and
-// cosine of the fraction are fp32.
+// cosine of the fraction are fp32.  A wave recomputes them for its 8 or 16
+// heads only, which the loads hide: 8,192 tokens of 24 heads of 128, fp32 to
+// bf16 (151 MB), take 28 us, 5.4 TB/s; 16 tokens 2.7 us, an empty launch.
 template <int D, bool SRC32, bool DST32>
 __global__ __launch_bounds__(256) void norm_rope(Rows q, Rows k, const uint16_t* __restrict__ qg,
                                                  const uint16_t* __restrict__ kg, const float* __restrict__ freq,
@@ -289,8 +291,12 @@ struct Raw8 {
 };
 
 // One team of T threads per block that rows go to and head, K and V both; a
-// workgroup holds 256 / T heads.  The rows stay in registers between the
-// maximum and the rounding, so the input is read once.
+// workgroup holds 256 / T heads.  The rows stay in registers as they were
+// loaded between the maximum and the rounding, so the input is read once (66
+// registers from bf16; expanded to fp32 it took 104, and 35 us where this takes
+// 24: 16,499 rows of 8 heads of 128 in ragged prompts, 101 MB, 4.2 TB/s).  One
+// row to each of 16 sequences takes 6 us: three loads in a row (lengths, table,
+// rows) and the launch.
 template <int D, int T, int PASSES, bool SRC32>
 __global__ __launch_bounds__(256) void append(Cache c, Batch b, Rows kr, Rows vr) {
   constexpr int HEADS = 256 / T;
@@ -463,6 +469,7 @@ __device__ __forceinline__ uint32_t gather4(uint32_t a, uint32_t b, uint32_t c, 
 }
 
 // A workgroup takes `heads` heads of one block; a thread a piece at a time.
+// Bound by the bytes: the same rows back as bf16 20 us (101 MB, 5.1 TB/s).
 template <int D, bool DST32>
 __global__ __launch_bounds__(256) void read_back(Cache c, Batch b, Rows kr, Rows vr, int heads) {
   Seq s;
@@ -706,6 +713,14 @@ struct Ids {
 // 16g + 4t + (0..3) of query row c -- the 16 positions whose V codes of one
 // dimension are the lane's 16-byte V load, which makes the weights the B
 // operand as they stand.
+//
+// Measured (whole calls, joins included): one sequence of 1,024 positions,
+// head_dim 64, 6.0 us, of which a launch is 2.7 and the rest three loads in a
+// row and one step; 16 sequences of 512 to 4,096 13.6 us (38 MB; whole
+// contexts on 128 CUs); one of 32,768, head_dim 128, 19.2 us (67 MB, 14.5 us
+// and 4.7 for the join); 3 to 6 tokens each of 16 sequences of 700 to 8,191
+// 39 us (148 MB, 34 and 5).  Streaming as many bytes without any work takes
+// 7, 12 and 27 us here.
 template <int D, int W>
 struct RowsLds {
   float lo[W][ROWS][D + 4];
@@ -788,7 +803,9 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   f32x4 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, sum = 0.f;
+  // the weights' reference of row c (or -inf), it negated (or 0), and what the
+  // lane's scores may reach before it is raised
+  float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f;
 
   // Both are waited for here: left to itself, the second would be asked for
   // behind the first codes, and the loop's waits be for everything.
@@ -859,21 +876,22 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) mt = fmaxf(mt, sc[i][j]);
-    mt = max_xor32(max_xor16(mt)) * p.scale;
-    if (__any(mt > m + RISE)) {
-      const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    mt *= p.scale;
+    if (__any(mt > up)) {  // joined over the row's four lanes only here
+      const float mn = fmaxf(m, max_xor32(max_xor16(mt))), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
+      below = mn == -INFINITY ? 0.f : -mn;
+      up = mn + RISE;
       sum *= al;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= al;
     }
-    const float mref = m == -INFINITY ? 0.f : m;
     float pr[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        pr[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], p.scale, -mref));
+        pr[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], p.scale, below));
         sum += pr[4 * i + j];
       }
     bf16x8 pb[2];
@@ -942,7 +960,14 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
 // Many query rows.  128 rows per workgroup, 32 to each of its four waves, on
 // v_mfma_f32_32x32x16_bf16; a step's 64 positions are turned from codes to
 // bf16 once and staged in LDS for all four (two buffers, one barrier a step;
-// the next step's codes are in flight meanwhile).  Rows of LDS are padded by
+// the next step's codes are in flight meanwhile).  1,024 tokens of 16 / 8 heads
+// of 128 at the end of 32,768 positions: 300 us with the join's 13, 900
+// TFLOP/s, where a large bf16 product reaches 1,215.  The matrix units are busy
+// 41 % of the time and the vector units, mostly with the weights, about as
+// much; two workgroups per CU overlap them in part.  64 rows per wave (half
+// the LDS reads) took 350 us: one wave per SIMD does not hide its own staging.
+// head_dim 64 is bound by the vector units: ragged prompts of 33 to 2,048
+// tokens 51 us.  Rows of LDS are padded by
 // 16 bytes, which spreads the eight lanes that a 16-byte read serves at once
 // over all banks.  K rows lie in LDS in the order that makes a lane's 16
 // scores of 32 positions two runs of eight positions, 8h + 16m of half-wave h,
@@ -1091,7 +1116,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-  float m = -INFINITY, sum = 0.f;
+  float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f;  // as in rows_item()
   // Both halves in turn: a product that adds to the one before it waits twice
   // as long as the unit takes.
   const auto scores = [&](int k) {
@@ -1167,17 +1192,18 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[a][i]);
-    mt = max_xor32(mt) * p.scale;
-    if (__any(mt > m + RISE)) {
-      const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    mt *= p.scale;
+    if (__any(mt > up)) {
+      const float mn = fmaxf(m, max_xor32(mt)), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
+      below = mn == -INFINITY ? 0.f : -mn;
+      up = mn + RISE;
       sum *= al;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= al;
     }
-    const float mref = m == -INFINITY ? 0.f : m;
     if (__builtin_expect((first + TILE > rows.all || gone) && lds.bad[buf] == k + 1, 0)) {
       // the NaN that stage_v() took out, put into the rows that see them
       const int x = min(max(see - first, 0), TILE);
@@ -1195,8 +1221,8 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
     const auto weights = [&](int a) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], p.scale, -mref));
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], p.scale, -mref));
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], p.scale, below));
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], p.scale, below));
         const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
         sum = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum, false);  // of the weights as V's product has them
         pb[a][i / 8][i % 8] = w[0];
@@ -1247,7 +1273,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
 }
 
 template <int D, int W>
-__global__ __launch_bounds__(W* kWave) void attn_rows(Attn p) {
+__global__ __launch_bounds__(W* kWave, D == 64 ? 3 : 2) void attn_rows(Attn p) {
   __shared__ __align__(16) RowsLds<D, W> lds;
   rows_item<D, W>(p, (int)blockIdx.x, &lds);
 }
