@@ -159,9 +159,9 @@ __device__ __forceinline__ void store8(void* p, long long e, const float (&f)[8]
 // lane and the mean is a DPP sum.  The angle is a product of a 24-bit and a
 // 31-bit number, formed and reduced to a fraction of a turn in fp64 (fp32
 // would be off by 2^-24 of an angle of up to 1e5 radians); the sine and
-// cosine of the fraction are fp32.  A wave recomputes them for its 8 or 16
-// heads only, which the loads hide: 8,192 tokens of 24 heads of 128, fp32 to
-// bf16 (151 MB), take 28 us, 5.4 TB/s; 16 tokens 2.7 us, an empty launch.
+// cosine of the fraction are fp32.  Every head forms its own, which the loads
+// hide: 8,192 tokens of 24 heads of 128, fp32 to bf16 (151 MB), take 28 us, 5.4
+// TB/s; 16 tokens 2.7 us, an empty launch.
 template <int D, bool SRC32, bool DST32>
 __global__ __launch_bounds__(256) void norm_rope(Rows q, Rows k, const uint16_t* __restrict__ qg,
                                                  const uint16_t* __restrict__ kg, const float* __restrict__ freq,
@@ -715,12 +715,14 @@ struct Ids {
 // operand as they stand.
 //
 // Measured (whole calls, joins included): one sequence of 1,024 positions,
-// head_dim 64, 6.0 us, of which a launch is 2.7 and the rest three loads in a
-// row and one step; 16 sequences of 512 to 4,096 13.6 us (38 MB; whole
-// contexts on 128 CUs); one of 32,768, head_dim 128, 19.2 us (67 MB, 14.5 us
-// and 4.7 for the join); 3 to 6 tokens each of 16 sequences of 700 to 8,191
-// 39 us (148 MB, 34 and 5).  Streaming as many bytes without any work takes
-// 7, 12 and 27 us here.
+// head_dim 64, 6.2 us, of which a launch is 2.7 and the rest three loads in a
+// row and one step; 16 sequences of 512 to 4,096 13.1 us (38 MB; whole
+// contexts on 128 CUs, bound by what a CU takes in: codes of two steps ahead,
+// and weights formed for the rows that are there alone, changed nothing); one
+// of 32,768, head_dim 128, 19.1 us (67 MB, 14.4 us and 4.7 for the join); 3 to
+// 6 tokens each of 16 sequences of 700 to 8,191 39 us (148 MB, 34 and 5); 64
+// sequences of 4,096, head_dim 64, 53 us (268 MB, 5.1 TB/s).  Streaming as many
+// bytes without any work takes 7, 12, 27 and 48 us here.
 template <int D, int W>
 struct RowsLds {
   float lo[W][ROWS][D + 4];
@@ -961,13 +963,13 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
 // v_mfma_f32_32x32x16_bf16; a step's 64 positions are turned from codes to
 // bf16 once and staged in LDS for all four (two buffers, one barrier a step;
 // the next step's codes are in flight meanwhile).  1,024 tokens of 16 / 8 heads
-// of 128 at the end of 32,768 positions: 300 us with the join's 13, 900
+// of 128 at the end of 32,768 positions: 290 us with the join's 12, 930
 // TFLOP/s, where a large bf16 product reaches 1,215.  The matrix units are busy
-// 41 % of the time and the vector units, mostly with the weights, about as
-// much; two workgroups per CU overlap them in part.  64 rows per wave (half
-// the LDS reads) took 350 us: one wave per SIMD does not hide its own staging.
-// head_dim 64 is bound by the vector units: ragged prompts of 33 to 2,048
-// tokens 51 us.  Rows of LDS are padded by
+// 40 % of the time and the vector units, mostly with the weights, as much; two
+// workgroups per CU overlap them in part.  64 rows per wave (half the LDS
+// reads) took 350 us: one wave per SIMD does not hide its own staging.  Without
+// a past the longest tile decides, a step a microsecond: ragged prompts of 33
+// to 2,048 tokens, head_dim 64, 50 us, one of 4,096 83.  Rows of LDS are padded by
 // 16 bytes, which spreads the eight lanes that a 16-byte read serves at once
 // over all banks.  K rows lie in LDS in the order that makes a lane's 16
 // scores of 32 positions two runs of eight positions, 8h + 16m of half-wave h,
