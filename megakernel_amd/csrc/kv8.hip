@@ -176,13 +176,15 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
     p.use[FEW] = true;
     p.few = 0x7fffffff;
   } else {
-    // In a batch that fills the chip a tile costs as much as about 64 rows in
-    // attn_rows (64 sequences, us of attn_rows / attn_tile: 64 rows each at
-    // 1,000 positions, head_dim 64 30 / 34, 128 62 / 52; 62 rows 29 / 34, 63 /
-    // 52; without a past 64 rows 14 / 10, 24 / 16; 62 rows of 128 24 / 15).
+    // In a batch that fills the chip a tile costs as much as 64 rows of
+    // attn_rows, or 32 (64 sequences, us of attn_rows / attn_tile; head_dim 64
+    // after 1,000 positions 62 rows each 29 / 34, after 200 17 / 15, without a
+    // past 14 / 9, 34 rows 23 / 31, 13 / 14, 11 / 8; 128: 62 rows 63 / 52, 31 /
+    // 22, 24 / 15, 34 rows 49 / 49, 24 / 20, 18 / 13, 32 rows 39 / 49, 18 / 20,
+    // 13 / 12).
     p.use[MANY] = true;
     p.use[FEW] = b->n_seq > 1;
-    p.few = b->n_seq == 1 ? 0 : d64 ? 63 : 32;
+    p.few = b->n_seq == 1 ? 0 : d64 && steps > 8 ? 64 : 32;
   }
   p.lr[FEW] = 4, p.lr[MANY] = 7;
   p.least[FEW] = 8, p.least[MANY] = 4;
