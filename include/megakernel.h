@@ -431,7 +431,8 @@ float megakernel_op_last_ms(void);
 
 /* Rows of heads: element d of head h of token t at p[t * token_stride +
  * h * head_stride + d], strides in elements.  Rows start at multiples of 16
- * bytes.  Rows that are written may not overlap. */
+ * bytes.  Rows that are written may not overlap each other, nor what a call
+ * reads, but for an output of the norms that is its own input. */
 typedef struct {
   void* p;
   long long token_stride, head_stride;

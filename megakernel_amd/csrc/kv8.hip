@@ -53,6 +53,13 @@ static bool apart(const char* op, const char* name, const megakernel_rows* r, in
   return true;
 }
 
+// Two tensors, one of them written, that cannot be the same.
+static bool two(const char* op, const char* names, const megakernel_rows* a, const megakernel_rows* b) {
+  if (a->p != b->p) return true;
+  set_err("%s: %s must not be the same rows", op, names);
+  return false;
+}
+
 static bool cache_ok(const char* op, const megakernel_kv8_cache* c) {
   if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) {
     set_err("%s: null cache pointer", op);
@@ -315,6 +322,7 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
     return -1;
   }
   if (n_tokens == 0) return 0;
+  if (!two(op, "q_out and k_out", q_out, k_out) || !two(op, "q_out and k", q_out, k) || !two(op, "k_out and q", k_out, q)) return -1;
   const int hpw = 1024 / head_dim;
   const long long waves = (long long)n_tokens * ((n_q + n_kv + hpw - 1) / hpw), groups = (waves + 3) / 4;
   if (!grid_ok(op, groups)) return -1;
@@ -376,7 +384,7 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
   while (heads < cache->n_kv && items * cache->n_kv > 2048ll * heads) heads *= 2;
   const long long groups = items * ((cache->n_kv + heads - 1) / heads);
   if (groups == 0) return 0;
-  if (!grid_ok(op, groups)) return -1;
+  if (!two(op, "k_out and v_out", k_out, v_out) || !grid_ok(op, groups)) return -1;
   auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, static_cast<hipStream_t>(stream), cache_of(cache),
                        batch_of(batch), rows_of(k_out), rows_of(v_out), heads);
@@ -440,7 +448,10 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   // tokens whose rows may have splits to join
   long long tokens = batch->n_tokens;
   if (!pl.target[MANY] && pl.use[MANY] && tokens > (long long)batch->n_seq * (pl.few / p.group)) tokens = (long long)batch->n_seq * (pl.few / p.group);
-  const long long joins = tokens * n_q;
+  // a workgroup for every row, or where rows are many a wave for four (verify of
+  // 1,152 rows 41.0 / 43.6 us in all, a prompt of 16,384 336 / 315)
+  const bool each = tokens * n_q <= 4096;
+  const long long joins = !need ? 0 : each ? tokens * n_q : (tokens * ((n_q + 3) / 4) + 3) / 4;
   if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
@@ -452,13 +463,8 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   else if (pl.waves == 2) d64 ? go(attn_rows<64, 2>, few, 128) : go(attn_rows<128, 2>, few, 128);
   else if (pl.waves == 4) d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
   else d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
-  // a workgroup for every row, or where rows are many a wave for four (verify of
-  // 1,152 rows 41.0 / 43.6 us in all, a prompt of 16,384 336 / 315)
-  if (need && joins <= 4096) d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
-  else if (need) {
-    const long long waves = tokens * ((n_q + 3) / 4);
-    d64 ? go(attn_join_waves<64, 4>, (waves + 3) / 4, 256) : go(attn_join_waves<128, 4>, (waves + 3) / 4, 256);
-  }
+  if (need && each) d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
+  else if (need) d64 ? go(attn_join_waves<64, 4>, joins, 256) : go(attn_join_waves<128, 4>, joins, 256);
   return launched(op);
 }
 

@@ -13,7 +13,8 @@ Tensors are torch tensors on one GPU and belong to the caller, outputs
 included; nothing is copied, and no call waits.  Work is enqueued on torch's
 current stream of that GPU, so tensors that another stream wrote need that
 stream waited for, as with torch's own operators.  Calls can be captured into
-a graph: a replay reads lengths and tables anew, while sizes stay fixed.
+a graph: a replay reads lengths and tables anew, while sizes stay fixed.  No
+gradients are recorded.
 
     cache = kv8.Cache(k, v, k_scale, v_scale)      # or kv8.Cache.empty(...)
     batch = kv8.Batch(table, q_start, kv_len, n_tokens)
@@ -109,7 +110,17 @@ def _call(name: str, device: int, *args):
         _lib.check(_library, rc, name[11:])
 
 
-class Cache:
+class _Fixed:
+    """The library is handed the tensors' addresses: another tensor in the
+    place of one would not be seen, and the first one's memory be reused."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{name} of a {type(self).__name__} stays what it was made with; make another one")
+        self.__dict__[name] = value
+
+
+class Cache(_Fixed):
     """A pool of blocks of one layer: e4m3 codes ``k`` [n_blocks][n_kv][block][head_dim]
     and ``v`` [n_blocks][n_kv][head_dim][block] (uint8), and their power-of-two
     scales [n_blocks][n_kv] (float32).  ``block`` is 16, 32, 64 or 128
@@ -138,7 +149,7 @@ class Cache:
         return cls(*codes, *(torch.empty((n_blocks, n_kv), dtype=torch.float32, device=device) for _ in range(2)))
 
 
-class Batch:
+class Batch(_Fixed):
     """Rows of several sequences.  Sequence i has rows q_start[i] ..
     q_start[i + 1] - 1 of the row tensors, and these are the newest of its
     kv_len[i] positions.  ``table`` [n_seq][width] names its blocks in order;

@@ -799,3 +799,22 @@ def test_attention_tiles_negative_positions_and_rising_maxima():
     q = c.rows(3, torch.bfloat16, 0.5) + 0.25
     _, out = _check_attention(c, 3, q=q)
     assert torch.all(out[:40] == 0)
+
+
+def test_more_rows_than_workgroups_of_one_launch():
+    """2^25 rows of heads, most of them before position 0: zeros."""
+    _say("2^20 tokens")
+    tokens = 1 << 20
+    c = Case(32, 8, 64, [40], [40], seed=40)
+    q = c.rows(32, torch.bfloat16)
+    want, out = np.zeros((40, 32, 64)), torch.empty((tokens, 32, 64), dtype=torch.bfloat16, device="cuda")
+    size, reach = c.pool.attention(c.table, c.start, c.lens, _f64(q), want, 64 ** -0.5)
+    many = torch.zeros((tokens, 32, 64), dtype=torch.bfloat16, device="cuda")
+    many[-40:] = q.cuda()
+    start = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+    batch = kv8.Batch(c.batch.table, start, c.batch.kv_len, tokens)
+    kv8.attention(c.cache, batch, many, out)
+    torch.cuda.synchronize()
+    tol = np.abs(want) * 2.0 ** -8 + (2.0 ** -8 + (2 * 64 * reach + 40 + 16)[..., None] * U) * size
+    assert np.all(np.abs(_f64(out[-40:]) - want) <= tol)
+    assert not out[:-40].any()

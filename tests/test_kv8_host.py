@@ -207,3 +207,20 @@ def test_python_entry_points_refuse_cpu_tensors():
     q = torch.zeros((1, 1, 64))
     with pytest.raises(ValueError, match="on the GPU"):
         kv8.qk_norm_rope(q, q, q[0, 0], q[0, 0], q[0, 0], q[0, 0], q, q)
+
+
+def test_outputs_that_are_one_are_refused(clib):
+    c, b, far = _ref(_cache()), _ref(_batch()), [_ref(_r(i * FAKE)) for i in range(1, 5)]
+    _refused(clib, clib.megakernel_op_kv8_read(c, b, far[0], far[0], None), "same rows")
+    for q, k, qo, ko in ((0, 1, 2, 2), (0, 1, 1, 2), (0, 1, 2, 0), (0, 1, 1, 0)):
+        _refused(clib, clib.megakernel_op_qk_norm_rope(far[q], far[k], FAKE, FAKE, FAKE, FAKE, far[qo], far[ko], 5, 8, 8, 64,
+                                                       1e-6, None), "same rows")
+
+
+def test_tensors_of_a_cache_or_batch_cannot_be_replaced():
+    for cls in (kv8.Cache, kv8.Batch):
+        x = cls.__new__(cls)
+        x.device = 0
+        with pytest.raises(AttributeError, match="make another"):
+            x.device = 1
+        assert x.device == 0
