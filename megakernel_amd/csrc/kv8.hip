@@ -206,10 +206,13 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
     // 9.3, of 4,096 12.0 / 9.3, four of 2,048 8.3 / 9.5, 16 of 4,096 15.2 /
     // 18.9; 128: 1,024 9.6 / 10.7, 4,096 23.3 / 10.8, four of 2,048 15.6 /
     // 12.3, 16 of 4,096 37.4 / 32.6).  Split work goes to workgroups of four
-    // waves, two for every CU.
+    // waves, two for every CU.  Sequences end inside a part, which makes half a
+    // part more for every row tile: with these over the two, some CUs would
+    // start a third when the others end (16 of 700 to 8,191, 128: 37.6, now
+    // 35.0; 12 of 500 to 20,000: 58 / 54; four of 8,000 alike 19.3 / 19.9).
     const long long units = tiles * c->n_kv;
     if (units < 256 && steps * (256 - units) > 256 * (d64 ? 40 : 16)) {
-      p.target[FEW] = (512 + c->n_kv - 1) / c->n_kv;
+      p.target[FEW] = (512 + c->n_kv - 1) / c->n_kv - (b->n_seq > 1 ? (int)tiles / 2 : 0);
       p.waves = 4;
     } else {
       // Whole contexts: as many waves as the steps occupy, fewer where

@@ -170,8 +170,8 @@ __global__ __launch_bounds__(256) void norm_rope(Rows q, Rows k, const uint16_t*
   constexpr int LPH = D / 16, HPW = kWave / LPH;  // lanes per head, heads per wave
   const int l = (int)(threadIdx.x & 63u), j = l % LPH;
   const int heads = n_q + n_kv, passes = (heads + HPW - 1) / HPW;
-  const long long it = (long long)blockIdx.x * 4 + threadIdx.x / 64;
-  const int t = (int)(it / passes), h = (int)(it % passes) * HPW + l / LPH;
+  const unsigned it = blockIdx.x * 4 + threadIdx.x / 64;  // below 2^26
+  const int t = (int)(it / (unsigned)passes), h = (int)(it % (unsigned)passes) * HPW + l / LPH;
   if (t >= n_tokens || h >= heads) return;
   const bool is_k = h >= n_q;
   const Rows& src = is_k ? k : q;
@@ -565,15 +565,15 @@ struct RowTile {
   int n_rows, any, all;
 };
 __device__ __forceinline__ RowTile row_tile(const Seq& s, int G, int rt, int rows) {
-  const long long r0 = (long long)rt * rows, left = (long long)s.rows * G - r0;
+  const int r0 = rt * rows;  // rows times G are at most 2^30
   RowTile t;
-  t.n_rows = (int)min(left, (long long)rows);
-  t.all = min(max(s.pos0 + (int)(r0 / G) + 1, 0), s.len);
-  t.any = min(max(s.pos0 + (int)((r0 + t.n_rows - 1) / G) + 1, 0), s.len);
+  t.n_rows = min(s.rows * G - r0, rows);
+  t.all = min(max(s.pos0 + r0 / G + 1, 0), s.len);
+  t.any = min(max(s.pos0 + (r0 + t.n_rows - 1) / G + 1, 0), s.len);
   return t;
 }
 __device__ __forceinline__ int row_tiles(const Seq& s, int G, int lr) {
-  return (int)(((long long)s.rows * G + (1 << lr) - 1) >> lr);
+  return (s.rows * G + (1 << lr) - 1) >> lr;
 }
 
 // Most splits of one row tile (attn_join gives each a thread).
@@ -585,6 +585,10 @@ struct Item {
   int rt, split, ns;  // row tile, split, splits of this sequence's row tiles
   int slot;           // of the tile's first partial, if ns > 1
   int kind;
+  // first step of split i, of the row tile's `steps`
+  __device__ __forceinline__ int step(int i, int steps) const {
+    return ns == 1 ? i * steps : steps / ns * i + min(i, steps % ns);
+  }
 };
 
 // Steps of a sequence's longest row tile.
@@ -611,7 +615,9 @@ __device__ __forceinline__ int steps_per_item(const Attn& p, int kind, const Seq
     const int lo = wave_prefix((int)(w & 0xffffff)), hi = wave_prefix((int)min(w >> 24, 0x1ffffffll));
     total += ((long long)__builtin_amdgcn_readlane(hi, 63) << 24) + __builtin_amdgcn_readlane(lo, 63);
   }
-  return (int)min(max((total + d.target - 1) / d.target, (long long)d.least), 0x7fffffffll);
+  // (a division of 64 bits takes longer than all the rest)
+  const long long per = total < 0x7fffffff ? (int)total / d.target + ((int)total % d.target != 0) : (total + d.target - 1) / d.target;
+  return (int)min(max(per, (long long)d.least), 0x7fffffffll);
 }
 
 // Where sequences are of unlike length, equal splits of each would leave most
@@ -637,7 +643,7 @@ __device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
     if (KIND < 0 ? (kind ? p.d[1].target : p.d[0].target) != 0 : kind == KIND) {
       const int per = kind ? per1 : per0;
       const int rt = row_tiles(q, G, kind ? p.d[1].lr : p.d[0].lr), n = most_steps(q);
-      ns = min(max(n / per + (n % per != 0), 1), kMaxSplits);
+      if (p.d[0].target | p.d[1].target) ns = min(max(n / per + (n % per != 0), 1), kMaxSplits);
       const int sl = ns > 1 ? rt * ns : 0;
       s0 = kind ? 0 : sl;
       s1 = kind ? sl : 0;
@@ -660,8 +666,8 @@ __device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
         r.rt = within;
         r.split = 0;
       } else {
-        r.rt = within / r.ns;
-        r.split = within % r.ns;
+        r.rt = r.ns == 1 ? within : within / r.ns;
+        r.split = within - r.rt * r.ns;
         r.slot += r.rt * r.ns;
       }
       return true;
@@ -744,7 +750,7 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   const int c = l & 15, g = l >> 4;  // this lane's query row; its 16 positions of a step
   const RowTile rows = row_tile(s, G, it.rt, ROWS);
   const int r0 = it.rt * ROWS, tiles = (rows.any + TILE - 1) / TILE;
-  const int t0 = (int)((long long)tiles * it.split / it.ns), t1 = (int)((long long)tiles * (it.split + 1) / it.ns);
+  const int t0 = it.step(it.split, tiles), t1 = it.step(it.split + 1, tiles);
   const bool mine = c < rows.n_rows;
   const int rr = mine ? r0 + c : r0, tok = rr / G, hd = head * G + rr % G;
   const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
@@ -1005,7 +1011,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   const int c = l & 31, h = l >> 5;
   const RowTile rows = row_tile(s, G, it.rt, TILE_ROWS);
   const int r0 = it.rt * TILE_ROWS, tiles = (rows.any + TILE - 1) / TILE;
-  const int t0 = (int)((long long)tiles * it.split / it.ns), t1 = (int)((long long)tiles * (it.split + 1) / it.ns);
+  const int t0 = it.step(it.split, tiles), t1 = it.step(it.split + 1, tiles);
   const int n = t1 - t0, end = min(s.len, t1 * TILE);
   const bool mine = 32 * wv + c < rows.n_rows;
   const int rr = mine ? r0 + 32 * wv + c : r0, tok = rr / G, hd = head * G + rr % G;
