@@ -129,9 +129,21 @@ static bool grid_ok(const char* op, long long groups) {
   return true;
 }
 
-static int launched(const char* op) {
-  const hipError_t e = hipGetLastError();
+template <class T>
+struct Same {
+  typedef T type;
+};
+// What a kernel's launch returns; no error that an earlier call left is taken
+// for its own.
+template <class... P>
+static hipError_t launch(void (*kern)(P...), long long groups, int threads, hipStream_t st, typename Same<P>::type... args) {
+  void* a[] = {&args...};
+  return hipLaunchKernel(reinterpret_cast<const void*>(kern), dim3((unsigned)groups), dim3(threads), a, 0, st);
+}
+
+static int launched(const char* op, hipError_t e) {
   if (e == hipSuccess) return 0;
+  (void)hipGetLastError();  // reported here
   set_err("%s: launch failed: %s", op, hipGetErrorString(e));
   return -1;
 }
@@ -266,8 +278,8 @@ static bool heads_ok(const char* op, int n_q, int n_kv) {
 static int block_pieces(const megakernel_kv8_cache* c) { return c->block / 4 * (c->head_dim / 8); }
 
 template <int D>
-static void launch_append(int pieces, bool f32, dim3 g, hipStream_t st, Cache c, Batch b, Rows k, Rows v) {
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, g, dim3(256), 0, st, c, b, k, v); };
+static hipError_t launch_append(int pieces, bool f32, long long groups, hipStream_t st, Cache c, Batch b, Rows k, Rows v) {
+  auto go = [&](auto kern) { return launch(kern, groups, 256, st, c, b, k, v); };
   if constexpr (D == 64)
     if (pieces == 32) return f32 ? go(append<D, 32, 1, true>) : go(append<D, 32, 1, false>);
   if (pieces == 64) return f32 ? go(append<D, 64, 1, true>) : go(append<D, 64, 1, false>);
@@ -330,18 +342,15 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
   const long long waves = (long long)n_tokens * ((n_q + n_kv + hpw - 1) / hpw), groups = (waves + 3) / 4;
   if (!grid_ok(op, groups)) return -1;
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, static_cast<hipStream_t>(stream), rows_of(q), rows_of(k),
-                       static_cast<const uint16_t*>(q_gain), static_cast<const uint16_t*>(k_gain), inv_freq, pos,
-                       rows_of(q_out), rows_of(k_out), n_tokens, n_q, n_kv, eps);
+    return launch(kern, groups, 256, static_cast<hipStream_t>(stream), rows_of(q), rows_of(k),
+                  static_cast<const uint16_t*>(q_gain), static_cast<const uint16_t*>(k_gain), inv_freq, pos, rows_of(q_out),
+                  rows_of(k_out), n_tokens, n_q, n_kv, eps);
   };
   const bool s32 = q->type == MK_TYPE_F32, d32 = q_out->type == MK_TYPE_F32;
-  if (head_dim == 64)
-    s32 ? (d32 ? go(norm_rope<64, true, true>) : go(norm_rope<64, true, false>))
-        : (d32 ? go(norm_rope<64, false, true>) : go(norm_rope<64, false, false>));
-  else
-    s32 ? (d32 ? go(norm_rope<128, true, true>) : go(norm_rope<128, true, false>))
-        : (d32 ? go(norm_rope<128, false, true>) : go(norm_rope<128, false, false>));
-  return launched(op);
+  return launched(op, head_dim == 64 ? s32 ? (d32 ? go(norm_rope<64, true, true>) : go(norm_rope<64, true, false>))
+                                           : (d32 ? go(norm_rope<64, false, true>) : go(norm_rope<64, false, false>))
+                      : s32          ? (d32 ? go(norm_rope<128, true, true>) : go(norm_rope<128, true, false>))
+                                     : (d32 ? go(norm_rope<128, false, true>) : go(norm_rope<128, false, false>)));
 }
 
 int megakernel_op_kv8_append(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
@@ -358,12 +367,10 @@ int megakernel_op_kv8_append(const megakernel_kv8_cache* cache, const megakernel
   const long long groups = block_items(batch, cache->block) * ((cache->n_kv + heads - 1) / heads);
   if (groups == 0) return 0;
   if (!grid_ok(op, groups)) return -1;
-  const dim3 g((unsigned)groups);
   const bool f32 = k->type == MK_TYPE_F32;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->head_dim == 64) launch_append<64>(pieces, f32, g, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v));
-  else launch_append<128>(pieces, f32, g, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v));
-  return launched(op);
+  const auto go = cache->head_dim == 64 ? launch_append<64> : launch_append<128>;
+  return launched(op, go(pieces, f32, groups, st, cache_of(cache), batch_of(batch), rows_of(k), rows_of(v)));
 }
 
 int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
@@ -389,12 +396,11 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
   if (groups == 0) return 0;
   if (!two(op, "k_out and v_out", k_out, v_out) || !grid_ok(op, groups)) return -1;
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, static_cast<hipStream_t>(stream), cache_of(cache),
-                       batch_of(batch), rows_of(k_out), rows_of(v_out), heads);
+    return launch(kern, groups, 256, static_cast<hipStream_t>(stream), cache_of(cache), batch_of(batch), rows_of(k_out),
+                  rows_of(v_out), heads);
   };
-  if (cache->head_dim == 64) f32 ? go(read_back<64, true>) : go(read_back<64, false>);
-  else f32 ? go(read_back<128, true>) : go(read_back<128, false>);
-  return launched(op);
+  return launched(op, cache->head_dim == 64 ? (f32 ? go(read_back<64, true>) : go(read_back<64, false>))
+                                            : (f32 ? go(read_back<128, true>) : go(read_back<128, false>)));
 }
 
 long long megakernel_op_kv8_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, int n_q) {
@@ -458,17 +464,18 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool d64 = cache->head_dim == 64;
-  auto go = [&](auto kern, long long groups, int threads) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(threads), 0, st, p);
-  };
-  if (pl.use[FEW] && pl.use[MANY]) d64 ? go(attn_both<64>, many + few, 256) : go(attn_both<128>, many + few, 256);
-  else if (pl.use[MANY]) d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
-  else if (pl.waves == 2) d64 ? go(attn_rows<64, 2>, few, 128) : go(attn_rows<128, 2>, few, 128);
-  else if (pl.waves == 4) d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
-  else d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
-  if (need && each) d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
-  else if (need) d64 ? go(attn_join_waves<64, 4>, joins, 256) : go(attn_join_waves<128, 4>, joins, 256);
-  return launched(op);
+  auto go = [&](auto kern, long long groups, int threads) { return launch(kern, groups, threads, st, p); };
+  hipError_t e;
+  if (pl.use[FEW] && pl.use[MANY]) e = d64 ? go(attn_both<64>, many + few, 256) : go(attn_both<128>, many + few, 256);
+  else if (pl.use[MANY]) e = d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
+  else if (pl.waves == 2) e = d64 ? go(attn_rows<64, 2>, few, 128) : go(attn_rows<128, 2>, few, 128);
+  else if (pl.waves == 4) e = d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
+  else e = d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
+  if (e == hipSuccess && need) {
+    if (each) e = d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
+    else e = d64 ? go(attn_join_waves<64, 4>, joins, 256) : go(attn_join_waves<128, 4>, joins, 256);
+  }
+  return launched(op, e);
 }
 
 }  // extern "C"

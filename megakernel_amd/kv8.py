@@ -28,7 +28,7 @@ import ctypes
 import struct
 
 import torch
-from torch._C import _cuda_getCurrentRawStream as _raw_stream
+from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device
 
 from . import _lib
 
@@ -101,7 +101,7 @@ def _call(name: str, device: int, *args):
         _library = _lib.load()
     fn = getattr(_library, name)
     # the handle of torch.cuda.current_stream(device), without the object around it
-    if device == torch.cuda.current_device():
+    if device == _current_device():
         rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
