@@ -441,8 +441,8 @@ __device__ __forceinline__ void decode4(uint32_t w, float s, float* f) {
 }
 // 16 bytes of a row: 8 bf16 or 4 fp32.  Past the caches: nothing here reads
 // them again, and as ordinary stores they pushed out codes that were still to
-// be read (16 contexts of 512 to 4,096 into fp32, 377 MB: 94 us, now 67,
-// 5.6 TB/s).
+// be read (16 contexts of 512 to 4,096 into fp32, 377 MB: 94 us, now 66,
+// 5.7 TB/s).
 template <bool F32>
 __device__ __forceinline__ void put16(void* p, long long e, const float* f) {
   u32x4 w;
@@ -721,13 +721,13 @@ struct Ids {
 // operand as they stand.
 //
 // Measured (whole calls, joins included): one sequence of 1,024 positions,
-// head_dim 64, 6.2 us, of which a launch is 2.7 and the rest three loads in a
-// row and one step; 16 sequences of 512 to 4,096 13.1 us (38 MB; whole
+// head_dim 64, 5.7 us, of which a launch is 2.7 and the rest three loads in a
+// row and one step; 16 sequences of 512 to 4,096 12.5 us (38 MB; whole
 // contexts on 128 CUs, bound by what a CU takes in: codes of two steps ahead,
 // and weights formed for the rows that are there alone, changed nothing); one
-// of 32,768, head_dim 128, 19.1 us (67 MB, 14.4 us and 4.7 for the join); 3 to
-// 6 tokens each of 16 sequences of 700 to 8,191 39 us (148 MB, 34 and 5); 64
-// sequences of 4,096, head_dim 64, 53 us (268 MB, 5.1 TB/s).  Streaming as many
+// of 32,768, head_dim 128, 18 us (67 MB, 13.5 us and 4.6 for the join); 3 to 6
+// tokens each of 16 sequences of 700 to 8,191 37 us (148 MB, 32 and 5); 64
+// sequences of 4,096, head_dim 64, 52 us (268 MB, 5.1 TB/s).  Streaming as many
 // bytes without any work takes 7, 12, 27 and 48 us here.
 template <int D, int W>
 struct RowsLds {
@@ -969,13 +969,13 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
 // v_mfma_f32_32x32x16_bf16; a step's 64 positions are turned from codes to
 // bf16 once and staged in LDS for all four (two buffers, one barrier a step;
 // the next step's codes are in flight meanwhile).  1,024 tokens of 16 / 8 heads
-// of 128 at the end of 32,768 positions: 290 us with the join's 12, 930
+// of 128 at the end of 32,768 positions: 293 us with the join's 12, 925
 // TFLOP/s, where a large bf16 product reaches 1,215.  The matrix units are busy
 // 40 % of the time and the vector units, mostly with the weights, as much; two
 // workgroups per CU overlap them in part.  64 rows per wave (half the LDS
 // reads) took 350 us: one wave per SIMD does not hide its own staging.  Without
 // a past the longest tile decides, a step a microsecond: ragged prompts of 33
-// to 2,048 tokens, head_dim 64, 50 us, one of 4,096 83.  Rows of LDS are padded by
+// to 2,048 tokens, head_dim 64, 49 us, one of 4,096 83.  Rows of LDS are padded by
 // 16 bytes, which spreads the eight lanes that a 16-byte read serves at once
 // over all banks.  K rows lie in LDS in the order that makes a lane's 16
 // scores of 32 positions two runs of eight positions, 8h + 16m of half-wave h,
@@ -1374,10 +1374,12 @@ __global__ __launch_bounds__(256) void attn_join_waves(Attn p) {
   }
 }
 
-// Few rows: a workgroup for each, all its partials in flight together.
+// Few rows: a workgroup for each, 64 partials in flight together (32 of 128
+// dimensions: one sequence of 32,768 19.7 us, now 18.6).  5 us, of which a launch
+// is 2.7 and the rest the lengths, the partials and the sums in turn.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join(Attn p) {
-  constexpr int LPP = D / 4, NG = 256 / LPP, PER = 4;  // lanes per partial, groups, partials in flight per group
+  constexpr int LPP = D / 4, NG = 256 / LPP, PER = 64 / NG;  // lanes per partial, groups, partials in flight per group
   __shared__ float lw[kMaxSplits], red1[4];
   __shared__ f32x4 red[NG][LPP];
   const int oh = (int)(blockIdx.x % (unsigned)p.n_q);
