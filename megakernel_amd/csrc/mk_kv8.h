@@ -756,7 +756,7 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
 
   // Table entries of a step, loaded a step before the codes they lead to and
-  // judged only there: the loads are waited for in the order of their issue,
+  // checked only there: the loads are waited for in the order of their issue,
   // so an entry asked for behind codes would arrive behind them.
   const int* row = p.b.table + (long long)s.i * p.b.width;
   const auto ids = [&](int t) {
@@ -1045,7 +1045,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
     const int pos = first_of(16 * w) + 16 * l;
     return row[min(pos >> lb, top)];
   };
-  const auto judge = [&](int w, int& tab) {  // which of them are there; the others' place is taken by block 0
+  const auto confirm = [&](int w, int& tab) {  // which of them are there; the others' place is taken by block 0
     const bool ok = first_of(16 * w) + 16 * l < end && tab >= 0 && tab < p.c.n_blocks;
     tab = ok ? tab : 0;
     return __ballot(ok);
@@ -1146,8 +1146,8 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   if (n > 0) {
     tab0 = window(0);
     tab1 = window(1);
-    ok0 = judge(0, tab0);
-    ok1 = judge(1, tab1);
+    ok0 = confirm(0, tab0);
+    ok1 = confirm(1, tab1);
     load_k(0);
     load_v(0);
   }
@@ -1173,10 +1173,10 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   for (int k = 0; k < n; ++k) {
     const int first = first_of(k), buf = k & 1;
     const unsigned gone = gone_of(k);
-    // window w + 1, looked up and judged during window w, in the place of w - 1
+    // window w + 1, looked up and confirmed during window w, in the place of w - 1
     if ((k & 15) == 12 && k > 16) {
-      if (k & 16) ok0 = judge((k >> 4) + 1, tab0);
-      else ok1 = judge((k >> 4) + 1, tab1);
+      if (k & 16) ok0 = confirm((k >> 4) + 1, tab0);
+      else ok1 = confirm((k >> 4) + 1, tab1);
     }
     stage_v(k + 1);
     load_v(k + 2);
