@@ -97,6 +97,8 @@ _library = None
 def _call(name: str, device: int, *args):
     """Enqueue on the current stream of GPU `device`; raises what the library reports."""
     global _library
+    if device < 0:
+        raise ValueError(f"{name[11:]} needs tensors on a GPU")
     if _library is None:
         _library = _lib.load()
     fn = getattr(_library, name)
@@ -189,6 +191,8 @@ def qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q_out, k_out, eps: float =
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k are [tokens][heads][head_dim], not {tuple(q.shape)} and {tuple(k.shape)}")
     device = q.get_device()
+    if device < 0:  # of other tensors of the host it would be the device that they are expected on
+        raise ValueError(f"q must be on the GPU, not on {q.device}")
     tokens, n_q, dim = q.shape
     n_kv = k.shape[1]
     _whole(pos, torch.int32, (tokens,), device, "pos")

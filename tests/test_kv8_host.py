@@ -224,3 +224,23 @@ def test_tensors_of_a_cache_or_batch_cannot_be_replaced():
         with pytest.raises(AttributeError, match="make another"):
             x.device = 1
         assert x.device == 0
+
+
+def test_host_tensors_never_reach_a_launch(monkeypatch):
+    """Types, shapes and strides are right, so that only the device can be why a call is refused."""
+    def reached(name, device, *args):
+        raise AssertionError(f"{name} was handed host addresses (device {device})")
+
+    monkeypatch.setattr(kv8, "_call", reached)
+    for dtype in (torch.bfloat16, torch.float32):
+        for tokens in (1, 3):
+            q, k = torch.zeros((tokens, 4, 64), dtype=dtype), torch.zeros((tokens, 2, 64), dtype=dtype)
+            gain, inv = torch.ones(64, dtype=torch.bfloat16), torch.ones(32)
+            pos = torch.zeros(tokens, dtype=torch.int32)
+            with pytest.raises(ValueError, match="on the GPU, not on cpu"):
+                kv8.qk_norm_rope(q, k, gain, gain, inv, pos, q, k)
+
+
+def test_no_call_is_made_for_a_device_that_is_no_gpu():
+    with pytest.raises(ValueError, match="op_kv8_read needs tensors on a GPU"):
+        kv8._call("megakernel_op_kv8_read", -1)
