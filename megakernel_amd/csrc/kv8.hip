@@ -202,8 +202,8 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
     // 22, 24 / 15, 34 rows 49 / 49, 24 / 20, 18 / 13, 32 rows 39 / 49, 18 / 20,
     // 13 / 12).
     p.use[MANY] = true;
-    p.use[FEW] = b->n_seq > 1;
     p.few = b->n_seq == 1 ? 0 : d64 && steps > 8 ? 64 : 32;
+    p.use[FEW] = group <= p.few;  // one token has `group` rows
   }
   p.lr[FEW] = 4, p.lr[MANY] = 7;
   p.least[FEW] = 8, p.least[MANY] = 4;

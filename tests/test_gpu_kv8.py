@@ -818,3 +818,13 @@ def test_more_rows_than_workgroups_of_one_launch():
     tol = np.abs(want) * 2.0 ** -8 + (2.0 ** -8 + (2 * 64 * reach + 40 + 16)[..., None] * U) * size
     assert np.all(np.abs(_f64(out[-40:]) - want) <= tol)
     assert not out[:-40].any()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 71), (64, 64), (128, 66), (128, 33), (128, 32)])
+def test_attention_of_more_query_heads_than_the_kernel_for_few_rows_takes(dim, group):
+    """A prompt and a short sequence: a single token has more rows than the
+    limit between the kernels, or as many."""
+    _say(f"attention of {group} query heads per KV head D={dim}")
+    for new in ([1020, 4], [1, 1023]):
+        c = _hint(Case(64, 1, dim, [1023, 1023], new, seed=group, gap=0), 4096)
+        _check_attention(c, group, say=str(new))

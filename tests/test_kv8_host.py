@@ -244,3 +244,12 @@ def test_host_tensors_never_reach_a_launch(monkeypatch):
 def test_no_call_is_made_for_a_device_that_is_no_gpu():
     with pytest.raises(ValueError, match="op_kv8_read needs tensors on a GPU"):
         kv8._call("megakernel_op_kv8_read", -1)
+
+
+@pytest.mark.parametrize("dim,group,n_tokens,max_kv", [(64, 71, 1024, 4096), (128, 66, 1024, 4096), (128, 64, 1040, 1 << 20)])
+def test_no_splits_for_few_rows_where_a_token_has_more(clib, dim, group, n_tokens, max_kv):
+    """Two sequences of so many tokens are not split, and with more query heads
+    per KV head than the kernel for few rows takes, nothing is its own."""
+    for n_kv in (1, 2):
+        c, b = _cache(head_dim=dim, n_kv=n_kv), _batch(n_tokens=n_tokens, max_kv=max_kv)
+        assert clib.megakernel_op_kv8_workspace_bytes(_ref(c), _ref(b), group * n_kv) == 0
