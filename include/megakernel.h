@@ -502,7 +502,7 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
  * out = sum_j softmax_j(scale * q . k_j) v_j, zeros for a row that sees
  * nothing.  Query head h reads KV head h / (n_q / n_kv).  q and out bf16; the
  * scores, the softmax and the sums are fp32, the weights are rounded to bf16
- * for the product with V.  workspace: megakernel_op_kv8_workspace_bytes(...)
+ * for the product with V and for their sum.  workspace: megakernel_op_kv8_workspace_bytes(...)
  * bytes (NULL where that is 0), 16-byte aligned, without an initial value;
  * calls that may overlap in time need one each.  out may not overlap q or the
  * cache.  n_tokens * (n_q / n_kv) is at most 2^30. */

@@ -828,3 +828,49 @@ def test_attention_of_more_query_heads_than_the_kernel_for_few_rows_takes(dim, g
     for new in ([1020, 4], [1, 1023]):
         c = _hint(Case(64, 1, dim, [1023, 1023], new, seed=group, gap=0), 4096)
         _check_attention(c, group, say=str(new))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_late_key_that_decides_a_row(dim):
+    """The first key's score is a row's reference; a key of a later step of the
+    same wave, less than 2^8 times as heavy, decides the row.  Weights are
+    rounded to bf16, relative h = 2^-8, but their sum is that of the rounded
+    ones, so an output is off by its own rounding, |o| h, and by
+    h sum_j p_j |v_j - o| (1 + 2 h, as the sum is off by h): near nothing where
+    the deciding key's value is the output.  Terms of fp32, 16 u and 2 D u of a
+    score of 8, as in the general tolerance."""
+    _say(f"late key D={dim}")
+    h, block = 2.0 ** -8, 16
+    late = 4 * 64 + 5  # waves take every fourth step: positions 0 and 261 are one wave's
+    for weight in (1 + 0.97 * h, 128 * (1 + 0.97 * h), 180.37, 3 * (1 + 0.65 * h), 254.6):
+        c = Case(block, 1, dim, [late + 1], [1], seed=41)
+        c.table[:] = -1
+        c.table[0, 0], c.table[0, late // block] = 0, 1
+        c.pool.ks[:], c.pool.vs[:] = 1.0, 1.0
+        c.pool.k[:] = 0
+        c.pool.k[:, :, :, 0] = 0xF7  # -240: the other keys of the two blocks
+        c.pool.k[0, 0, 0, 0] = 0x00
+        c.pool.k[1, 0, late % block, 0] = 0x50  # 8
+        c.pool.v[0, 0, :, 0] = c.pool.v[1, 0, :, late % block] = 0x38 + np.arange(dim) % 8  # 1, 1.125, .. 1.875
+        c.pool.v[0, 0, 0, 0] = 0xB8  # and one dimension in which they differ
+        c.upload()
+        _hint(c, 64)
+        assert kv8.workspace_bytes(c.cache, c.batch, 1) == 0
+        q = torch.zeros((1, 1, dim), dtype=torch.bfloat16)
+        q[..., 0] = 1
+        scale, want = float(np.log(weight) / 8), np.zeros((1, 1, dim))
+        c.pool.attention(c.table, c.start, c.lens, _f64(q), want, scale)
+        out = torch.empty((1, 1, dim), dtype=torch.bfloat16, device="cuda")
+        kv8.attention(c.cache, c.batch, q.cuda(), out, scale=scale)
+        torch.cuda.synchronize()
+        there = [c.pool.place(c.table[0], j) for j in range(late + 1)]
+        keys, v = (np.stack([c.pool.values(*at)[i][0] for at in there if at]) for i in (0, 1))
+        p = np.exp(keys[:, 0] * scale)  # the first key's is 1
+        assert p.max() == p[-1] and abs(p[-1] / weight - 1) < 1e-12
+        p /= p.sum()
+        o = p @ v
+        np.testing.assert_allclose(o, want[0, 0], rtol=1e-9)
+        size = p @ np.abs(v)
+        tol = np.abs(o) * h + (p @ np.abs(v - o)) * h * (1 + 2 * h) + (16 + 2 * dim * 8) * U * size
+        off = np.abs(_f64(out)[0, 0] - o)
+        assert np.all(off <= tol), f"weight {weight}: {np.max(off / tol):.2f} of the tolerance"
