@@ -442,7 +442,7 @@ typedef struct {
 /* A pool of n_blocks blocks of `block` positions (16, 32, 64 or 128):
  *   k        e4m3 codes [n_blocks][n_kv][block][head_dim]
  *   v        e4m3 codes [n_blocks][n_kv][head_dim][block]
- *   k_scale, v_scale  fp32 [n_blocks][n_kv], powers of two
+ *   k_scale, v_scale  fp32 [n_blocks][n_kv], powers of two, 2^-126 to 2^119
  * value = code * scale.  head_dim 64 or 128.  Codes and scales of a block
  * need no initial value. */
 typedef struct {
@@ -480,11 +480,12 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
 
 /* Quantise rows of K and V (n_kv heads, bf16 or fp32, one type) into their
  * blocks.  Per block, head and K / V: the scale is the smallest power of two
- * s >= 2^-126 with |x| <= 448 s for the new rows, or the block's own scale
- * where it is larger and older rows are in the block; codes are x / s rounded
- * to nearest even.  Where the scale grows, the older rows' codes are rounded
- * again from their values.  Infinities do not count for the scale and become
- * +-448 s; NaN stays NaN.  Rows whose block is missing or whose position is
+ * s >= 2^-126 with |x| <= 448 s for the new rows, 2^119 at most, or the block's
+ * own scale where it is larger and older rows are in the block; codes are x / s
+ * rounded to nearest even.  Where the scale grows, the older rows' codes are
+ * rounded again from their values.  Infinities do not count for the scale and
+ * become +-448 s, as do values beyond 448 * 2^119 (1.75 * 2^127), so what is read
+ * back is finite; NaN stays NaN.  Rows whose block is missing or whose position is
  * negative are dropped.  Other rows of a block are left as they were.  A block
  * that a call appends to may stand in one table entry only, of one sequence;
  * blocks that nothing is appended to may be shared. */

@@ -208,22 +208,25 @@ __global__ __launch_bounds__(256) void norm_rope(Rows q, Rows k, const uint16_t*
 
 // ------------------------------------------------------- quantised append
 // Exponent of the smallest power of two s >= 2^-126 with amax <= 448 s
-// (448 = 1.75 * 2^8).  Zero rows give 2^-126, so that a block that starts
-// with them takes the scale of the rows that follow.
+// (448 = 1.75 * 2^8), but at most 2^119: beyond, codes times the scale would
+// pass fp32's and bf16's largest values, and an infinite value reaches rows
+// that do not see it (0 * inf).  Zero rows give 2^-126, so that a block that
+// starts with them takes the scale of the rows that follow.
+constexpr float kTop = 0x1.cp127f;  // 448 * 2^119
 __device__ __forceinline__ int scale_exp(float amax) {
   if (!(amax > 0.f)) return -126;
   int e = ilogbf(amax) - 8;
   if (amax > ldexpf(448.f, e)) ++e;
-  return max(e, -126);
+  return min(max(e, -126), 119);
 }
 
 // Codes of four values that were divided by the scale: nearest, ties to even.
-// Finite values are within 448.
+// The values are within 448, or saturate()d.
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
   const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
-// Infinities to +-448; NaN stays.
+// Infinities, and what is beyond 448 s of the largest scale, to +-448; NaN stays.
 __device__ __forceinline__ float saturate(float x) { return x != x ? x : fminf(fmaxf(x, -448.f), 448.f); }
 
 // Four codes re-rounded after multiplying by a power of two of at most one.
@@ -347,8 +350,8 @@ __global__ __launch_bounds__(256) void append(Cache c, Batch b, Rows kr, Rows vr
       vr8[p][i].top(vtop);
     }
   float kmax = Raw8<SRC32>::top_value(ktop), vmax = Raw8<SRC32>::top_value(vtop);
-  const bool odd = __any(!(kmax < INFINITY) || !(vmax < INFINITY));  // some value is no finite number
-  if (__builtin_expect(odd, 0)) {                                    // the scale is that of the finite values
+  const bool odd = __any(!(kmax <= kTop) || !(vmax <= kTop));  // some value is no finite number, or too large for any scale
+  if (__builtin_expect(odd, 0)) {                              // the scale is that of the finite values
     kmax = vmax = 0.f;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p)

@@ -216,8 +216,9 @@ def _one_gpu(cache: Cache, batch: Batch):
 def append(cache: Cache, batch: Batch, k, v):
     """Quantise rows k, v [n_tokens][n_kv][head_dim] (bf16 or fp32) into their
     blocks.  A block and head has one scale, the smallest power of two that
-    fits its rows into e4m3; rows that a block already holds are rounded again
-    where a new row makes its scale grow.  A block that a call appends to may
+    fits its rows into e4m3 (2^-126 to 2^119; what is larger saturates at
+    448 * 2^119); rows that a block already holds are rounded again where a new
+    row makes its scale grow.  A block that a call appends to may
     stand in one table entry only."""
     _one_gpu(cache, batch)
     shape = (batch.n_tokens, cache.n_kv, cache.head_dim)

@@ -13,19 +13,19 @@ import numpy as np
 
 from . import fp8
 
-MIN_EXP = -126
+MIN_EXP, MAX_EXP = -126, 119  # 448 * 2^119 is fp32's last such value
 
 
 def scale_exp(amax: float) -> int:
-    """The smallest e >= -126 with amax <= 448 * 2^e (-126 for zero)."""
+    """The smallest e >= -126 with amax <= 448 * 2^e (-126 for zero), at most 119."""
     if amax <= 0:
         return MIN_EXP
     m, e = math.frexp(amax)
-    return max(MIN_EXP, e - 9 + (m > 0.875))
+    return min(max(MIN_EXP, e - 9 + (m > 0.875)), MAX_EXP)
 
 
 def encode(x: np.ndarray, e: int) -> np.ndarray:
-    """Codes of x / 2^e: infinities saturate, NaN is the NaN code."""
+    """Codes of x / 2^e: what is beyond 448 saturates, NaN is the NaN code."""
     with np.errstate(invalid="ignore"):
         y = np.clip(np.ldexp(np.asarray(x, np.float64), -e), -448.0, 448.0)
     c = fp8.e4m3_encode(np.nan_to_num(y, nan=0.0).astype(np.float32))

@@ -874,3 +874,69 @@ def test_a_late_key_that_decides_a_row(dim):
         tol = np.abs(o) * h + (p @ np.abs(v - o)) * h * (1 + 2 * h) + (16 + 2 * dim * 8) * U * size
         off = np.abs(_f64(out)[0, 0] - o)
         assert np.all(off <= tol), f"weight {weight}: {np.max(off / tol):.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float32])
+def test_rows_at_the_end_of_the_range_are_read_back_finite(dim, src):
+    """The type's lowest and largest values, those around the last that fits,
+    1.75 * 2^127, and infinities beside them."""
+    _say(f"rows of the lowest value D={dim} {src}")
+    last = 1.75 * 2.0 ** 127
+    values = [torch.finfo(src).min, torch.finfo(src).max, last, last * (1 + 2.0 ** -7), 1.9375 * 2.0 ** 127, last * (1 - 2.0 ** -8)]
+    for block in (16, 64):
+        c = Case(block, 2, dim, [block + 3, 9], [block + 1, 9], seed=42)
+        k, v = c.rows(2, src), c.rows(2, src)
+        for i, x in enumerate(values):
+            k[i + 2, i % 2, 7 * i], v[i + 1, 1 - i % 2, 9 * i] = x, -x
+        v[3, 0, 1], k[0] = np.inf, torch.finfo(src).min
+        c.pool.append(c.table, c.start, c.lens, _f64(k), _f64(v))
+        assert c.pool.ks.max() == c.pool.vs.max() == 2.0 ** 119
+        kv8.append(c.cache, c.batch, k.cuda(), v.cuda())
+        torch.cuda.synchronize()
+        c.same_pool()
+        for dst in (torch.bfloat16, torch.float32):
+            want = [np.zeros(k.shape) for _ in range(2)]
+            c.pool.read(c.table, c.start, c.lens, *want)
+            got = [torch.empty(k.shape, dtype=dst, device="cuda") for _ in range(2)]
+            kv8.read(c.cache, c.batch, *got)
+            torch.cuda.synchronize()
+            for g, w in zip(got, want):
+                assert np.isfinite(w).all()
+                np.testing.assert_array_equal(_f64(g), w)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,n_kv,hint", [(2, 1, 64), (80, 2, 64), (2, 2, 1 << 20)])
+def test_rows_of_the_lowest_value_reach_no_row_that_does_not_see_them(dim, group, n_kv, hint):
+    """Padding rows of the type's lowest value behind a sequence's own, and
+    codes of 448 that an earlier sequence left behind both.  The sequence's own
+    rows are held to the general tolerance (what they see is below 448 * 2^-3),
+    those at the padding's positions to nothing."""
+    _say(f"lowest value unseen D={dim} group {group} hint {hint}")
+    lens, own = [190, 70], [185, 61]
+    c = Case(32, n_kv, dim, lens, [140, 40], seed=43)
+    c.pool.k[:], c.pool.v[:] = np.where(c.pool.k == 0x60, 0x7E, c.pool.k), np.where(c.pool.v == 0x60, 0x7E, c.pool.v)
+    c.upload()
+    k, v = (c.rows(n_kv, torch.bfloat16) for _ in range(2))
+    for i, n in enumerate(own):
+        first = int(c.start[i + 1]) - (lens[i] - n)
+        k[first : c.start[i + 1]] = v[first : c.start[i + 1]] = torch.finfo(torch.bfloat16).min
+    c.pool.append(c.table, c.start, c.lens, _f64(k), _f64(v))
+    kv8.append(c.cache, c.batch, k.cuda(), v.cuda())
+    torch.cuda.synchronize()
+    c.same_pool()
+    _hint(c, hint)
+    q = c.rows(n_kv * group, torch.bfloat16, 1.5)
+    want, out = np.zeros(q.shape), torch.empty_like(q, device="cuda")
+    size, reach = c.pool.attention(c.table, c.start, c.lens, _f64(q), want, dim ** -0.5)
+    kv8.attention(c.cache, c.batch, q.cuda(), out)
+    torch.cuda.synchronize()
+    got = _f64(out)
+    for i, n in enumerate(own):
+        rows = slice(int(c.start[i]), int(c.start[i + 1]) - (lens[i] - n))
+        w, n_seen = want[rows], lens[i]
+        tol = np.abs(w) * 2.0 ** -8 + (2.0 ** -8 + (2 * dim * reach[rows] + n_seen + 16)[..., None] * U) * size[rows]
+        tol += n_seen * 2.0 ** -126 * 448 * 2.0 ** -3
+        n_bad = int((~(np.abs(got[rows] - w) <= tol)).sum())
+        assert n_bad == 0, f"sequence {i}: {n_bad} outputs off"

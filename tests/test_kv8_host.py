@@ -253,3 +253,12 @@ def test_no_splits_for_few_rows_where_a_token_has_more(clib, dim, group, n_token
     for n_kv in (1, 2):
         c, b = _cache(head_dim=dim, n_kv=n_kv), _batch(n_tokens=n_tokens, max_kv=max_kv)
         assert clib.megakernel_op_kv8_workspace_bytes(_ref(c), _ref(b), group * n_kv) == 0
+
+
+def test_scales_stop_where_values_would_leave_fp32():
+    top = 448.0 * 2.0 ** 119
+    for a, e in ((top / 2, 118), (top, 119), (1.9375 * 2.0 ** 127, 119), (float(np.finfo(np.float32).max), 119)):
+        assert okv8.scale_exp(a) == e
+        codes = okv8.encode(np.array([a, -a, np.inf]), e)
+        np.testing.assert_array_equal(okv8.decode(codes) * 2.0 ** e, [min(a, top), -min(a, top), 448.0 * 2.0 ** e])
+        assert np.isfinite(np.float32(448.0 * 2.0 ** e))
