@@ -940,3 +940,58 @@ def test_rows_of_the_lowest_value_reach_no_row_that_does_not_see_them(dim, group
         tol += n_seen * 2.0 ** -126 * 448 * 2.0 ** -3
         n_bad = int((~(np.abs(got[rows] - w) <= tol)).sum())
         assert n_bad == 0, f"sequence {i}: {n_bad} outputs off"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_tiles_refresh_their_block_ids(dim):
+    """attn_tile looks block ids up 16 steps of 64 positions at a time, the
+    first two such windows before it starts; a whole context of 79 steps
+    refreshes each of their two places at least once.  Three of the KV heads are
+    compared, of a pool that has only them."""
+    block, n_kv, lens, new = 16, 64, [5003], [449]
+    _say(f"attention tiles, 79 steps D={dim}")
+    c = _hint(Case(block, n_kv, dim, lens, new, seed=44 + dim, missing=0.05), 64)
+    assert kv8.workspace_bytes(c.cache, c.batch, n_kv) == 0  # whole
+    q, out = c.rows(n_kv, torch.bfloat16, 1.5), torch.full((c.tokens, n_kv, dim), 5.0, dtype=torch.bfloat16, device="cuda")
+    kv8.attention(c.cache, c.batch, q.cuda(), out)
+    torch.cuda.synchronize()
+    heads, p = [0, 31, 63], c.pool
+    some = okv8.Pool(p.k[:, heads], p.v[:, heads], p.ks[:, heads], p.vs[:, heads])
+    want = np.zeros((c.tokens, 3, dim))
+    size, reach = some.attention(c.table, c.start, c.lens, _f64(q[:, heads]), want, dim ** -0.5)
+    tol = np.abs(want) * 2.0 ** -8 + (2.0 ** -8 + (2 * dim * reach + lens[0] + 16)[..., None] * U) * size
+    n_bad = int((~(np.abs(_f64(out[:, heads]) - want) <= tol)).sum())
+    assert n_bad == 0, f"{n_bad} outputs off"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("length", [33100, 131300])
+def test_attention_of_one_row_in_hundreds_of_parts(dim, length):
+    """A part is 8 steps of 64 positions at least: 65 parts, one more than
+    attn_join reads at once, and 257, of which 256 are the most."""
+    _say(f"attention of {length} positions D={dim}")
+    c = Case(128, 1, dim, [length], [1], seed=45, missing=0.02)
+    assert kv8.workspace_bytes(c.cache, c.batch, 3) > 0
+    _check_attention(c, 3)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("length", [20100, 131300])
+def test_attention_of_hundreds_of_parts_joined_by_waves(dim, length):
+    """A single token over 40 and 256 parts (a wave reads 32 at a time, 16 of
+    head_dim 128) beside a prompt, which makes the rows too many for a
+    workgroup each."""
+    _say(f"attention of {length} positions beside a prompt D={dim}")
+    c = _hint(Case(128, 1, dim, [length, 300], [1, 300], seed=46, missing=0.02), 1 << 20)
+    assert kv8.workspace_bytes(c.cache, c.batch, 16) > 0 and c.tokens * 16 > 4096
+    _check_attention(c, 16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_one_tile_in_dozens_of_parts(dim):
+    """120 rows of 60 tokens, more than attn_rows takes where contexts may be
+    long: 315 steps in parts of 4."""
+    _say(f"one tile of 20,100 positions D={dim}")
+    c = _hint(Case(64, 1, dim, [20100], [60], seed=47, missing=0.02), 1 << 20)
+    assert kv8.workspace_bytes(c.cache, c.batch, 2) > 0
+    _check_attention(c, 2)
