@@ -14,7 +14,8 @@ included; nothing is copied, and no call waits.  Work is enqueued on torch's
 current stream of that GPU, so tensors that another stream wrote need that
 stream waited for, as with torch's own operators.  Calls can be captured into
 a graph: a replay reads lengths and tables anew, while sizes stay fixed.  No
-gradients are recorded.
+gradients are recorded: while torch records them (outside torch.no_grad()),
+tensors that require one are refused.
 
     cache = kv8.Cache(k, v, k_scale, v_scale)      # or kv8.Cache.empty(...)
     batch = kv8.Batch(table, q_start, kv_len, n_tokens)
@@ -57,9 +58,16 @@ class _CBatch(ctypes.Structure):
                 ("max_kv", ctypes.c_int)]
 
 
+def _no_grad(t, name: str):
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and none is recorded here: call under torch.no_grad()")
+
+
 def _whole(t, dtype, shape, device: int, name: str):
     """A contiguous tensor of one type and shape on GPU `device`; None in
     `shape` is any size."""
+    if t.requires_grad:
+        _no_grad(t, name)
     if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
         return
     if not t.is_cuda:
@@ -77,6 +85,8 @@ def _whole(t, dtype, shape, device: int, name: str):
 def _rows(t, shape, device: int, name: str, types=_TYPES) -> bytes:
     """Rows [tokens][heads][dim] with any token and head stride, as a
     megakernel_rows."""
+    if t.requires_grad:
+        _no_grad(t, name)
     typ = types.get(t.dtype)
     if typ is None or t.shape != shape or t.get_device() != device:
         if typ is None:

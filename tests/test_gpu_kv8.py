@@ -995,3 +995,21 @@ def test_attention_of_one_tile_in_dozens_of_parts(dim):
     c = _hint(Case(64, 1, dim, [20100], [60], seed=47, missing=0.02), 1 << 20)
     assert kv8.workspace_bytes(c.cache, c.batch, 2) > 0
     _check_attention(c, 2)
+
+
+def test_gradients_that_would_be_lost_are_refused():
+    _say("gradients")
+    c = Case(16, 2, 64, [20], [3], seed=48)
+    q, k = c.rows(4, torch.bfloat16).cuda(), c.rows(2, torch.bfloat16).cuda()
+    gain = torch.nn.Parameter(torch.ones(64, dtype=torch.bfloat16, device="cuda"))
+    inv, pos = torch.ones(32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    wants = k.clone().requires_grad_()
+    calls = [lambda: kv8.qk_norm_rope(q, k, gain, gain, inv, pos, torch.empty_like(q), torch.empty_like(k)),
+             lambda: kv8.append(c.cache, c.batch, wants, k), lambda: kv8.read(c.cache, c.batch, torch.empty_like(k), wants),
+             lambda: kv8.attention(c.cache, c.batch, torch.nn.Parameter(q), torch.empty_like(q))]
+    for call in calls:
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    torch.cuda.synchronize()

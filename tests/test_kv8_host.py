@@ -262,3 +262,16 @@ def test_scales_stop_where_values_would_leave_fp32():
         codes = okv8.encode(np.array([a, -a, np.inf]), e)
         np.testing.assert_array_equal(okv8.decode(codes) * 2.0 ** e, [min(a, top), -min(a, top), 448.0 * 2.0 ** e])
         assert np.isfinite(np.float32(448.0 * 2.0 ** e))
+
+
+def test_tensors_that_require_a_gradient_are_refused_while_torch_records_them():
+    rows, gain = torch.zeros((2, 1, 64), requires_grad=True), torch.ones(64, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="q requires a gradient.*no_grad"):
+        kv8._rows(rows, (2, 1, 64), -1, "q")
+    with pytest.raises(ValueError, match="q_gain requires a gradient"):
+        kv8._whole(gain, torch.bfloat16, (64,), -1, "q_gain")
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            kv8._rows(rows, (2, 1, 64), -1, "q")
+            kv8._whole(gain, torch.bfloat16, (64,), -1, "q_gain")
+    kv8._rows(rows.detach(), (2, 1, 64), -1, "q")
