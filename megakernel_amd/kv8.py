@@ -176,13 +176,15 @@ class Batch(_Fixed):
     """
 
     def __init__(self, table, q_start, kv_len, n_tokens: int, max_kv: int = 0):
+        if not (0 <= n_tokens <= 1 << 27 and 0 <= max_kv < 1 << 31):  # the library's integers have 32 bits
+            raise ValueError(f"n_tokens {n_tokens} (0 to 2^27), max_kv {max_kv} (0 to 2^31 - 1)")
         device = kv_len.get_device()
         _whole(kv_len, torch.int32, (None,), device, "kv_len")
         n_seq = kv_len.shape[0]
         _whole(table, torch.int32, (n_seq, None), device, "table")
         _whole(q_start, torch.int32, (n_seq + 1,), device, "q_start")
-        if n_tokens < 0 or max_kv < 0 or table.shape[1] < 1:
-            raise ValueError(f"n_tokens {n_tokens} and max_kv {max_kv} (at least 0), table width {table.shape[1]} (at least 1)")
+        if table.shape[1] < 1:
+            raise ValueError("table needs a width of at least 1")
         self.table, self.q_start, self.kv_len = table, q_start, kv_len
         self.n_seq, self.n_tokens, self.max_kv, self.device = n_seq, int(n_tokens), int(max_kv), device
         # of no sequence there are no addresses to hand over, and nothing to do

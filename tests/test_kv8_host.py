@@ -275,3 +275,11 @@ def test_tensors_that_require_a_gradient_are_refused_while_torch_records_them():
             kv8._rows(rows, (2, 1, 64), -1, "q")
             kv8._whole(gain, torch.bfloat16, (64,), -1, "q_gain")
     kv8._rows(rows.detach(), (2, 1, 64), -1, "q")
+
+
+@pytest.mark.parametrize("n_tokens,max_kv", [(2 ** 32 + 5, 0), (-1, 0), (2 ** 27 + 1, 0), (5, 2 ** 32 + 64), (5, 2 ** 31), (5, -1)])
+def test_sizes_that_32_bits_do_not_hold_are_refused(n_tokens, max_kv):
+    """Handed on, 2^32 + 5 rows would be 5."""
+    i32 = torch.int32
+    with pytest.raises(ValueError, match="n_tokens .* max_kv"):
+        kv8.Batch(torch.zeros((1, 1), dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(1, dtype=i32), n_tokens, max_kv)
