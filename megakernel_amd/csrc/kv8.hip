@@ -425,8 +425,9 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
     set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows", op, batch->n_tokens, n_q / cache->n_kv);
     return -1;
   }
-  if (!(scale > 0.f && scale < INFINITY)) {
-    set_err("%s: scale=%g must be positive and finite", op, scale);
+  const float scale2 = scale * 1.4426950408889634f;  // scores are taken to base 2
+  if (!(scale > 0.f && scale2 < INFINITY)) {
+    set_err("%s: scale=%g must be positive and finite, also times log2(e)", op, scale);
     return -1;
   }
   const Plan pl = plan(cache, batch, n_q);
@@ -443,7 +444,7 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   p.out = rows_of(out);
   p.n_q = n_q;
   p.group = n_q / cache->n_kv;
-  p.scale = scale * 1.4426950408889634f;
+  p.scale = scale2;
   p.few = pl.few;
   char* ws = static_cast<char*>(d_workspace);
   for (int k = 0; k < 2; ++k) {

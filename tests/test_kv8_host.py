@@ -283,3 +283,9 @@ def test_sizes_that_32_bits_do_not_hold_are_refused(n_tokens, max_kv):
     i32 = torch.int32
     with pytest.raises(ValueError, match="n_tokens .* max_kv"):
         kv8.Batch(torch.zeros((1, 1), dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(1, dtype=i32), n_tokens, max_kv)
+
+
+def test_a_scale_that_leaves_fp32_in_base_2_is_refused(clib):
+    """It would make NaN of every score of zero."""
+    c, b, r, far = _ref(_cache()), _ref(_batch()), _ref(_r()), _ref(_r(2 * FAKE))
+    _refused(clib, clib.megakernel_op_kv8_attention(c, b, r, far, 8, 3e38, None, 0, None), "scale=3e+38")
