@@ -470,7 +470,7 @@ typedef struct {
 
 /* RMSNorm of every head of q and k with its gain (bf16 [head_dim]), then the
  * rotate-half rotation by pos[t] * inv_freq[i] (fp32 [head_dim / 2]; the
- * product is formed exactly).  n_q heads of q, n_kv of k; q and k have one
+ * angle is formed in fp64).  n_q heads of q, n_kv of k; q and k have one
  * type, q_out and k_out one type, bf16 or fp32; an output may be its own
  * input.  The arithmetic is fp32, rounded once. */
 int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* k, const void* q_gain,
@@ -506,7 +506,9 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
  * for the product with V and for their sum.  workspace: megakernel_op_kv8_workspace_bytes(...)
  * bytes (NULL where that is 0), 16-byte aligned, without an initial value;
  * calls that may overlap in time need one each.  out may not overlap q or the
- * cache.  n_tokens * (n_q / n_kv) is at most 2^30. */
+ * cache.  n_tokens * (n_q / n_kv) is at most 2^30.  The sum over the positions
+ * comes before the division, with weights of up to 2^8 each: a row's values are
+ * to stay below 2^119 / positions, or it may be infinite. */
 long long megakernel_op_kv8_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, int n_q);
 int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                                 const megakernel_rows* q, const megakernel_rows* out, int n_q, float scale,

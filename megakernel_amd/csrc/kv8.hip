@@ -222,6 +222,13 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
     // part more for every row tile: with these over the two, some CUs would
     // start a third when the others end (16 of 700 to 8,191, 128: 37.6, now
     // 35.0; 12 of 500 to 20,000: 58 / 54; four of 8,000 alike 19.3 / 19.9).
+    // `tiles` is a bound from sizes alone: beside a prompt it counts every
+    // sequence as if it had `few` rows, so with 8 KV heads nothing is split
+    // from 8 sequences of head_dim 64 on, or 16 of 128, and of single tokens
+    // alone from about 30.  One context of 32,768 among others of 512 is then
+    // walked whole: 31 single tokens 70 us (head_dim 128 190), 16, split, 15
+    // (22); beside a prompt of 1,024 tokens 8 of head_dim 64 113, 6, split, 34,
+    // and 15 of 128 274, 14, split, 53.
     const long long units = tiles * c->n_kv;
     if (units < 256 && steps * (256 - units) > 256 * (d64 ? 40 : 16)) {
       p.target[FEW] = (512 + c->n_kv - 1) / c->n_kv - (b->n_seq > 1 ? (int)tiles / 2 : 0);
@@ -458,8 +465,9 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
   // tokens whose rows may have splits to join
   long long tokens = batch->n_tokens;
   if (!pl.target[MANY] && pl.use[MANY] && tokens > (long long)batch->n_seq * (pl.few / p.group)) tokens = (long long)batch->n_seq * (pl.few / p.group);
-  // a workgroup for every row, or where rows are many a wave for four (verify of
-  // 1,152 rows 41.0 / 43.6 us in all, a prompt of 16,384 336 / 315)
+  // a workgroup for every row, or where rows are many a wave for four (us in all,
+  // in a graph: one row of 32,768 positions 18.9 / 31.5, 1,056 rows of drafted
+  // tokens 38.8 / 40.8, a prompt's 16,384 335 / 311)
   const bool each = tokens * n_q <= 4096;
   const long long joins = !need ? 0 : each ? tokens * n_q : (tokens * ((n_q + 3) / 4) + 3) / 4;
   if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;

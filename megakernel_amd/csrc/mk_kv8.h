@@ -158,10 +158,12 @@ __device__ __forceinline__ void store8(void* p, long long e, const float (&f)[8]
 // lane j holds elements 8j..8j+7 of both halves, so a pair never leaves its
 // lane and the mean is a DPP sum.  The angle is a product of a 24-bit and a
 // 31-bit number, formed and reduced to a fraction of a turn in fp64 (fp32
-// would be off by 2^-24 of an angle of up to 1e5 radians); the sine and
-// cosine of the fraction are fp32.  Every head forms its own, which the loads
-// hide: 8,192 tokens of 24 heads of 128, fp32 to bf16 (151 MB), take 28 us, 5.4
-// TB/s; 16 tokens 2.7 us, an empty launch.
+// would be off by 2^-24 of an angle of up to 1e5 radians; fp64's roundings are
+// off by 2^-52); the sine and cosine of the fraction are fp32.  Every head
+// forms its own.  8,192 tokens of 24 heads of 128, fp32 to bf16 (151 MB), take
+// 28 us, 5.4 TB/s; bf16 in place (101 MB) 22.5, 4.5 TB/s, and of 64 (50 MB)
+// 15.7, 3.2 TB/s, where the arithmetic is no longer behind the loads; 16 tokens
+// 2.7 us in a graph, where an empty launch takes as long.
 template <int D, bool SRC32, bool DST32>
 __global__ __launch_bounds__(256) void norm_rope(Rows q, Rows k, const uint16_t* __restrict__ qg,
                                                  const uint16_t* __restrict__ kg, const float* __restrict__ freq,
@@ -297,8 +299,8 @@ struct Raw8 {
 // workgroup holds 256 / T heads.  The rows stay in registers as they were
 // loaded between the maximum and the rounding, so the input is read once (66
 // registers from bf16; expanded to fp32 it took 104, and 35 us where this takes
-// 24: 16,499 rows of 8 heads of 128 in ragged prompts, 101 MB, 4.2 TB/s).  One
-// row to each of 16 sequences takes 6 us: three loads in a row (lengths, table,
+// 24: 16,499 rows of 8 heads of 128 in ragged prompts, 101 MB, 4.2 TB/s; from
+// fp32 41 us, 169 MB, 4.1 TB/s).  One row to each of 16 sequences takes 6 us: three loads in a row (lengths, table,
 // rows) and the launch.
 template <int D, int T, int PASSES, bool SRC32>
 __global__ __launch_bounds__(256) void append(Cache c, Batch b, Rows kr, Rows vr) {
@@ -986,8 +988,8 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
 // v_mfma_f32_32x32x16_bf16; a step's 64 positions are turned from codes to
 // bf16 once and staged in LDS for all four (two buffers, one barrier a step;
 // the next step's codes are in flight meanwhile).  1,024 tokens of 16 / 8 heads
-// of 128 at the end of 32,768 positions: 293 us with the join's 12, 925
-// TFLOP/s, where a large bf16 product reaches 1,215.  The matrix units are busy
+// of 128 at the end of 32,768 positions: 289 us with the join's 13, 935
+// TFLOP/s, where a large bf16 product reaches 1,370.  The matrix units are busy
 // 40 % of the time and the vector units, mostly with the weights, as much; two
 // workgroups per CU overlap them in part.  64 rows per wave (half the LDS
 // reads) took 350 us: one wave per SIMD does not hide its own staging.  Without
@@ -1021,7 +1023,10 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
   const int head = item % p.c.n_kv;
   Item it;
-  // the last items first: a prompt's last row tiles have the most positions
+  // The last items first: a prompt's last row tiles have the most positions.
+  // Of several prompts the last sequence's tiles start first, whatever its
+  // length (prompts of 33 to 2,048 tokens ascending / shuffled / descending:
+  // head_dim 64 54 / 56 / 57 us, 128 84 / 86 / 96).
   if (!find_split<MANY>(p, p.d[MANY].items - 1 - item / p.c.n_kv, it)) return;
   const Seq& s = it.s;
   const int l = (int)(threadIdx.x & 63u), wv = wave_id(), tid = (int)threadIdx.x;
@@ -1391,8 +1396,8 @@ __global__ __launch_bounds__(256) void attn_join_waves(Attn p) {
   }
 }
 
-// Few rows: a workgroup for each, 64 partials in flight together (32 of 128
-// dimensions: one sequence of 32,768 19.7 us, now 18.6).  5 us, of which a launch
+// Few rows: a workgroup for each, 64 partials in flight together (one sequence
+// of 32,768, head_dim 128, in a graph 18.9 us; with 32 19.8).  5 us, of which a launch
 // is 2.7 and the rest the lengths, the partials and the sums in turn.
 template <int D>
 __global__ __launch_bounds__(256) void attn_join(Attn p) {
