@@ -486,7 +486,9 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
  * rounded again from their values.  Infinities do not count for the scale and
  * become +-448 s, as do values beyond 448 * 2^119 (1.75 * 2^127), so what is read
  * back is finite; NaN stays NaN.  Rows whose block is missing or whose position is
- * negative are dropped.  Other rows of a block are left as they were.  A block
+ * negative are dropped.  Other rows of a block are left as they were.  A row at
+ * the block's first place starts the block anew; one further on stands behind
+ * rows that were appended before it, whose codes and scale are read.  A block
  * that a call appends to may stand in one table entry only, of one sequence;
  * blocks that nothing is appended to may be shared. */
 int megakernel_op_kv8_append(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
