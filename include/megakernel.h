@@ -516,6 +516,37 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
                                 const megakernel_rows* q, const megakernel_rows* out, int n_q, float scale,
                                 void* workspace, long long workspace_bytes, void* stream);
 
+/* What scores are beyond scale * q . k, and which positions a row sees beyond
+ * the causal ones.  For the row at position p and a position j:
+ *   s = softcap * tanh(scale * q . k / softcap)   (softcap 0: scale * q . k)
+ *       - slopes[query head] * |p - j|            (fp32 [n_q], finite; NULL: none)
+ * seen if lo <= j < hi, with
+ *   lo = max(0, first[row], p + 1 - window)       (int [n_tokens]; window 0: none)
+ *   hi = p + 1, or prefix[sequence] if that is more (int [n_seq])
+ * so `first` is where the row's document begins, `window` how many positions
+ * it looks back on, its own among them, and the rows of a prefix see it whole.
+ * softcap is 0 or 2^-30 to 2^30.  Positions are those of the cache: after
+ * megakernel_op_kv8_compact the places that rows were moved to.  The arrays are
+ * read when a call runs, and values beyond a sequence's bounds are cut to them. */
+typedef struct {
+  const float* slopes;
+  const int* first;
+  const int* prefix;
+  float softcap;
+  int window;
+} megakernel_kv8_scores;
+
+/* megakernel_op_kv8_attention with such scores, and with the rows'
+ * log-sum-exps: lse [n_tokens][n_q] (fp32, NULL where not wanted) receives
+ * ln sum_j e^s, -infinity for a row that sees nothing.  Its workspace is of
+ * megakernel_op_kv8_scored_workspace_bytes(...) bytes. */
+long long megakernel_op_kv8_scored_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                                   const megakernel_kv8_scores* scores, int n_q);
+int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                       const megakernel_kv8_scores* scores, const megakernel_rows* q,
+                                       const megakernel_rows* out, float* lse, int n_q, float scale, void* workspace,
+                                       long long workspace_bytes, void* stream);
+
 /* Self-test of the hand-off primitive that replaces the reference's grid
  * barrier (src/barriers.cuh:38-73): one workgroup per CU runs `rounds`
  * all-gather rounds of tagged words (full tags and 4-bit packed pairs,

@@ -171,12 +171,14 @@ struct Plan {
 // Lengths are on the device, so what is chosen here goes by the sizes that
 // the host has: rows, sequences, and how long contexts may get (max_kv).
 // Every choice is right for any lengths.
-static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q) {
+static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q, int window = 0) {
   Plan p{};
   const int group = n_q / c->n_kv;
   const bool d64 = c->head_dim == 64;
   const long long rows = (long long)b->n_tokens * group;
-  const long long kv = b->max_kv ? b->max_kv : (long long)b->table_width * c->block, steps = (kv + TILE - 1) / TILE;
+  long long kv = b->max_kv ? b->max_kv : (long long)b->table_width * c->block;
+  if (window && kv > (long long)window + TILE) kv = (long long)window + TILE;  // a window lies across one step more
+  const long long steps = (kv + TILE - 1) / TILE;
   // Which kernel takes a batch.  attn_rows reads a context once for every 16
   // rows but starts fast; attn_tile has two to three times the rate once its
   // 128-row tiles fill the chip, and before that waits for its longest tile, or
@@ -266,11 +268,14 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
 }
 
 static long long part_floats(const Plan& p, int k, int n_kv, int head_dim) { return p.slots[k] * n_kv * head_dim << p.lr[k]; }
+static long long part_rows(const Plan& p, int k, int n_kv) { return p.slots[k] * n_kv << p.lr[k]; }
 static long long part_bytes(const Plan& p, int k, int n_kv, int head_dim) {
-  return part_floats(p, k, n_kv, head_dim) * 4 + (p.slots[k] * n_kv << p.lr[k]) * 8;
+  return part_floats(p, k, n_kv, head_dim) * 4 + part_rows(p, k, n_kv) * 8;
 }
-static long long workspace(const Plan& p, int n_kv, int head_dim) {
-  return part_bytes(p, FEW, n_kv, head_dim) + part_bytes(p, MANY, n_kv, head_dim);
+// `scored`: with the sums of the weights before their rounding, behind the rest
+static long long workspace(const Plan& p, int n_kv, int head_dim, bool scored) {
+  return part_bytes(p, FEW, n_kv, head_dim) + part_bytes(p, MANY, n_kv, head_dim) +
+         (scored ? 4 * (part_rows(p, FEW, n_kv) + part_rows(p, MANY, n_kv)) : 0);
 }
 
 static bool heads_ok(const char* op, int n_q, int n_kv) {
@@ -294,6 +299,123 @@ static hipError_t launch_append(int pieces, bool f32, long long groups, hipStrea
   if constexpr (D == 128)
     if (pieces == 512) return f32 ? go(append<D, 256, 2, true>) : go(append<D, 256, 2, false>);
   return f32 ? go(append<D, 256, 1, true>) : go(append<D, 256, 1, false>);
+}
+
+static bool scores_ok(const char* op, const megakernel_kv8_scores* x) {
+  if (!x) {
+    set_err("%s: null scores", op);
+    return false;
+  }
+  if (!aligned(x->slopes, 4) || !aligned(x->first, 4) || !aligned(x->prefix, 4)) {
+    set_err("%s: slopes, first and prefix need 4-byte alignment", op);
+    return false;
+  }
+  if (!(x->softcap == 0.f || (x->softcap >= 0x1p-30f && x->softcap <= 0x1p30f)) || x->window < 0) {
+    set_err("%s: softcap=%g (0, or 2^-30 to 2^30), window=%d (0, or at least 1)", op, x->softcap, x->window);
+    return false;
+  }
+  return true;
+}
+
+// The softmax scale to base 2, or 0 where it cannot be.
+static float scale_of(const char* op, const megakernel_kv8_scores* x, float scale) {
+  const float scale2 = scale * 1.4426950408889634f;  // scores are taken to base 2
+  if (!(scale > 0.f && scale2 < INFINITY)) {
+    set_err("%s: scale=%g must be positive and finite, also times log2(e)", op, scale);
+    return 0.f;
+  }
+  if (x && x->softcap > 0.f && !(scale2 / x->softcap >= 0x1p-120f && scale2 / x->softcap <= 0x1p120f)) {
+    set_err("%s: scale=%g is too far from softcap=%g", op, scale, x->softcap);
+    return 0.f;
+  }
+  return scale2;
+}
+static Scores scores_of(const megakernel_kv8_scores* x, float scale2) {
+  Scores r{x->slopes, x->first, x->prefix, x->window, x->softcap > 64.f, 0.f, 0.f};
+  if (x->softcap > 0.f) {
+    r.cap = x->softcap * 1.4426950408889634f;
+    r.cap_in = 2.f * scale2 / x->softcap;
+  }
+  return r;
+}
+
+// P: Attn, or AttnScored with x and where wanted lse.
+template <class P>
+static int attend(const char* op, const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                  const megakernel_kv8_scores* x, const megakernel_rows* q, const megakernel_rows* out, float* lse, int n_q,
+                  float scale, void* d_workspace, long long workspace_bytes, hipStream_t st) {
+  constexpr bool SCORED = IsScored<P>::value;
+  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !heads_ok(op, n_q, cache->n_kv) ||
+      !rows_ok(op, "q", q, n_q, cache->head_dim, true) || !rows_ok(op, "out", out, n_q, cache->head_dim, true) ||
+      !apart(op, "out", out, n_q, cache->head_dim, batch->n_tokens) || (SCORED && !scores_ok(op, x)))
+    return -1;
+  if (!aligned(lse, 4)) {
+    set_err("%s: lse needs 4-byte alignment", op);
+    return -1;
+  }
+  if (q->p == out->p) {
+    set_err("%s: out must not be q", op);
+    return -1;
+  }
+  if ((long long)batch->n_tokens * (n_q / cache->n_kv) > (1ll << 30)) {
+    set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows", op, batch->n_tokens, n_q / cache->n_kv);
+    return -1;
+  }
+  const float scale2 = scale_of(op, x, scale);
+  if (!scale2) return -1;
+  const Plan pl = plan(cache, batch, n_q, SCORED ? x->window : 0);
+  const long long need = workspace(pl, cache->n_kv, cache->head_dim, SCORED);
+  if (need && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < need)) {
+    set_err("%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", op, need, d_workspace ? workspace_bytes : 0);
+    return -1;
+  }
+  if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
+  P p;
+  p.c = cache_of(cache);
+  p.b = batch_of(batch);
+  p.q = rows_of(q);
+  p.out = rows_of(out);
+  p.n_q = n_q;
+  p.group = n_q / cache->n_kv;
+  p.scale = scale2;
+  p.few = pl.few;
+  char* ws = static_cast<char*>(d_workspace);
+  for (int k = 0; k < 2; ++k) {
+    Deal& d = p.d[k];
+    d.lr = pl.lr[k], d.target = pl.target[k], d.least = pl.least[k], d.items = (int)pl.items[k];
+    d.part = reinterpret_cast<float*>(ws);
+    d.ml = reinterpret_cast<float2*>(d.part + part_floats(pl, k, cache->n_kv, cache->head_dim));
+    ws += part_bytes(pl, k, cache->n_kv, cache->head_dim);
+  }
+  if constexpr (SCORED) {
+    p.x = scores_of(x, scale2);
+    p.lse = lse;
+    p.ex[FEW] = reinterpret_cast<float*>(ws);
+    p.ex[MANY] = p.ex[FEW] + part_rows(pl, FEW, cache->n_kv);
+  }
+  const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv;
+  // tokens whose rows may have splits to join
+  long long tokens = batch->n_tokens;
+  if (!pl.target[MANY] && pl.use[MANY] && tokens > (long long)batch->n_seq * (pl.few / p.group)) tokens = (long long)batch->n_seq * (pl.few / p.group);
+  // a workgroup for every row, or where rows are many a wave for four (us in all,
+  // in a graph: one row of 32,768 positions 18.9 / 31.5, 1,056 rows of drafted
+  // tokens 38.8 / 40.8, a prompt's 16,384 335 / 311)
+  const bool each = tokens * n_q <= 4096;
+  const long long joins = !need ? 0 : each ? tokens * n_q : (tokens * ((n_q + 3) / 4) + 3) / 4;
+  if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
+  const bool d64 = cache->head_dim == 64;
+  auto go = [&](auto kern, long long groups, int threads) { return launch(kern, groups, threads, st, p); };
+  hipError_t e;
+  if (pl.use[FEW] && pl.use[MANY]) e = d64 ? go(attn_both<64, P>, many + few, 256) : go(attn_both<128, P>, many + few, 256);
+  else if (pl.use[MANY]) e = d64 ? go(attn_tile<64, P>, many, 256) : go(attn_tile<128, P>, many, 256);
+  else if (pl.waves == 2) e = d64 ? go(attn_rows<64, 2, P>, few, 128) : go(attn_rows<128, 2, P>, few, 128);
+  else if (pl.waves == 4) e = d64 ? go(attn_rows<64, 4, P>, few, 256) : go(attn_rows<128, 4, P>, few, 256);
+  else e = d64 ? go(attn_rows<64, 8, P>, few, 512) : go(attn_rows<128, 8, P>, few, 512);
+  if (e == hipSuccess && need) {
+    if (each) e = d64 ? go(attn_join<64, P>, joins, 256) : go(attn_join<128, P>, joins, 256);
+    else e = d64 ? go(attn_join_waves<64, 4, P>, joins, 256) : go(attn_join_waves<128, 4, P>, joins, 256);
+  }
+  return launched(op, e);
 }
 
 }  // namespace kv8
@@ -413,78 +535,29 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
 long long megakernel_op_kv8_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, int n_q) {
   const char* op = "op_kv8_workspace_bytes";
   if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !heads_ok(op, n_q, cache->n_kv)) return -1;
-  return workspace(plan(cache, batch, n_q), cache->n_kv, cache->head_dim);
+  return workspace(plan(cache, batch, n_q), cache->n_kv, cache->head_dim, false);
 }
 
 int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                                 const megakernel_rows* q, const megakernel_rows* out, int n_q, float scale,
                                 void* d_workspace, long long workspace_bytes, void* stream) {
-  const char* op = "op_kv8_attention";
-  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !heads_ok(op, n_q, cache->n_kv) ||
-      !rows_ok(op, "q", q, n_q, cache->head_dim, true) || !rows_ok(op, "out", out, n_q, cache->head_dim, true) ||
-      !apart(op, "out", out, n_q, cache->head_dim, batch->n_tokens))
-    return -1;
-  if (q->p == out->p) {
-    set_err("%s: out must not be q", op);
-    return -1;
-  }
-  if ((long long)batch->n_tokens * (n_q / cache->n_kv) > (1ll << 30)) {
-    set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows", op, batch->n_tokens, n_q / cache->n_kv);
-    return -1;
-  }
-  const float scale2 = scale * 1.4426950408889634f;  // scores are taken to base 2
-  if (!(scale > 0.f && scale2 < INFINITY)) {
-    set_err("%s: scale=%g must be positive and finite, also times log2(e)", op, scale);
-    return -1;
-  }
-  const Plan pl = plan(cache, batch, n_q);
-  const long long need = workspace(pl, cache->n_kv, cache->head_dim);
-  if (need && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < need)) {
-    set_err("%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", op, need, d_workspace ? workspace_bytes : 0);
-    return -1;
-  }
-  if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
-  Attn p;
-  p.c = cache_of(cache);
-  p.b = batch_of(batch);
-  p.q = rows_of(q);
-  p.out = rows_of(out);
-  p.n_q = n_q;
-  p.group = n_q / cache->n_kv;
-  p.scale = scale2;
-  p.few = pl.few;
-  char* ws = static_cast<char*>(d_workspace);
-  for (int k = 0; k < 2; ++k) {
-    Deal& d = p.d[k];
-    d.lr = pl.lr[k], d.target = pl.target[k], d.least = pl.least[k], d.items = (int)pl.items[k];
-    d.part = reinterpret_cast<float*>(ws);
-    d.ml = reinterpret_cast<float2*>(d.part + part_floats(pl, k, cache->n_kv, cache->head_dim));
-    ws += part_bytes(pl, k, cache->n_kv, cache->head_dim);
-  }
-  const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv;
-  // tokens whose rows may have splits to join
-  long long tokens = batch->n_tokens;
-  if (!pl.target[MANY] && pl.use[MANY] && tokens > (long long)batch->n_seq * (pl.few / p.group)) tokens = (long long)batch->n_seq * (pl.few / p.group);
-  // a workgroup for every row, or where rows are many a wave for four (us in all,
-  // in a graph: one row of 32,768 positions 18.9 / 31.5, 1,056 rows of drafted
-  // tokens 38.8 / 40.8, a prompt's 16,384 335 / 311)
-  const bool each = tokens * n_q <= 4096;
-  const long long joins = !need ? 0 : each ? tokens * n_q : (tokens * ((n_q + 3) / 4) + 3) / 4;
-  if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  const bool d64 = cache->head_dim == 64;
-  auto go = [&](auto kern, long long groups, int threads) { return launch(kern, groups, threads, st, p); };
-  hipError_t e;
-  if (pl.use[FEW] && pl.use[MANY]) e = d64 ? go(attn_both<64>, many + few, 256) : go(attn_both<128>, many + few, 256);
-  else if (pl.use[MANY]) e = d64 ? go(attn_tile<64>, many, 256) : go(attn_tile<128>, many, 256);
-  else if (pl.waves == 2) e = d64 ? go(attn_rows<64, 2>, few, 128) : go(attn_rows<128, 2>, few, 128);
-  else if (pl.waves == 4) e = d64 ? go(attn_rows<64, 4>, few, 256) : go(attn_rows<128, 4>, few, 256);
-  else e = d64 ? go(attn_rows<64, 8>, few, 512) : go(attn_rows<128, 8>, few, 512);
-  if (e == hipSuccess && need) {
-    if (each) e = d64 ? go(attn_join<64>, joins, 256) : go(attn_join<128>, joins, 256);
-    else e = d64 ? go(attn_join_waves<64, 4>, joins, 256) : go(attn_join_waves<128, 4>, joins, 256);
-  }
-  return launched(op, e);
+  return attend<Attn>("op_kv8_attention", cache, batch, nullptr, q, out, nullptr, n_q, scale, d_workspace, workspace_bytes,
+                      static_cast<hipStream_t>(stream));
+}
+
+long long megakernel_op_kv8_scored_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                                   const megakernel_kv8_scores* scores, int n_q) {
+  const char* op = "op_kv8_scored_workspace_bytes";
+  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !scores_ok(op, scores) || !heads_ok(op, n_q, cache->n_kv)) return -1;
+  return workspace(plan(cache, batch, n_q, scores->window), cache->n_kv, cache->head_dim, true);
+}
+
+int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                       const megakernel_kv8_scores* scores, const megakernel_rows* q,
+                                       const megakernel_rows* out, float* lse, int n_q, float scale, void* d_workspace,
+                                       long long workspace_bytes, void* stream) {
+  return attend<AttnScored>("op_kv8_attention_scored", cache, batch, scores, q, out, lse, n_q, scale, d_workspace,
+                            workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

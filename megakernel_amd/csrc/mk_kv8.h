@@ -68,6 +68,11 @@ __device__ __forceinline__ Seq seq_at(const Batch& b, int i, int lb) {
   return s;
 }
 
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+
 // Sum over the lanes up to and with this one (DPP: no step through LDS).
 __device__ __forceinline__ int wave_prefix(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
@@ -560,18 +565,46 @@ struct Attn {
   Deal d[2];
 };
 
+// What a score is beyond scale * q . k, and which positions a row sees beyond
+// the causal ones: s = cap * tanh(scale q.k / cap) - slope[head] |p - j| for
+// the row at position p and position j, seen if max(first[row], p + 1 -
+// window) <= j < max(p + 1, prefix[sequence]).
+struct Scores {
+  const float* slopes;  // [n_q], or null
+  const int* first;     // [n_tokens], or null
+  const int* prefix;    // [n_seq], or null
+  int window;           // 0: none
+  int wide;             // the cap is large: tanh of small arguments by its series (see capped())
+  float cap, cap_in;    // cap * log2(e) (0: none), 2 log2(e) scale / cap
+};
+// The attention with such scores, or with each row's log-sum-exp.
+struct AttnScored : Attn {
+  Scores x;
+  float* lse;    // [n_tokens][n_q], or null
+  float* ex[2];  // with splits, next to Deal::ml: sums of the weights as they were before their rounding
+};
+template <class P>
+struct IsScored {
+  static constexpr bool value = false;
+};
+template <>
+struct IsScored<AttnScored> {
+  static constexpr bool value = true;
+};
+
 constexpr int ROWS = 16;        // query rows of attn_rows's tile (the matrix columns)
 constexpr int TILE_ROWS = 128;  // and of attn_tile's
 constexpr int TILE = 64;        // positions of a step
 
-// Row tile rt of a sequence: its rows, and the positions [0, any) that some
-// row of it sees, [0, all) that every row sees.
+// Row tile rt of a sequence: its rows, and the positions [from, any) that some
+// row of it sees, [shut, all) that every row sees.
 struct RowTile {
-  int n_rows, any, all;
+  int n_rows, from, shut, any, all;
 };
 __device__ __forceinline__ RowTile row_tile(const Seq& s, int G, int rt, int rows) {
   const int r0 = rt * rows;  // rows times G are at most 2^30
   RowTile t;
+  t.from = t.shut = 0;
   t.n_rows = min(s.rows * G - r0, rows);
   t.all = min(max(s.pos0 + r0 / G + 1, 0), s.len);
   t.any = min(max(s.pos0 + (r0 + t.n_rows - 1) / G + 1, 0), s.len);
@@ -579,6 +612,85 @@ __device__ __forceinline__ RowTile row_tile(const Seq& s, int G, int rt, int row
 }
 __device__ __forceinline__ int row_tiles(const Seq& s, int G, int lr) {
   return (s.rows * G + (1 << lr) - 1) >> lr;
+}
+
+// Largest over the wave.
+__device__ __forceinline__ int wave_imax(int v) {
+  const auto sel = [](int x, auto ctrl) { return __builtin_amdgcn_update_dpp(0x80000000, x, decltype(ctrl)::value, 0xf, 0xf, false); };
+  v = max(v, sel(v, Int<DPP_XOR1>{}));
+  v = max(v, sel(v, Int<DPP_XOR2>{}));
+  v = max(v, sel(v, Int<DPP_HALF_MIRROR>{}));
+  v = max(v, sel(v, Int<DPP_MIRROR>{}));
+  auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  v = max((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane(max((int)r[0], (int)r[1]));
+}
+__device__ __forceinline__ int wave_imin(int v) { return ~wave_imax(~v); }
+
+// Positions [lo, hi) that a row sees; of none both are 0.
+struct Sight {
+  int lo, hi;
+};
+__device__ __forceinline__ Sight sight(const Batch& b, const Scores& x, const Seq& s, int tok) {
+  const int p = s.pos0 + tok;
+  int lo = 0, hi = p + 1;
+  if (x.window) lo = (int)max((long long)p + 1 - x.window, 0ll);
+  if (x.first) lo = max(lo, x.first[s.row0 + tok]);
+  if (x.prefix && p >= 0) hi = max(hi, x.prefix[s.i]);
+  hi = min(max(hi, 0), s.len);
+  return lo < hi ? Sight{lo, hi} : Sight{0, 0};
+}
+// The bounds of a row tile from its rows' (each in some lane of the wave).
+struct Bounds {
+  int from = 0x7fffffff, shut = 0, any = 0, all = 0x7fffffff;
+  __device__ __forceinline__ void add(const Sight& v) {
+    if (v.hi) from = min(from, v.lo);
+    shut = max(shut, v.lo);
+    any = max(any, v.hi);
+    all = min(all, v.hi);
+  }
+  __device__ __forceinline__ void join() {
+    any = wave_imax(any);
+    from = min(wave_imin(from), any);
+    shut = wave_imax(shut);
+    all = wave_imin(all);
+  }
+};
+
+// Scores to base 2 from q . k, where they are capped: cap * tanh(y) with
+// tanh(y) = 1 - 2 / (e^2y + 1), which is off by 2^-23 of the cap where y is
+// small.  For caps of up to 64 that is what rounding scores of tens costs
+// anyway; for larger ones tanh is its series where |y| is below 1/4 (the first
+// term left out is 2^-26.8 of the value).
+__device__ __forceinline__ float capped(const Scores& x, float s) {
+  const float t = __builtin_amdgcn_exp2f(s * x.cap_in);
+  return fmaf(-2.f * x.cap, __builtin_amdgcn_rcpf(t + 1.f), x.cap);
+}
+__device__ __forceinline__ float capped_wide(const Scores& x, float s, float scale) {
+  const float y = s * x.cap_in * 0.34657359027997264f;  // ln(2) / 2
+  const float z = y * y;
+  const float r = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
+  return fabsf(y) < 0.25f ? s * scale * r : capped(x, s);
+}
+// Scores of one row to base 2, in place: N of them, at(i) is the position of
+// the i-th less that of the row.
+template <int N, class At>
+__device__ __forceinline__ void score(const Scores& x, float scale, float slope, float* s, At at) {
+  if (!x.cap) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] *= scale;
+  } else if (!x.wide) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = capped(x, s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = capped_wide(x, s[i], scale);
+  }
+  if (x.slopes) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = fmaf(-slope, fabsf((float)at(i)), s[i]);
+  }
 }
 
 // Most splits of one row tile (attn_join gives each a thread).
@@ -597,7 +709,20 @@ struct Item {
 };
 
 // Steps of a sequence's longest row tile.
-__device__ __forceinline__ int most_steps(const Seq& s) { return (min(max(s.pos0 + s.rows, 0), s.len) + TILE - 1) / TILE; }
+__device__ __forceinline__ int most_steps(const Attn&, const Deal&, const Seq& s) {
+  return (min(max(s.pos0 + s.rows, 0), s.len) + TILE - 1) / TILE;
+}
+// With a window those that it lets a row tile see, and one more where it lies
+// across steps; documents are not known here.
+__device__ __forceinline__ int most_steps(const AttnScored& p, const Deal& d, const Seq& s) {
+  if (s.rows <= 0) return 0;
+  int hi = max(s.pos0 + s.rows, 0);
+  const int prefix = p.x.prefix ? p.x.prefix[s.i] : 0;
+  hi = min(max(hi, prefix), s.len);
+  int n = (hi + TILE - 1) / TILE;
+  if (p.x.window && prefix <= max(s.pos0, 0)) n = (int)min((long long)n, ((long long)p.x.window + (1 << d.lr) / p.group + 2 * TILE) / TILE);
+  return n;
+}
 
 __device__ __forceinline__ int kind_of(const Attn& p, const Seq& s) { return (long long)s.rows * p.group > p.few; }
 
@@ -609,13 +734,14 @@ __device__ __forceinline__ Seq lane_seq(const Attn& p, int base) {
 
 // Steps of an item: the target-th part of all steps of the kernel's row tiles.
 // `first` holds the first 64 sequences.
-__device__ __forceinline__ int steps_per_item(const Attn& p, int kind, const Seq& first) {
+template <class P>
+__device__ __forceinline__ int steps_per_item(const P& p, int kind, const Seq& first) {
   const Deal& d = p.d[kind];
   if (!d.target) return 0x7fffffff;
   long long total = 0;
   for (int base = 0; base < p.b.n_seq; base += kWave) {
     const Seq q = base ? lane_seq(p, base) : first;
-    const long long w = kind_of(p, q) == kind ? (long long)row_tiles(q, p.group, d.lr) * most_steps(q) : 0;
+    const long long w = kind_of(p, q) == kind ? (long long)row_tiles(q, p.group, d.lr) * most_steps(p, d, q) : 0;
     // 64 lanes' sum in two halves that stay inside 32 bits
     const int lo = wave_prefix((int)(w & 0xffffff)), hi = wave_prefix((int)min(w >> 24, 0x1ffffffll));
     total += ((long long)__builtin_amdgcn_readlane(hi, 63) << 24) + __builtin_amdgcn_readlane(lo, 63);
@@ -635,8 +761,8 @@ __device__ __forceinline__ int steps_per_item(const Attn& p, int kind, const Seq
 // Finds item `it` of a kernel, or with kind -1 the item that holds token `it`
 // of all tokens of kernels that split (r.rt is then the token's number within
 // its sequence).
-template <int KIND>
-__device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
+template <int KIND, class P>
+__device__ __forceinline__ bool find_split(const P& p, int it, Item& r) {
   const int G = p.group;
   const Seq first = lane_seq(p, 0);
   const int per0 = KIND != MANY ? steps_per_item(p, FEW, first) : 0, per1 = KIND != FEW ? steps_per_item(p, MANY, first) : 0;
@@ -647,7 +773,7 @@ __device__ __forceinline__ bool find_split(const Attn& p, int it, Item& r) {
     int c = 0, s0 = 0, s1 = 0, ns = 1;
     if (KIND < 0 ? (kind ? p.d[1].target : p.d[0].target) != 0 : kind == KIND) {
       const int per = kind ? per1 : per0;
-      const int rt = row_tiles(q, G, kind ? p.d[1].lr : p.d[0].lr), n = most_steps(q);
+      const int rt = row_tiles(q, G, kind ? p.d[1].lr : p.d[0].lr), n = most_steps(p, kind ? p.d[1] : p.d[0], q);
       if (p.d[0].target | p.d[1].target) ns = min(max(n / per + (n % per != 0), 1), kMaxSplits);
       const int sl = ns > 1 ? rt * ns : 0;
       s0 = kind ? 0 : sl;
@@ -719,6 +845,12 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi, float s) 
   return __builtin_bit_cast(bf16x8, fp8x8_to_bf16x8_scaled(u32x2{lo, hi}, s));
 }
 
+// ln sum_j e^(s_j) of a row from its scores' reference m (to base 2) and the
+// sum of 2^(s - m); -inf of a row that sees nothing.
+__device__ __forceinline__ void put_lse(const AttnScored& p, long long row, int h, float m, float sum) {
+  p.lse[row * p.n_q + h] = (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+}
+
 // Block ids of the positions whose K, and whose V, a lane loads in a step.
 struct Ids {
   int k, v;
@@ -747,16 +879,19 @@ struct Ids {
 // tokens each of 16 sequences of 700 to 8,191 37 us (148 MB, 32 and 5); 64
 // sequences of 4,096, head_dim 64, 52 us (268 MB, 5.1 TB/s).  Streaming as many
 // bytes without any work takes 7, 12, 27 and 48 us here.
-template <int D, int W>
+template <int D, int W, bool SCORED>
 struct RowsLds {
   float lo[W][ROWS][D + 4];
   float lm[W][ROWS], ls[W][ROWS];
+  float le[SCORED ? W : 1][ROWS];
 };
 
-template <int D, int W>
-__device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
+template <int D, int W, class P>
+__device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
   constexpr int KH = D / 64, DT = D / 16;  // 64-dimension halves of K, 16-dimension tiles of V
-  RowsLds<D, W>& lds = *static_cast<RowsLds<D, W>*>(smem);
+  constexpr bool SCORED = IsScored<P>::value;
+  typedef RowsLds<D, W, SCORED> Lds;
+  Lds& lds = *static_cast<Lds*>(smem);
   auto &lm = lds.lm, &ls = lds.ls;
   auto& lo = lds.lo;
   const int lb = p.c.lb, G = p.group, off = (1 << lb) - 1;
@@ -766,12 +901,23 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   const Seq& s = it.s;
   const int l = (int)(threadIdx.x & 63u), wv = wave_id();
   const int c = l & 15, g = l >> 4;  // this lane's query row; its 16 positions of a step
-  const RowTile rows = row_tile(s, G, it.rt, ROWS);
-  const int r0 = it.rt * ROWS, tiles = (rows.any + TILE - 1) / TILE;
-  const int t0 = it.step(it.split, tiles), t1 = it.step(it.split + 1, tiles);
+  RowTile rows = row_tile(s, G, it.rt, ROWS);
+  const int r0 = it.rt * ROWS;
   const bool mine = c < rows.n_rows;
   const int rr = mine ? r0 + c : r0, tok = rr / G, hd = head * G + rr % G;
-  const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
+  int shut = 0, see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [shut, see)
+  float slope = 0.f;
+  if constexpr (SCORED) {
+    const Sight v = sight(p.b, p.x, s, tok);
+    Bounds b;
+    if (mine) b.add(v);
+    b.join();
+    rows = RowTile{rows.n_rows, b.from, b.shut, b.any, b.all};
+    shut = v.lo, see = mine ? v.hi : 0;
+    if (p.x.slopes) slope = p.x.slopes[hd] * 1.4426950408889634f;
+  }
+  const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
+  const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);
 
   // Table entries of a step, loaded a step before the codes they lead to and
   // checked only there: the loads are waited for in the order of their issue,
@@ -831,7 +977,8 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   // the weights' reference of row c (or -inf), it negated (or 0), and what the
   // lane's scores may reach before it is raised
-  float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f;
+  float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f, ex = 0.f;  // ex: of the weights as they are, for the log-sum-exp
+  const float scale = SCORED ? 1.f : p.scale;  // of what score() left
 
   // Both are waited for here: left to itself, the second would be asked for
   // behind the first codes, and the loop's waits be for everything.
@@ -860,13 +1007,23 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
       load_k(t + W, next.k);
     }
     // scores of positions pv + 4i + j of row c
-    if ((t + 1) * TILE > rows.all || __any(gone)) {
+    if constexpr (SCORED) {
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = sc[i / 4][i % 4];
+      const int rel = pv - (s.pos0 + tok);
+      score<16>(p.x, p.scale, slope, x, [&](int i) { return rel + i; });
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i / 4][i % 4] = x[i];
+    }
+    if ((t + 1) * TILE > rows.all || (SCORED && t * TILE < rows.shut) || __any(gone)) {
       // opaque: a branch for the few steps that need it, not its selects in every step
-      const int lim = opaque_v(gone ? 0 : see - pv);
+      const int lim = opaque_v(gone ? 0 : see - pv), lol = SCORED ? opaque_v(shut - pv) : 0;
+      const auto in = [&](int i) { return i < lim && (!SCORED || i >= lol); };
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[i][j] = 4 * i + j < lim ? sc[i][j] : -INFINITY;
+        for (int j = 0; j < 4; ++j) sc[i][j] = in(4 * i + j) ? sc[i][j] : -INFINITY;
       // A NaN in V must not reach the rows that do not see it (0 * NaN): it
       // is taken out here, and put into the rows that do see it.
       uint32_t bad = 0;
@@ -879,7 +1036,7 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) seen[e][i] = (__bf16)(8 * e + i < lim ? 1.f : 0.f);
+          for (int i = 0; i < 8; ++i) seen[e][i] = (__bf16)(in(8 * e + i) ? 1.f : 0.f);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           f32x4 hit = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -902,13 +1059,14 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) mt = fmaxf(mt, sc[i][j]);
-    mt *= p.scale;
+    mt *= scale;
     if (__any(mt > up)) {  // joined over the row's four lanes only here
       const float mn = fmaxf(m, max_xor32(max_xor16(mt))), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
+      if constexpr (SCORED) ex *= al;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= al;
     }
@@ -917,8 +1075,14 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        pr[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], p.scale, below));
+        pr[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], scale, below));
       }
+    if constexpr (SCORED) {
+      if (p.lse) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ex += pr[i];
+      }
+    }
     const bf16x2 one = bf16x2{(__bf16)1.f, (__bf16)1.f};
     bf16x8 pb[2];
 #pragma unroll
@@ -946,10 +1110,14 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
   }
 
   sum = sum_xor32(sum_xor16(sum));
+  if constexpr (SCORED) ex = sum_xor32(sum_xor16(ex));
 
   // join the waves: o[d][i] is dimension 16d + 4g + i of row c
   if (mine) {
     if (g == 0) lm[wv][c] = m, ls[wv][c] = sum;
+    if constexpr (SCORED) {
+      if (g == 0) lds.le[wv][c] = ex;
+    }
 #pragma unroll
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&lo[wv][c][16 * d + 4 * g]) = o[d];
   }
@@ -961,14 +1129,21 @@ __device__ __forceinline__ void rows_item(const Attn& p, int item, void* smem) {
     for (int w = 1; w < W; ++w) mm = fmaxf(mm, lm[w][row]);
     const float mref = mm == -INFINITY ? 0.f : mm;
     f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    float tot = 0.f;
+    float tot = 0.f, te = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float f = __builtin_amdgcn_exp2f(lm[w][row] - mref);
       tot += f * ls[w][row];
+      if constexpr (SCORED) te += f * lds.le[w][row];
       v += f * *reinterpret_cast<const f32x4*>(&lo[w][row][d]);
     }
     const int tk = (r0 + row) / G, oh = head * G + (r0 + row) % G;
+    if constexpr (SCORED) {
+      if (p.lse && d == 0) {
+        if (it.ns == 1) put_lse(p, s.row0 + tk, oh, mm, te);
+        else p.ex[FEW][((long long)(it.slot + it.split) * p.c.n_kv + head) * ROWS + row] = te;
+      }
+    }
     if (it.ns == 1) {
       v *= tot > 0.f || tot != tot ? 1.f / tot : 0.f;
       uint16_t* op = static_cast<uint16_t*>(p.out.p) + (s.row0 + tk) * p.out.ts + oh * p.out.hs + d;
@@ -1013,8 +1188,9 @@ struct TileLds {
   int bad[2];                     // 1 + the step in the buffer, if nans has any
 };
 
-template <int D>
-__device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
+template <int D, class P>
+__device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
+  constexpr bool SCORED = IsScored<P>::value;
   constexpr int KC = D / 16, DB = D / 32;    // 16-dimension pieces of a K row, 32-dimension blocks of V
   constexpr int NL = D * TILE / (256 * 16);  // 16-byte loads per thread of K, and of V
   typedef TileLds<D> Lds;
@@ -1031,15 +1207,30 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   const Seq& s = it.s;
   const int l = (int)(threadIdx.x & 63u), wv = wave_id(), tid = (int)threadIdx.x;
   const int c = l & 31, h = l >> 5;
-  const RowTile rows = row_tile(s, G, it.rt, TILE_ROWS);
-  const int r0 = it.rt * TILE_ROWS, tiles = (rows.any + TILE - 1) / TILE;
-  const int t0 = it.step(it.split, tiles), t1 = it.step(it.split + 1, tiles);
-  const int n = t1 - t0, end = min(s.len, t1 * TILE);
+  RowTile rows = row_tile(s, G, it.rt, TILE_ROWS);
+  const int r0 = it.rt * TILE_ROWS;
   const bool mine = 32 * wv + c < rows.n_rows;
   const int rr = mine ? r0 + 32 * wv + c : r0, tok = rr / G, hd = head * G + rr % G;
-  const int see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [0, see)
-  // every row of the wave sees [0, all)
-  const int all = min(max(s.pos0 + (r0 + min(32 * wv, rows.n_rows - 1)) / G + 1, 0), s.len);
+  int shut = 0, see = mine ? min(max(s.pos0 + tok + 1, 0), s.len) : 0;  // this row sees [shut, see)
+  // every row of the wave sees [none, all)
+  int none = 0, all = min(max(s.pos0 + (r0 + min(32 * wv, rows.n_rows - 1)) / G + 1, 0), s.len);
+  float slope = 0.f;
+  if constexpr (SCORED) {
+    const Sight v = sight(p.b, p.x, s, tok);
+    Bounds mb, b;  // of the wave's rows, of the tile's
+    if (mine) mb.add(v);
+    mb.join();
+    none = mb.shut, all = mb.all;
+    for (int i = l; i < rows.n_rows; i += kWave) b.add(sight(p.b, p.x, s, (r0 + i) / G));
+    b.join();
+    rows = RowTile{rows.n_rows, b.from, b.shut, b.any, b.all};
+    shut = v.lo, see = mine ? v.hi : 0;
+    if (p.x.slopes) slope = p.x.slopes[hd] * 1.4426950408889634f;
+  }
+  const float scale = SCORED ? 1.f : p.scale;  // of what score() left
+  const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
+  const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);
+  const int n = t1 - t0, end = min(s.len, t1 * TILE);
 
   bf16x8 qv[KC];
   {
@@ -1110,7 +1301,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   };
   const auto stage_v = [&](int k) {
     const int first = first_of(k);
-    if (first + TILE > rows.all || gone_of(k)) {
+    if (first + TILE > rows.all || (SCORED && first < rows.shut) || gone_of(k)) {
       const int left = gone_of(k) >> wv & 1 ? 0 : opaque_v(end - first - 16 * wv);  // of the run's 16 positions
       // What no row may see is zero.  Where rows differ in what they see, a
       // NaN must not reach those that do not see it (0 * NaN): it is taken
@@ -1146,7 +1337,7 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-  float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f;  // as in rows_item()
+  float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f, ex = 0.f;  // as in rows_item()
   // Both halves in turn: a product that adds to the one before it waits twice
   // as long as the unit takes.
   const auto scores = [&](int k) {
@@ -1208,36 +1399,54 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
       else tab1 = x;
     }
     // score i of half a: position 32a + 16(i/8) + 8h + i%8 of the step
-    if (first + TILE > all || gone) {
+    const auto place = [](int a, int i) { return 32 * a + 16 * (i / 8) + i % 8; };
+    if constexpr (SCORED) {
+      const int rel = first + 8 * h - (s.pos0 + tok);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = sc[a][i];
+        score<16>(p.x, p.scale, slope, x, [&](int i) { return rel + place(a, i); });
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[a][i] = x[i];
+      }
+    }
+    if (first + TILE > all || (SCORED && first < none) || gone) {
       // opaque: a branch for the few steps that need it, not its 64 selects in every step
-      const int lim = opaque_v(see - first - 8 * h);
+      const int lim = opaque_v(see - first - 8 * h), lol = SCORED ? opaque_v(shut - first - 8 * h) : 0;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          sc[a][i] = 32 * a + 16 * (i / 8) + i % 8 < lim && !(gone >> (2 * a + i / 8) & 1) ? sc[a][i] : -INFINITY;
+          sc[a][i] = place(a, i) < lim && (!SCORED || place(a, i) >= lol) && !(gone >> (2 * a + i / 8) & 1) ? sc[a][i] : -INFINITY;
     }
     float mt = sc[0][0];
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[a][i]);
-    mt *= p.scale;
+    mt *= scale;
     if (__any(mt > up)) {
       const float mn = fmaxf(m, max_xor32(mt)), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
+      if constexpr (SCORED) ex *= al;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= al;
     }
-    if (__builtin_expect((first + TILE > rows.all || gone) && lds.bad[buf] == k + 1, 0)) {
+    if (__builtin_expect((first + TILE > rows.all || (SCORED && first < rows.shut) || gone) && lds.bad[buf] == k + 1, 0)) {
       // the NaN that stage_v() took out, put into the rows that see them
       const int x = min(max(see - first, 0), TILE);
       unsigned long long seen = x < 64 ? (1ull << x) - 1ull : ~0ull;
+      if constexpr (SCORED) {
+        const int y = min(max(shut - first, 0), TILE);
+        seen &= y < 64 ? ~0ull << y : 0ull;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) seen &= gone >> i & 1 ? ~(0xffffull << (16 * i)) : ~0ull;
 #pragma unroll
@@ -1251,8 +1460,9 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
     const auto weights = [&](int a) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], p.scale, below));
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], p.scale, below));
+        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], scale, below));
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], scale, below));
+        if constexpr (SCORED) ex += x + y;
         const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
         sum = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum, false);  // of the rounded weights
         pb[a][i / 8][i % 8] = w[0];
@@ -1276,6 +1486,13 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
     __syncthreads();
   }
   sum = sum_xor32(sum);
+  if constexpr (SCORED) {
+    ex = sum_xor32(ex);
+    if (p.lse && mine && h == 0) {
+      if (it.ns == 1) put_lse(p, s.row0 + tok, hd, m, ex);
+      else p.ex[MANY][((long long)(it.slot + it.split) * p.c.n_kv + head) * TILE_ROWS + 32 * wv + c] = ex;
+    }
+  }
   if (!mine) return;
   // o[d][4b + j] is dimension 32d + 8b + 4h + j of row c
   if (it.ns == 1) {
@@ -1302,23 +1519,23 @@ __device__ __forceinline__ void tile_item(const Attn& p, int item, void* smem) {
   }
 }
 
-template <int D, int W>
-__global__ __launch_bounds__(W* kWave, D == 64 ? 3 : 2) void attn_rows(Attn p) {
-  __shared__ __align__(16) RowsLds<D, W> lds;
+template <int D, int W, class P>
+__global__ __launch_bounds__(W* kWave, D == 64 ? 3 : 2) void attn_rows(P p) {
+  __shared__ __align__(16) RowsLds<D, W, IsScored<P>::value> lds;
   rows_item<D, W>(p, (int)blockIdx.x, &lds);
 }
-template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_tile(Attn p) {
+template <int D, class P>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_tile(P p) {
   __shared__ __align__(16) TileLds<D> lds;
   tile_item<D>(p, (int)blockIdx.x, &lds);
 }
 // Batches with sequences of both kinds: one launch, so that neither waits for
 // the other's last workgroup; the tiles first, they take longest.
-template <int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_both(Attn p) {
+template <int D, class P>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_both(P p) {
   __shared__ __align__(16) union {
     TileLds<D> t;
-    RowsLds<D, 4> r;
+    RowsLds<D, 4, IsScored<P>::value> r;
   } lds;
   const int many = p.d[MANY].items * p.c.n_kv;
   if ((int)blockIdx.x < many) tile_item<D>(p, (int)blockIdx.x, &lds);
@@ -1342,6 +1559,9 @@ __device__ __forceinline__ Parts parts_of(const Attn& p, const Item& it, int oh)
   x.ml = d.ml + at;
   return x;
 }
+__device__ __forceinline__ const float* ex_of(const AttnScored& p, const Item& it, const Parts& x) {
+  return p.ex[it.kind] + (x.ml - p.d[it.kind].ml);
+}
 __device__ __forceinline__ void put_row4(const Rows& out, long long e, f32x4 a, float tot) {
   a *= tot > 0.f || tot != tot ? 1.f / tot : 0.f;
   u32x2 w;
@@ -1353,8 +1573,8 @@ __device__ __forceinline__ void put_row4(const Rows& out, long long e, f32x4 a, 
 // Joins the splits of the rows that have more than one; D/4 lanes read a
 // partial, the order of the sums is fixed.  Many rows: a wave takes HEADS
 // rows of one token after the other.
-template <int D, int HEADS>
-__global__ __launch_bounds__(256) void attn_join_waves(Attn p) {
+template <int D, int HEADS, class P>
+__global__ __launch_bounds__(256) void attn_join_waves(P p) {
   constexpr int LPP = D / 4, NG = kWave / LPP, PER = 8;  // lanes per partial, partials at once, loads in flight
   const int l = (int)(threadIdx.x & 63u), per_token = (p.n_q + HEADS - 1) / HEADS;
   const int w = (int)blockIdx.x * 4 + wave_id();
@@ -1393,14 +1613,22 @@ __global__ __launch_bounds__(256) void attn_join_waves(Attn p) {
     if (NG == 4) tot = sum_xor16(tot);
     tot = sum_xor32(tot);
     if (grp == 0) put_row4(p.out, (it.s.row0 + it.rt) * p.out.ts + oh * p.out.hs + 4 * ln, a, tot);
+    if constexpr (IsScored<P>::value) {
+      if (p.lse) {
+        float te = 0.f;
+        for (int z = l; z < ns; z += kWave) te += __builtin_amdgcn_exp2f(x.ml[z * x.stride].x - mref) * ex_of(p, it, x)[z * x.stride];
+        te = wave_sum(te);
+        if (l == 0) put_lse(p, it.s.row0 + it.rt, oh, mm, te);
+      }
+    }
   }
 }
 
 // Few rows: a workgroup for each, 64 partials in flight together (one sequence
 // of 32,768, head_dim 128, in a graph 18.9 us; with 32 19.8).  5 us, of which a launch
 // is 2.7 and the rest the lengths, the partials and the sums in turn.
-template <int D>
-__global__ __launch_bounds__(256) void attn_join(Attn p) {
+template <int D, class P>
+__global__ __launch_bounds__(256) void attn_join(P p) {
   constexpr int LPP = D / 4, NG = 256 / LPP, PER = 64 / NG;  // lanes per partial, groups, partials in flight per group
   __shared__ float lw[kMaxSplits], red1[4];
   __shared__ f32x4 red[NG][LPP];
@@ -1422,6 +1650,12 @@ __global__ __launch_bounds__(256) void attn_join(Attn p) {
   const float w = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(q.x - mm);
   lw[tz] = w;
   const float tot = block_sum<4>(w * q.y, red1);
+  if constexpr (IsScored<P>::value) {
+    if (p.lse) {
+      const float te = block_sum<4>(tz < ns ? w * ex_of(p, it, x)[tz * x.stride] : 0.f, red1);
+      if (tz == 0) put_lse(p, it.s.row0 + it.rt, oh, mm, te);
+    }
+  }
   f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < PER; ++i) a += lw[grp + i * NG] * v[i];

@@ -52,6 +52,11 @@ class _CCache(ctypes.Structure):
                 ("n_kv", ctypes.c_int), ("head_dim", ctypes.c_int)]
 
 
+class _CScores(ctypes.Structure):
+    _fields_ = [("slopes", ctypes.c_void_p), ("first", ctypes.c_void_p), ("prefix", ctypes.c_void_p),
+                ("softcap", ctypes.c_float), ("window", ctypes.c_int)]
+
+
 class _CBatch(ctypes.Structure):
     _fields_ = [("table", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
                 ("n_seq", ctypes.c_int), ("table_width", ctypes.c_int), ("n_tokens", ctypes.c_int),
@@ -194,6 +199,57 @@ class Batch(_Fixed):
         self._need: dict[tuple, int] = {}
 
 
+class Scores(_Fixed):
+    """What the scores of :func:`attention` and :func:`weigh` are, and what a
+    row sees.  The row at position p and a position j have the score
+
+        softcap * tanh(scale * q.k / softcap) - slopes[head] * |p - j|
+
+    without the tanh where ``softcap`` is 0, and without the bias where there
+    are no ``slopes`` (float32 [n_q], finite).  The row sees
+    max(0, first[row], p + 1 - window) <= j < max(p + 1, prefix[sequence]):
+    ``window`` positions up to its own (0: all), none before its document
+    (``first``, int32 [n_tokens]), and of a prefix all (``prefix``, int32
+    [n_seq]: how many positions it has).  The tensors are read when a call runs,
+    so they may change between calls and replays.
+    """
+
+    def __init__(self, softcap: float = 0.0, slopes=None, window: int = 0, first=None, prefix=None):
+        given = [t for t in (slopes, first, prefix) if t is not None]
+        device = given[0].get_device() if given else None
+        for t, name, dtype in ((slopes, "slopes", torch.float32), (first, "first", torch.int32), (prefix, "prefix", torch.int32)):
+            if t is not None:
+                _whole(t, dtype, (None,), device, name)
+        if not (softcap == 0 or 2.0 ** -30 <= softcap <= 2.0 ** 30) or not 0 <= window < 1 << 31:
+            raise ValueError(f"softcap {softcap} (0, or 2^-30 to 2^30), window {window} (0 to 2^31 - 1)")
+        self.slopes, self.first, self.prefix = slopes, first, prefix
+        self.softcap, self.window, self.device = float(softcap), int(window), device
+        # an empty tensor has no address, and no row asks for what is in it
+        self._c = _CScores(*(None if t is None else t.data_ptr() or 16 for t in (slopes, first, prefix)), self.softcap,
+                           self.window)
+        self._ref = ctypes.byref(self._c)
+
+    def _fits(self, batch: "Batch", n_q: int):
+        for t, name, n in ((self.slopes, "slopes", n_q), (self.first, "first", batch.n_tokens), (self.prefix, "prefix", batch.n_seq)):
+            if t is not None and t.shape[0] != n:
+                raise ValueError(f"{name} of the scores has shape {tuple(t.shape)}, not {(n,)}")
+        if self.device is not None and self.device != batch.device:
+            raise ValueError(f"the scores are on cuda:{self.device}, not on cuda:{batch.device}")
+
+
+_plain = None  # Scores() of a call that has none
+
+
+def _scores(scores: "Scores | None", batch: "Batch", n_q: int) -> Scores:
+    global _plain
+    if scores is None:
+        if _plain is None:
+            _plain = Scores()
+        return _plain
+    scores._fits(batch, n_q)
+    return scores
+
+
 def qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q_out, k_out, eps: float = 1e-6):
     """RMSNorm of every head of q [T][n_q][D] and k [T][n_kv][D] with its gain
     (bf16 [D]), then the rotate-half rotation by ``pos[t] * inv_freq[i]``
@@ -250,22 +306,32 @@ def read(cache: Cache, batch: Batch, k_out, v_out):
         _call("megakernel_op_kv8_read", cache.device, cache._ref, batch._ref, a, b)
 
 
-def workspace_bytes(cache: Cache, batch: Batch, n_q: int) -> int:
-    """Bytes of :func:`attention`'s workspace for these sizes (0: none)."""
-    key = (cache.n_kv, cache.head_dim, cache.block, n_q)
+def workspace_bytes(cache: Cache, batch: Batch, n_q: int, scores: Scores | None = None, lse: bool = False) -> int:
+    """Bytes of :func:`attention`'s workspace for these sizes (0: none), with
+    scores and a log-sum-exp as the call will have them."""
+    scored = scores is not None or lse
+    key = (cache.n_kv, cache.head_dim, cache.block, n_q, (scores.window if scores else 0) if scored else None)
     need = batch._need.get(key)
     if need is None:
         lib = _lib.load()
-        need = _lib.check(lib, lib.megakernel_op_kv8_workspace_bytes(cache._ref, batch._ref, n_q), "op_kv8_workspace_bytes")
-        batch._need[key] = need
+        if scored:
+            x = _scores(scores, batch, n_q)
+            need = lib.megakernel_op_kv8_scored_workspace_bytes(cache._ref, batch._ref, x._ref, n_q)
+        else:
+            need = lib.megakernel_op_kv8_workspace_bytes(cache._ref, batch._ref, n_q)
+        batch._need[key] = _lib.check(lib, need, "op_kv8_workspace_bytes")
     return need
 
 
-def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, workspace=None):
+def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, workspace=None, scores: Scores | None = None,
+              lse=None):
     """Causal attention of q [n_tokens][n_q][head_dim] (bf16) over the cache
     into out: each row sees its sequence's positions up to its own, its own
     among them.  Query head h reads KV head h / (n_q / n_kv); rows that see
     nothing are zeros.  ``scale`` is 1 / sqrt(head_dim) unless given.
+    ``scores`` changes what scores are and what rows see (:class:`Scores`).
+    ``lse`` (float32 [n_tokens][n_q]) receives the rows' log-sum-exps,
+    -infinity for a row that sees nothing.
     ``workspace`` is a uint8 tensor of :func:`workspace_bytes`, one for each
     call that may run at the same time; without one, a call takes its own from
     torch's allocator."""
@@ -275,7 +341,12 @@ def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, wo
     device, n_q = cache.device, q.shape[1]
     shape = (batch.n_tokens, n_q, cache.head_dim)
     a, b = _rows(q, shape, device, "q", _BF16), _rows(out, shape, device, "out", _BF16)
-    need = workspace_bytes(cache, batch, n_q)
+    x = None
+    if scores is not None or lse is not None:
+        x = _scores(scores, batch, n_q)
+        if lse is not None:
+            _whole(lse, torch.float32, (batch.n_tokens, n_q), device, "lse")
+    need = workspace_bytes(cache, batch, n_q, scores, lse is not None)
     if not batch.n_seq or not batch.n_tokens:
         return
     at = size = None
@@ -285,5 +356,10 @@ def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, wo
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     if workspace is not None:
         at, size = workspace.data_ptr(), workspace.numel()
-    _call("megakernel_op_kv8_attention", device, cache._ref, batch._ref, a, b, n_q,
-          cache.head_dim ** -0.5 if scale is None else scale, at, size or 0)
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    if x is None:
+        _call("megakernel_op_kv8_attention", device, cache._ref, batch._ref, a, b, n_q, scale, at, size or 0)
+    else:
+        _call("megakernel_op_kv8_attention_scored", device, cache._ref, batch._ref, x._ref, a, b,
+              None if lse is None else lse.data_ptr(), n_q, scale, at, size or 0)
