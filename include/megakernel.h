@@ -547,6 +547,55 @@ int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const 
                                        const megakernel_rows* out, float* lse, int n_q, float scale, void* workspace,
                                        long long workspace_bytes, void* stream);
 
+/* What each cached position is worth: mass [n_seq][n_kv][positions] (fp32 rows;
+ * token_stride from one sequence to the next, positions at least table_width *
+ * block).  For sequence i, KV head h and position j
+ *   mass[i][h][j] = (j before the batch's rows ? mass[i][h][j] : 0)
+ *                   + sum over its rows r and the query heads of h of e^(s_rj - lse_r)
+ * with the scores and the lse of megakernel_op_kv8_attention_scored() of the same
+ * batch.  Positions of the batch's own rows start anew, so blocks need no initial
+ * weights; positions past kv_len and sequences without rows are left alone.
+ * Sums are fp32, in an order that depends on sizes alone. */
+int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                            const megakernel_kv8_scores* scores, const megakernel_rows* q, const float* lse,
+                            const megakernel_rows* mass, int n_q, float scale, void* stream);
+
+/* The positions that stay of each sequence and KV head: kept [n_seq][n_kv][keep]
+ * receives them in rising order, -1 behind the last; kept_len [n_seq] how many
+ * there are, min(kv_len, keep).  Of a longer sequence these are its first `sinks`
+ * and last `recent` positions and the heaviest of the others; of equal weights the
+ * lower position stays, NaN weighs less than anything.  The batch's table_width,
+ * kv_len and n_seq count, its rows do not. */
+int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const megakernel_rows* mass,
+                             int keep, int recent, int sinks, int* kept, int* kept_len, void* stream);
+
+/* Moves kept rows to blocks of their own: row r of sequence i and KV head h in
+ * the blocks of new_table [n_seq][new_width] becomes position kept[i][h][r] of the
+ * batch's table, r < min(kept_len[i], keep, new_width * block).  The same as
+ * megakernel_op_kv8_read() of these rows and megakernel_op_kv8_append() to blocks
+ * that start anew: a new block has the smallest scale that fits its rows, rows of
+ * missing blocks (and of kept entries outside the table) are zeros, rows to missing
+ * new blocks are dropped, and rows of a block behind the last stay as they were.
+ * new_table's blocks are none that the call reads, each in one entry only.  With
+ * mass and new_mass (both or neither; new_mass [n_seq][n_kv][new_width * block])
+ * the rows' weights move along.  kept_len is the new sequences' kv_len. */
+int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const int* kept,
+                              const int* kept_len, int keep, const int* new_table, int new_width, const megakernel_rows* mass,
+                              const megakernel_rows* new_mass, void* stream);
+
+/* Rotation of every head of q (n_q heads) and k (n_kv) by its token's position,
+ * without a norm, for the first `turned` dimensions of a head (even, up to
+ * head_dim, which is even and at most 1024); the others are copied.  Pairs are
+ * (i, i + turned / 2), or with `interleaved` (2i, 2i + 1);
+ *   (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t), t = pos[row] * inv_freq[i]
+ * (fp32 [turned / 2]; the angle is formed in fp64).  Types and in-place outputs are
+ * as for megakernel_op_qk_norm_rope; rows need no alignment beyond their type's,
+ * and are fastest where head_dim and turned are multiples of 16 and rows lie on
+ * 16 bytes. */
+int megakernel_op_rotary(const megakernel_rows* q, const megakernel_rows* k, const float* inv_freq, const int* pos,
+                         const megakernel_rows* q_out, const megakernel_rows* k_out, int n_tokens, int n_q, int n_kv,
+                         int head_dim, int turned, int interleaved, float amplitude, void* stream);
+
 /* Self-test of the hand-off primitive that replaces the reference's grid
  * barrier (src/barriers.cuh:38-73): one workgroup per CU runs `rounds`
  * all-gather rounds of tagged words (full tags and 4-bit packed pairs,

@@ -5,6 +5,8 @@
 // grids come from the row count alone, and each workgroup finds its sequence
 // there.
 #include "mk_kv8.h"
+#include "mk_kv8_evict.h"
+#include "mk_kv8_rotary.h"
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -19,9 +21,13 @@ static bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)
 
 static int type_size(int type) { return type == MK_TYPE_F32 ? 4 : type == MK_TYPE_BF16 ? 2 : 0; }
 
-// A tensor of rows: type, alignment for 16-byte accesses, and strides that
-// keep the heads of one token apart.
-static bool rows_ok(const char* op, const char* name, const megakernel_rows* r, int heads, int head_dim, bool bf16_only) {
+static bool rows_aligned(const megakernel_rows* r, int n) {
+  const int sz = type_size(r->type);
+  return aligned(r->p, n) && r->token_stride * sz % n == 0 && r->head_stride * sz % n == 0;
+}
+// A tensor of rows: type, alignment for 16-byte accesses (or, with align 0,
+// that of its elements), and strides that keep the heads of one token apart.
+static bool rows_ok(const char* op, const char* name, const megakernel_rows* r, int heads, int head_dim, bool bf16_only, int align = 16) {
   if (!r || !r->p) {
     set_err("%s: null %s", op, name);
     return false;
@@ -31,8 +37,8 @@ static bool rows_ok(const char* op, const char* name, const megakernel_rows* r, 
     set_err("%s: %s has type %d (%s)", op, name, r->type, bf16_only ? "bf16 only" : "bf16 or fp32");
     return false;
   }
-  if (!aligned(r->p, 16) || r->token_stride * sz % 16 || r->head_stride * sz % 16) {
-    set_err("%s: %s needs 16-byte aligned rows (strides %lld, %lld)", op, name, r->token_stride, r->head_stride);
+  if (!rows_aligned(r, align == 16 ? 16 : sz)) {
+    set_err("%s: %s needs %d-byte aligned rows (strides %lld, %lld)", op, name, align == 16 ? 16 : sz, r->token_stride, r->head_stride);
     return false;
   }
   if (r->token_stride < 0 || r->head_stride < 0 || (heads > 1 && r->head_stride < head_dim)) {
@@ -58,6 +64,25 @@ static bool two(const char* op, const char* names, const megakernel_rows* a, con
   if (a->p != b->p) return true;
   set_err("%s: %s must not be the same rows", op, names);
   return false;
+}
+
+// Queries and keys that are turned: one type in and one out, and outputs in
+// place of inputs only where a lane writes what it alone has read.
+static bool same_types(const char* op, const megakernel_rows* q, const megakernel_rows* k, const megakernel_rows* q_out,
+                       const megakernel_rows* k_out) {
+  if (q->type != k->type || q_out->type != k_out->type) {
+    set_err("%s: q and k must have one type (%d, %d), and so must q_out and k_out (%d, %d)", op, q->type, k->type,
+            q_out->type, k_out->type);
+    return false;
+  }
+  auto moved = [](const megakernel_rows* a, const megakernel_rows* b) {
+    return a->p == b->p && (a->type != b->type || a->token_stride != b->token_stride || a->head_stride != b->head_stride);
+  };
+  if (moved(q, q_out) || moved(k, k_out)) {
+    set_err("%s: an output in place of its input needs the same type and strides", op);
+    return false;
+  }
+  return true;
 }
 
 static bool cache_ok(const char* op, const megakernel_kv8_cache* c) {
@@ -418,6 +443,27 @@ static int attend(const char* op, const megakernel_kv8_cache* cache, const megak
   return launched(op, e);
 }
 
+// Weights of cached positions: fp32 rows [n_seq][n_kv] of all positions that a table holds.
+static bool mass_ok(const char* op, const char* name, const megakernel_rows* m, int n_seq, int n_kv, long long positions) {
+  if (!rows_ok(op, name, m, n_kv, (int)positions, false, 0) || !apart(op, name, m, n_kv, (int)positions, n_seq)) return false;
+  if (m->type == MK_TYPE_F32) return true;
+  set_err("%s: %s must be fp32", op, name);
+  return false;
+}
+static Mass mass_of(const megakernel_rows* m) { return Mass{static_cast<float*>(m->p), m->token_stride, m->head_stride}; }
+
+template <int D>
+static hipError_t launch_move(int pieces, long long groups, hipStream_t st, const Move& p) {
+  auto go = [&](auto kern) { return launch(kern, groups, 256, st, p); };
+  if constexpr (D == 64)
+    if (pieces == 32) return go(move<D, 32, 1>);
+  if (pieces == 64) return go(move<D, 64, 1>);
+  if (pieces == 128) return go(move<D, 128, 1>);
+  if constexpr (D == 128)
+    if (pieces == 512) return go(move<D, 256, 2>);
+  return go(move<D, 256, 1>);
+}
+
 }  // namespace kv8
 }  // namespace mk
 
@@ -452,19 +498,7 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
     set_err("%s: null or unaligned gains (16 bytes), inv_freq or pos (4)", op);
     return -1;
   }
-  if (q->type != k->type || q_out->type != k_out->type) {
-    set_err("%s: q and k must have one type (%d, %d), and so must q_out and k_out (%d, %d)", op, q->type, k->type,
-            q_out->type, k_out->type);
-    return -1;
-  }
-  // in place: a lane writes what it alone has read, if the layout is the same
-  auto moved = [](const megakernel_rows* a, const megakernel_rows* b) {
-    return a->p == b->p && (a->type != b->type || a->token_stride != b->token_stride || a->head_stride != b->head_stride);
-  };
-  if (moved(q, q_out) || moved(k, k_out)) {
-    set_err("%s: an output in place of its input needs the same type and strides", op);
-    return -1;
-  }
+  if (!same_types(op, q, k, q_out, k_out)) return -1;
   if (n_tokens == 0) return 0;
   if (!two(op, "q_out and k_out", q_out, k_out) || !two(op, "q_out and k", q_out, k) || !two(op, "k_out and q", k_out, q)) return -1;
   const int hpw = 1024 / head_dim;
@@ -558,6 +592,150 @@ int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const 
                                        long long workspace_bytes, void* stream) {
   return attend<AttnScored>("op_kv8_attention_scored", cache, batch, scores, q, out, lse, n_q, scale, d_workspace,
                             workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                            const megakernel_kv8_scores* scores, const megakernel_rows* q, const float* lse,
+                            const megakernel_rows* mass, int n_q, float scale, void* stream) {
+  const char* op = "op_kv8_weigh";
+  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !scores_ok(op, scores) || !heads_ok(op, n_q, cache->n_kv) ||
+      !rows_ok(op, "q", q, n_q, cache->head_dim, true) ||
+      !mass_ok(op, "mass", mass, batch->n_seq, cache->n_kv, (long long)batch->table_width * cache->block))
+    return -1;
+  if (!lse || !aligned(lse, 4)) {
+    set_err("%s: null lse, or not 4-byte aligned", op);
+    return -1;
+  }
+  const int group = n_q / cache->n_kv;
+  const long long rows = (long long)batch->n_tokens * group, all = (long long)batch->table_width * cache->block;
+  if (rows > (1ll << 30) || batch->n_seq * ((all + TILE - 1) / TILE) > (1ll << 30)) {
+    set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows, or n_seq=%d times %lld positions 2^36", op,
+            batch->n_tokens, group, batch->n_seq, all);
+    return -1;
+  }
+  const float scale2 = scale_of(op, scores, scale);
+  if (!scale2) return -1;
+  if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
+  Weigh p{cache_of(cache), batch_of(batch), rows_of(q), lse, mass_of(mass), n_q, group, scale2, scores_of(scores, scale2)};
+  long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all;
+  const bool split = rows > 32ll * batch->n_seq;
+  // a step of positions each, and more than one where that is more workgroups than run at once
+  long long groups = (batch->n_seq * ((kv + TILE - 1) / TILE) + (split ? 0 : 3)) / (split ? 1 : 4);
+  if (groups > 4096 / cache->n_kv) groups = 4096 / cache->n_kv;
+  groups = (groups < 1 ? 1 : groups) * cache->n_kv;
+  auto go = [&](auto kern, int threads) { return launch(kern, groups, threads, static_cast<hipStream_t>(stream), p); };
+  return launched(op, cache->head_dim == 64 ? (split ? go(weigh<64, 8, true>, 512) : go(weigh<64, 4, false>, 256))
+                                            : (split ? go(weigh<128, 8, true>, 512) : go(weigh<128, 4, false>, 256)));
+}
+
+int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const megakernel_rows* mass,
+                             int keep, int recent, int sinks, int* kept, int* kept_len, void* stream) {
+  const char* op = "op_kv8_select";
+  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block)) return -1;
+  const long long all = (long long)batch->table_width * cache->block;
+  if (!mass_ok(op, "mass", mass, batch->n_seq, cache->n_kv, all)) return -1;
+  if (keep < 1 || keep > (1 << 30) || recent < 0 || sinks < 0 || (long long)recent + sinks > keep) {
+    set_err("%s: keep=%d (1..2^30), recent=%d and sinks=%d (at least 0, together at most keep)", op, keep, recent, sinks);
+    return -1;
+  }
+  if (!kept || !kept_len || !aligned(kept, 4) || !aligned(kept_len, 4)) {
+    set_err("%s: null kept or kept_len, or not 4-byte aligned", op);
+    return -1;
+  }
+  if (batch->n_seq == 0) return 0;
+  const long long groups = (long long)batch->n_seq * cache->n_kv;
+  if (!grid_ok(op, groups * 4)) return -1;
+  Choose p{mass_of(mass), batch->kv_len, kept, kept_len, cache->n_kv, keep, recent, sinks, (int)all};
+  return launched(op, launch(choose, groups, 1024, static_cast<hipStream_t>(stream), p));
+}
+
+int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const int* kept,
+                              const int* kept_len, int keep, const int* new_table, int new_width, const megakernel_rows* mass,
+                              const megakernel_rows* new_mass, void* stream) {
+  const char* op = "op_kv8_compact";
+  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block)) return -1;
+  if (!kept || !kept_len || !new_table || !aligned(kept, 4) || !aligned(kept_len, 4) || !aligned(new_table, 4)) {
+    set_err("%s: null kept, kept_len or new_table, or not 4-byte aligned", op);
+    return -1;
+  }
+  const long long all = (long long)batch->table_width * cache->block, room = (long long)new_width * cache->block;
+  if (keep < 1 || keep > (1 << 30) || new_width < 1 || room > (1ll << 30)) {
+    set_err("%s: keep=%d (1..2^30), new_width=%d blocks of %d positions (at least 1 block, at most 2^30 positions)", op, keep,
+            new_width, cache->block);
+    return -1;
+  }
+  if (new_table == batch->table) {
+    set_err("%s: new_table must not be the batch's table", op);
+    return -1;
+  }
+  if (!mass != !new_mass) {
+    set_err("%s: mass and new_mass go together", op);
+    return -1;
+  }
+  if (mass && (!mass_ok(op, "mass", mass, batch->n_seq, cache->n_kv, all) ||
+               !mass_ok(op, "new_mass", new_mass, batch->n_seq, cache->n_kv, room) || !two(op, "mass and new_mass", mass, new_mass)))
+    return -1;
+  if (batch->n_seq == 0) return 0;
+  const int pieces = block_pieces(cache), heads = pieces < 256 ? 256 / pieces : 1;
+  const long long per = ((long long)keep + cache->block - 1) / cache->block;
+  const long long groups = batch->n_seq * per * ((cache->n_kv + heads - 1) / heads);
+  if (!grid_ok(op, groups)) return -1;
+  Move p{cache_of(cache), batch->table, kept, kept_len, new_table, batch->table_width, new_width, keep, Mass{}, Mass{}};
+  if (mass) p.from = mass_of(mass), p.to = mass_of(new_mass);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return launched(op, cache->head_dim == 64 ? launch_move<64>(pieces, groups, st, p) : launch_move<128>(pieces, groups, st, p));
+}
+
+int megakernel_op_rotary(const megakernel_rows* q, const megakernel_rows* k, const float* inv_freq, const int* pos,
+                         const megakernel_rows* q_out, const megakernel_rows* k_out, int n_tokens, int n_q, int n_kv,
+                         int head_dim, int turned, int interleaved, float amplitude, void* stream) {
+  const char* op = "op_rotary";
+  if (head_dim < 2 || head_dim > 1024 || head_dim % 2 || turned < 2 || turned > head_dim || turned % 2) {
+    set_err("%s: head_dim=%d (even, 2..1024), turned=%d (even, 2..head_dim)", op, head_dim, turned);
+    return -1;
+  }
+  if (n_q < 1 || n_q > 1024 || n_kv < 1 || n_kv > 1024 || n_tokens < 0 || n_tokens > (1 << 27)) {
+    set_err("%s: n_q=%d, n_kv=%d (both 1..1024), n_tokens=%d (0..2^27)", op, n_q, n_kv, n_tokens);
+    return -1;
+  }
+  if (!(fabsf(amplitude) < INFINITY)) {
+    set_err("%s: amplitude=%g must be finite", op, amplitude);
+    return -1;
+  }
+  if (!rows_ok(op, "q", q, n_q, head_dim, false, 0) || !rows_ok(op, "k", k, n_kv, head_dim, false, 0) ||
+      !rows_ok(op, "q_out", q_out, n_q, head_dim, false, 0) || !rows_ok(op, "k_out", k_out, n_kv, head_dim, false, 0) ||
+      !apart(op, "q_out", q_out, n_q, head_dim, n_tokens) || !apart(op, "k_out", k_out, n_kv, head_dim, n_tokens))
+    return -1;
+  if (!inv_freq || !pos || !aligned(inv_freq, 4) || !aligned(pos, 4)) {
+    set_err("%s: null or unaligned inv_freq or pos (4 bytes)", op);
+    return -1;
+  }
+  if (!same_types(op, q, k, q_out, k_out)) return -1;
+  if (n_tokens == 0) return 0;
+  if (!two(op, "q_out and k_out", q_out, k_out) || !two(op, "q_out and k", q_out, k) || !two(op, "k_out and q", k_out, q)) return -1;
+  const Turn p{rows_of(q), rows_of(k), rows_of(q_out), rows_of(k_out), inv_freq, pos, n_tokens, n_q, n_kv, head_dim, turned, amplitude};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool s32 = q->type == MK_TYPE_F32, d32 = q_out->type == MK_TYPE_F32;
+  long long groups;
+  auto go = [&](auto kern, auto... more) { return launch(kern, groups, 256, st, p, more...); };
+  if (head_dim % 16 || turned % 16 || !rows_aligned(q, 16) || !rows_aligned(k, 16) || !rows_aligned(q_out, 16) || !rows_aligned(k_out, 16)) {
+    groups = ((long long)n_tokens * (n_q + n_kv) * (head_dim / 2) + 255) / 256;
+    if (!grid_ok(op, groups)) return -1;
+    return launched(op, s32 ? (d32 ? go(rotate_pairs<true, true>, interleaved) : go(rotate_pairs<true, false>, interleaved))
+                            : (d32 ? go(rotate_pairs<false, true>, interleaved) : go(rotate_pairs<false, false>, interleaved)));
+  }
+  const long long units = (long long)n_tokens * (head_dim / 16);
+  const bool many = units * (n_q + n_kv) > 1 << 16;
+  groups = (units * (many ? (n_q + n_kv + 3) / 4 : n_q + n_kv) + 255) / 256;
+  if (!grid_ok(op, groups)) return -1;
+  auto pick = [&](auto il, auto n) {
+    constexpr bool I = decltype(il)::value;
+    constexpr int N = decltype(n)::value;
+    return s32 ? (d32 ? go(rotate<true, true, I, N>) : go(rotate<true, false, I, N>))
+               : (d32 ? go(rotate<false, true, I, N>) : go(rotate<false, false, I, N>));
+  };
+  return launched(op, interleaved ? (many ? pick(Bool<true>{}, Int<4>{}) : pick(Bool<true>{}, Int<1>{}))
+                                  : (many ? pick(Bool<false>{}, Int<4>{}) : pick(Bool<false>{}, Int<1>{})));
 }
 
 }  // extern "C"

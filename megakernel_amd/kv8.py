@@ -26,6 +26,7 @@ tensors that require one are refused.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 
 import torch
@@ -276,6 +277,67 @@ def qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q_out, k_out, eps: float =
           inv_freq.data_ptr(), pos.data_ptr(), rows[2], rows[3], tokens, n_q, n_kv, dim, eps)
 
 
+def rotary(q, k, inv_freq, pos, q_out, k_out, interleaved: bool = False, amplitude: float = 1.0):
+    """Rotation of every head of q [T][n_q][D] and k [T][n_kv][D] by its token's
+    position (int32 [T]), without a norm.  The first 2 * len(inv_freq) dimensions
+    of a head are turned, the others copied; pairs are the two halves of the
+    turned part, or with ``interleaved`` neighbours.  D is even, at most 1024.
+    Inputs and outputs are bf16 or fp32 with any token and head strides, and an
+    output may be its own input.  :func:`rotary_frequencies` gives ``inv_freq``
+    (float32) and ``amplitude``, what every turned value is multiplied by."""
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q and k are [tokens][heads][head_dim], not {tuple(q.shape)} and {tuple(k.shape)}")
+    device = q.get_device()
+    if device < 0:
+        raise ValueError(f"q must be on the GPU, not on {q.device}")
+    tokens, n_q, dim = q.shape
+    n_kv = k.shape[1]
+    _whole(pos, torch.int32, (tokens,), device, "pos")
+    _whole(inv_freq, torch.float32, (None,), device, "inv_freq")
+    qs, ks = (tokens, n_q, dim), (tokens, n_kv, dim)
+    rows = (_rows(q, qs, device, "q"), _rows(k, ks, device, "k"), _rows(q_out, qs, device, "q_out"),
+            _rows(k_out, ks, device, "k_out"))
+    if tokens == 0:
+        return
+    _call("megakernel_op_rotary", device, rows[0], rows[1], inv_freq.data_ptr(), pos.data_ptr(), rows[2], rows[3], tokens,
+          n_q, n_kv, dim, 2 * inv_freq.shape[0], bool(interleaved), amplitude)
+
+
+def rotary_frequencies(dims: int, theta: float = 1e6, scaling: str | None = None, factor: float = 1.0, original: int = 0,
+                       fast: float = 32.0, slow: float = 1.0, device="cuda"):
+    """(inv_freq, amplitude) for :func:`rotary` of ``dims`` dimensions: theta^(-2i / dims),
+    for contexts ``factor`` times as long as trained for scaled by
+
+    ``"linear"``  positions divided by the factor;
+    ``"base"``    theta times factor^(dims / (dims - 2)), which leaves the
+                  fastest pair as it is and divides the slowest by the factor;
+    ``"parts"``   pairs that turn more than ``fast`` times within the
+                  ``original`` context as they are, those that turn less than
+                  ``slow`` times divided by the factor, a ramp over the turns
+                  between; the amplitude is 0.1 ln(factor) + 1.
+
+    Computed in double precision, rounded once to float32."""
+    if dims < 2 or dims % 2:
+        raise ValueError(f"dims {dims} must be even and at least 2")
+    if not (theta > 0 and math.isfinite(theta) and factor >= 1 and math.isfinite(factor)):
+        raise ValueError(f"theta {theta} (above 0), factor {factor} (at least 1)")
+    amplitude = 1.0
+    if scaling == "base" and dims > 2:
+        theta *= factor ** (dims / (dims - 2))
+    inv = [theta ** (-2.0 * i / dims) for i in range(dims // 2)]
+    if scaling == "linear":
+        inv = [f / factor for f in inv]
+    elif scaling == "parts":
+        if original < 1 or not fast > slow > 0:
+            raise ValueError(f"original {original} (at least 1), fast {fast} and slow {slow} (fast above slow above 0)")
+        stay = [min(max((original * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0) for f in inv]
+        inv = [f * s + f / factor * (1 - s) for f, s in zip(inv, stay)]
+        amplitude = 0.1 * math.log(factor) + 1
+    elif scaling not in (None, "base"):
+        raise ValueError(f"scaling {scaling!r} (None, 'linear', 'base' or 'parts')")
+    return torch.tensor(inv, dtype=torch.float64).to(torch.float32).to(device), amplitude
+
+
 def _one_gpu(cache: Cache, batch: Batch):
     if cache.device != batch.device:
         raise ValueError(f"the batch is on cuda:{batch.device}, not on cuda:{cache.device}")
@@ -363,3 +425,82 @@ def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, wo
     else:
         _call("megakernel_op_kv8_attention_scored", device, cache._ref, batch._ref, x._ref, a, b,
               None if lse is None else lse.data_ptr(), n_q, scale, at, size or 0)
+
+
+def _mass(t, cache: Cache, n_seq: int, positions: int, name: str) -> bytes:
+    """Weights [n_seq][n_kv][at least `positions`] as a megakernel_rows."""
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name} must be torch.float32, not {t.dtype}")
+    if t.dim() != 3 or t.shape[2] < positions:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {(n_seq, cache.n_kv, positions)} (or more positions)")
+    return _rows(t, (n_seq, cache.n_kv, t.shape[2]), cache.device, name)
+
+
+def weigh(cache: Cache, batch: Batch, q, lse, mass, scale: float | None = None, scores: Scores | None = None):
+    """Add up what each cached position is worth: mass [n_seq][n_kv][positions]
+    (float32, any sequence and head strides, at least the table's positions) gains
+    the attention weights that the batch's rows give each position, summed over
+    rows and the query heads that share a KV head.  ``q``, ``scale`` and ``scores``
+    are those of the :func:`attention` that gave ``lse``.  Positions of the batch's
+    own rows start from zero, those before them from what mass holds; positions
+    past a length stay as they are."""
+    if q.dim() != 3:
+        raise ValueError(f"q is [tokens][heads][head_dim], not {tuple(q.shape)}")
+    _one_gpu(cache, batch)
+    device, n_q = cache.device, q.shape[1]
+    a = _rows(q, (batch.n_tokens, n_q, cache.head_dim), device, "q", _BF16)
+    _whole(lse, torch.float32, (batch.n_tokens, n_q), device, "lse")
+    b = _mass(mass, cache, batch.n_seq, batch.table.shape[1] * cache.block, "mass")
+    x = _scores(scores, batch, n_q)
+    if batch.n_seq and batch.n_tokens:
+        _call("megakernel_op_kv8_weigh", device, cache._ref, batch._ref, x._ref, a, lse.data_ptr(), b, n_q,
+              cache.head_dim ** -0.5 if scale is None else scale)
+
+
+def _kept(cache: Cache, batch: Batch, kept, kept_len):
+    _whole(kept, torch.int32, (batch.n_seq, cache.n_kv, None), cache.device, "kept")
+    _whole(kept_len, torch.int32, (batch.n_seq,), cache.device, "kept_len")
+    if kept.shape[2] < 1:
+        raise ValueError("kept needs room for at least 1 position")
+
+
+def select(cache: Cache, batch: Batch, mass, kept, kept_len, recent: int = 0, sinks: int = 0):
+    """The positions worth keeping of each sequence and KV head: kept
+    [n_seq][n_kv][keep] (int32) receives them in rising order, -1 behind the last,
+    and kept_len [n_seq] (int32) their number, min(kv_len, keep).  Of a longer
+    sequence they are its first ``sinks``, its last ``recent`` and the heaviest of
+    the others by ``mass`` (:func:`weigh`); of equal weights the lower position,
+    and NaN last."""
+    _one_gpu(cache, batch)
+    _kept(cache, batch, kept, kept_len)
+    a = _mass(mass, cache, batch.n_seq, batch.table.shape[1] * cache.block, "mass")
+    if batch.n_seq:
+        _call("megakernel_op_kv8_select", cache.device, cache._ref, batch._ref, a, kept.shape[2], recent, sinks,
+              kept.data_ptr(), kept_len.data_ptr())
+
+
+def compact(cache: Cache, batch: Batch, kept, kept_len, new_table, mass=None, new_mass=None):
+    """Move the kept rows (:func:`select`) to the blocks of new_table
+    [n_seq][width] (int32), in order and quantised anew: :func:`read` followed by
+    :func:`append` to blocks that start anew.  These blocks are none that the
+    batch's table names, and each stands in one entry; the old ones are free
+    afterwards.  With ``mass`` and ``new_mass`` ([n_seq][n_kv][the new table's
+    positions]) the rows' weights move along.  A :class:`Batch` of new_table with
+    kept_len as its lengths goes on from there: its positions are places in the
+    cache, so scores that count positions (a window, slopes, documents) count
+    kept ones, and the rotation goes on from the sequence's own position."""
+    _one_gpu(cache, batch)
+    _kept(cache, batch, kept, kept_len)
+    device = cache.device
+    _whole(new_table, torch.int32, (batch.n_seq, None), device, "new_table")
+    if new_table.shape[1] < 1:
+        raise ValueError("new_table needs a width of at least 1")
+    if (mass is None) != (new_mass is None):
+        raise ValueError("mass and new_mass go together")
+    a = b = None
+    if mass is not None:
+        a = _mass(mass, cache, batch.n_seq, batch.table.shape[1] * cache.block, "mass")
+        b = _mass(new_mass, cache, batch.n_seq, new_table.shape[1] * cache.block, "new_mass")
+    if batch.n_seq:
+        _call("megakernel_op_kv8_compact", device, cache._ref, batch._ref, kept.data_ptr(), kept_len.data_ptr(),
+              kept.shape[2], new_table.data_ptr(), new_table.shape[1], a, b)
