@@ -456,11 +456,11 @@ template <int D>
 static hipError_t launch_move(int pieces, long long groups, hipStream_t st, const Move& p) {
   auto go = [&](auto kern) { return launch(kern, groups, 256, st, p); };
   if constexpr (D == 64)
-    if (pieces == 32) return go(move<D, 32, 1>);
-  if (pieces == 64) return go(move<D, 64, 1>);
+    if (pieces == 64) return go(move<D, 64, 1>);
   if (pieces == 128) return go(move<D, 128, 1>);
+  if (pieces == 512) return go(move<D, 256, 2>);
   if constexpr (D == 128)
-    if (pieces == 512) return go(move<D, 256, 2>);
+    if (pieces == 1024) return go(move<D, 256, 4>);
   return go(move<D, 256, 1>);
 }
 
@@ -608,8 +608,8 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
   }
   const int group = n_q / cache->n_kv;
   const long long rows = (long long)batch->n_tokens * group, all = (long long)batch->table_width * cache->block;
-  if (rows > (1ll << 30) || batch->n_seq * ((all + TILE - 1) / TILE) > (1ll << 30)) {
-    set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows, or n_seq=%d times %lld positions 2^36", op,
+  if (rows > (1ll << 30) || batch->n_seq * ((all + 31) / 32) > (1ll << 30)) {
+    set_err("%s: n_tokens=%d times %d query heads per KV head exceeds 2^30 rows, or n_seq=%d times %lld positions 2^35", op,
             batch->n_tokens, group, batch->n_seq, all);
     return -1;
   }
@@ -618,14 +618,19 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
   if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
   Weigh p{cache_of(cache), batch_of(batch), rows_of(q), lse, mass_of(mass), n_q, group, scale2, scores_of(scores, scale2)};
   long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all;
-  const bool split = rows > 32ll * batch->n_seq;
-  // a step of positions each, and more than one where that is more workgroups than run at once
-  long long groups = (batch->n_seq * ((kv + TILE - 1) / TILE) + (split ? 0 : 3)) / (split ? 1 : 4);
+  const bool many = rows > 32ll * batch->n_seq;
+  // Steps of 64 positions: a wave's with few rows, a workgroup's with many, of 32
+  // where those would not be two workgroups for every CU.  More than one step each
+  // where that is more workgroups than run at once.
+  const long long steps = (kv + TILE - 1) / TILE * batch->n_seq;
+  const bool half = many && steps * cache->n_kv < 1024;
+  long long groups = half ? 2 * steps : many ? steps : (steps + 3) / 4;
   if (groups > 4096 / cache->n_kv) groups = 4096 / cache->n_kv;
   groups = (groups < 1 ? 1 : groups) * cache->n_kv;
   auto go = [&](auto kern, int threads) { return launch(kern, groups, threads, static_cast<hipStream_t>(stream), p); };
-  return launched(op, cache->head_dim == 64 ? (split ? go(weigh<64, 8, true>, 512) : go(weigh<64, 4, false>, 256))
-                                            : (split ? go(weigh<128, 8, true>, 512) : go(weigh<128, 4, false>, 256)));
+  if (!many) return launched(op, cache->head_dim == 64 ? go(weigh_few<64>, 256) : go(weigh_few<128>, 256));
+  return launched(op, cache->head_dim == 64 ? (half ? go(weigh_many<64, 1>, 512) : go(weigh_many<64, 2>, 512))
+                                            : (half ? go(weigh_many<128, 1>, 512) : go(weigh_many<128, 2>, 512)));
 }
 
 int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const megakernel_rows* mass,
@@ -646,7 +651,9 @@ int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel
   const long long groups = (long long)batch->n_seq * cache->n_kv;
   if (!grid_ok(op, groups * 4)) return -1;
   Choose p{mass_of(mass), batch->kv_len, kept, kept_len, cache->n_kv, keep, recent, sinks, (int)all};
-  return launched(op, launch(choose, groups, 1024, static_cast<hipStream_t>(stream), p));
+  const long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all, most = kv - recent - sinks;
+  auto go = [&](auto kern) { return launch(kern, groups, 1024, static_cast<hipStream_t>(stream), p); };
+  return launched(op, most <= 4096 ? go(choose<4>) : go(choose<32>));
 }
 
 int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const int* kept,
@@ -676,7 +683,7 @@ int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakerne
                !mass_ok(op, "new_mass", new_mass, batch->n_seq, cache->n_kv, room) || !two(op, "mass and new_mass", mass, new_mass)))
     return -1;
   if (batch->n_seq == 0) return 0;
-  const int pieces = block_pieces(cache), heads = pieces < 256 ? 256 / pieces : 1;
+  const int pieces = cache->block * cache->head_dim / 16, heads = pieces < 256 ? 256 / pieces : 1;
   const long long per = ((long long)keep + cache->block - 1) / cache->block;
   const long long groups = batch->n_seq * per * ((cache->n_kv + heads - 1) / heads);
   if (!grid_ok(op, groups)) return -1;

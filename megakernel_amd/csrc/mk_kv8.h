@@ -663,29 +663,31 @@ struct Bounds {
 // small.  For caps of up to 64 that is what rounding scores of tens costs
 // anyway; for larger ones tanh is its series where |y| is below 1/4 (the first
 // term left out is 2^-26.8 of the value).
-__device__ __forceinline__ float capped(const Scores& x, float s) {
+__device__ __forceinline__ float capped(const Scores& x, float s, float top) {  // top: the cap and what is added
   const float t = __builtin_amdgcn_exp2f(s * x.cap_in);
-  return fmaf(-2.f * x.cap, __builtin_amdgcn_rcpf(t + 1.f), x.cap);
+  return fmaf(-2.f * x.cap, __builtin_amdgcn_rcpf(t + 1.f), top);
 }
-__device__ __forceinline__ float capped_wide(const Scores& x, float s, float scale) {
+__device__ __forceinline__ float capped_wide(const Scores& x, float s, float scale, float add) {
   const float y = s * x.cap_in * 0.34657359027997264f;  // ln(2) / 2
   const float z = y * y;
   const float r = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
-  return fabsf(y) < 0.25f ? s * scale * r : capped(x, s);
+  const int tall = opaque_v(__float_as_int(capped(x, s, x.cap + add)));  // both, and no branch for every score
+  return fabsf(y) < 0.25f ? fmaf(s * scale, r, add) : __int_as_float(tall);
 }
-// Scores of one row to base 2, in place: N of them, at(i) is the position of
-// the i-th less that of the row.
+// Scores of one row to base 2, with `add` added, in place: N of them, at(i) is
+// the position of the i-th less that of the row.
 template <int N, class At>
-__device__ __forceinline__ void score(const Scores& x, float scale, float slope, float* s, At at) {
+__device__ __forceinline__ void score(const Scores& x, float scale, float slope, float add, float* s, At at) {
   if (!x.cap) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] *= scale;
+    for (int i = 0; i < N; ++i) s[i] = fmaf(s[i], scale, add);
   } else if (!x.wide) {
+    const float top = x.cap + add;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = capped(x, s[i]);
+    for (int i = 0; i < N; ++i) s[i] = capped(x, s[i], top);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = capped_wide(x, s[i], scale);
+    for (int i = 0; i < N; ++i) s[i] = capped_wide(x, s[i], scale, add);
   }
   if (x.slopes) {
 #pragma unroll
@@ -978,7 +980,6 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
   // the weights' reference of row c (or -inf), it negated (or 0), and what the
   // lane's scores may reach before it is raised
   float m = -INFINITY, below = 0.f, up = -INFINITY, sum = 0.f, ex = 0.f;  // ex: of the weights as they are, for the log-sum-exp
-  const float scale = SCORED ? 1.f : p.scale;  // of what score() left
 
   // Both are waited for here: left to itself, the second would be asked for
   // behind the first codes, and the loop's waits be for everything.
@@ -1012,7 +1013,7 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = sc[i / 4][i % 4];
       const int rel = pv - (s.pos0 + tok);
-      score<16>(p.x, p.scale, slope, x, [&](int i) { return rel + i; });
+      score<16>(p.x, p.scale, slope, below, x, [&](int i) { return rel + i; });
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i / 4][i % 4] = x[i];
     }
@@ -1059,10 +1060,15 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) mt = fmaxf(mt, sc[i][j]);
-    mt *= scale;
+    mt = SCORED ? mt - below : mt * p.scale;
     if (__any(mt > up)) {  // joined over the row's four lanes only here
       const float mn = fmaxf(m, max_xor32(max_xor16(mt))), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
+      if constexpr (SCORED) {  // scores are less the reference from the start
+        const float d = (mn == -INFINITY ? 0.f : -mn) - below;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] += d;
+      }
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
@@ -1075,7 +1081,7 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        pr[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], scale, below));
+        pr[4 * i + j] = __builtin_amdgcn_exp2f(SCORED ? sc[i][j] : fmaf(sc[i][j], p.scale, below));
       }
     if constexpr (SCORED) {
       if (p.lse) {
@@ -1227,7 +1233,6 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     shut = v.lo, see = mine ? v.hi : 0;
     if (p.x.slopes) slope = p.x.slopes[hd] * 1.4426950408889634f;
   }
-  const float scale = SCORED ? 1.f : p.scale;  // of what score() left
   const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
   const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);
   const int n = t1 - t0, end = min(s.len, t1 * TILE);
@@ -1407,7 +1412,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = sc[a][i];
-        score<16>(p.x, p.scale, slope, x, [&](int i) { return rel + place(a, i); });
+        score<16>(p.x, p.scale, slope, below, x, [&](int i) { return rel + place(a, i); });
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[a][i] = x[i];
       }
@@ -1426,10 +1431,17 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[a][i]);
-    mt *= scale;
+    mt = SCORED ? mt - below : mt * p.scale;
     if (__any(mt > up)) {
       const float mn = fmaxf(m, max_xor32(mt)), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
+      if constexpr (SCORED) {  // scores are less the reference from the start
+        const float d = (mn == -INFINITY ? 0.f : -mn) - below;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[a][i] += d;
+      }
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
@@ -1460,8 +1472,8 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     const auto weights = [&](int a) {
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(sc[a][i], scale, below));
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[a][i + 1], scale, below));
+        const float x = __builtin_amdgcn_exp2f(SCORED ? sc[a][i] : fmaf(sc[a][i], p.scale, below));
+        const float y = __builtin_amdgcn_exp2f(SCORED ? sc[a][i + 1] : fmaf(sc[a][i + 1], p.scale, below));
         if constexpr (SCORED) ex += x + y;
         const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
         sum = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum, false);  // of the rounded weights
