@@ -539,9 +539,10 @@ typedef struct {
 /* megakernel_op_kv8_attention with such scores, and with the rows'
  * log-sum-exps: lse [n_tokens][n_q] (fp32, NULL where not wanted) receives
  * ln sum_j e^s, -infinity for a row that sees nothing.  Its workspace is of
- * megakernel_op_kv8_scored_workspace_bytes(...) bytes. */
+ * megakernel_op_kv8_scored_workspace_bytes(...) bytes, with_lse not 0 where lse
+ * is wanted. */
 long long megakernel_op_kv8_scored_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
-                                                   const megakernel_kv8_scores* scores, int n_q);
+                                                   const megakernel_kv8_scores* scores, int n_q, int with_lse);
 int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                                        const megakernel_kv8_scores* scores, const megakernel_rows* q,
                                        const megakernel_rows* out, float* lse, int n_q, float scale, void* workspace,

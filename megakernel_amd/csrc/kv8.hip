@@ -297,10 +297,10 @@ static long long part_rows(const Plan& p, int k, int n_kv) { return p.slots[k] *
 static long long part_bytes(const Plan& p, int k, int n_kv, int head_dim) {
   return part_floats(p, k, n_kv, head_dim) * 4 + part_rows(p, k, n_kv) * 8;
 }
-// `scored`: with the sums of the weights before their rounding, behind the rest
-static long long workspace(const Plan& p, int n_kv, int head_dim, bool scored) {
+// `lse`: with the sums of the weights before their rounding, behind the rest
+static long long workspace(const Plan& p, int n_kv, int head_dim, bool lse) {
   return part_bytes(p, FEW, n_kv, head_dim) + part_bytes(p, MANY, n_kv, head_dim) +
-         (scored ? 4 * (part_rows(p, FEW, n_kv) + part_rows(p, MANY, n_kv)) : 0);
+         (lse ? 4 * (part_rows(p, FEW, n_kv) + part_rows(p, MANY, n_kv)) : 0);
 }
 
 static bool heads_ok(const char* op, int n_q, int n_kv) {
@@ -364,12 +364,12 @@ static Scores scores_of(const megakernel_kv8_scores* x, float scale2) {
   return r;
 }
 
-// P: Attn, or AttnScored with x and where wanted lse.
+// P: Attn, AttnScored with x, or AttnLse with x and lse.
 template <class P>
 static int attend(const char* op, const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                   const megakernel_kv8_scores* x, const megakernel_rows* q, const megakernel_rows* out, float* lse, int n_q,
                   float scale, void* d_workspace, long long workspace_bytes, hipStream_t st) {
-  constexpr bool SCORED = IsScored<P>::value;
+  constexpr bool SCORED = Has<P>::scores, LSE = Has<P>::lse;
   if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !heads_ok(op, n_q, cache->n_kv) ||
       !rows_ok(op, "q", q, n_q, cache->head_dim, true) || !rows_ok(op, "out", out, n_q, cache->head_dim, true) ||
       !apart(op, "out", out, n_q, cache->head_dim, batch->n_tokens) || (SCORED && !scores_ok(op, x)))
@@ -389,7 +389,7 @@ static int attend(const char* op, const megakernel_kv8_cache* cache, const megak
   const float scale2 = scale_of(op, x, scale);
   if (!scale2) return -1;
   const Plan pl = plan(cache, batch, n_q, SCORED ? x->window : 0);
-  const long long need = workspace(pl, cache->n_kv, cache->head_dim, SCORED);
+  const long long need = workspace(pl, cache->n_kv, cache->head_dim, LSE);
   if (need && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < need)) {
     set_err("%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", op, need, d_workspace ? workspace_bytes : 0);
     return -1;
@@ -412,8 +412,8 @@ static int attend(const char* op, const megakernel_kv8_cache* cache, const megak
     d.ml = reinterpret_cast<float2*>(d.part + part_floats(pl, k, cache->n_kv, cache->head_dim));
     ws += part_bytes(pl, k, cache->n_kv, cache->head_dim);
   }
-  if constexpr (SCORED) {
-    p.x = scores_of(x, scale2);
+  if constexpr (SCORED) p.x = scores_of(x, scale2);
+  if constexpr (LSE) {
     p.lse = lse;
     p.ex[FEW] = reinterpret_cast<float*>(ws);
     p.ex[MANY] = p.ex[FEW] + part_rows(pl, FEW, cache->n_kv);
@@ -580,18 +580,19 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
 }
 
 long long megakernel_op_kv8_scored_workspace_bytes(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
-                                                   const megakernel_kv8_scores* scores, int n_q) {
+                                                   const megakernel_kv8_scores* scores, int n_q, int with_lse) {
   const char* op = "op_kv8_scored_workspace_bytes";
   if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !scores_ok(op, scores) || !heads_ok(op, n_q, cache->n_kv)) return -1;
-  return workspace(plan(cache, batch, n_q, scores->window), cache->n_kv, cache->head_dim, true);
+  return workspace(plan(cache, batch, n_q, scores->window), cache->n_kv, cache->head_dim, with_lse != 0);
 }
 
 int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                                        const megakernel_kv8_scores* scores, const megakernel_rows* q,
                                        const megakernel_rows* out, float* lse, int n_q, float scale, void* d_workspace,
                                        long long workspace_bytes, void* stream) {
-  return attend<AttnScored>("op_kv8_attention_scored", cache, batch, scores, q, out, lse, n_q, scale, d_workspace,
-                            workspace_bytes, static_cast<hipStream_t>(stream));
+  const auto go = lse ? attend<AttnLse> : attend<AttnScored>;
+  return go("op_kv8_attention_scored", cache, batch, scores, q, out, lse, n_q, scale, d_workspace, workspace_bytes,
+            static_cast<hipStream_t>(stream));
 }
 
 int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,

@@ -580,16 +580,14 @@ struct Scores {
 // The attention with such scores, or with each row's log-sum-exp.
 struct AttnScored : Attn {
   Scores x;
-  float* lse;    // [n_tokens][n_q], or null
+};
+struct AttnLse : AttnScored {
+  float* lse;    // [n_tokens][n_q]
   float* ex[2];  // with splits, next to Deal::ml: sums of the weights as they were before their rounding
 };
 template <class P>
-struct IsScored {
-  static constexpr bool value = false;
-};
-template <>
-struct IsScored<AttnScored> {
-  static constexpr bool value = true;
+struct Has {
+  static constexpr bool scores = __is_base_of(AttnScored, P), lse = __is_base_of(AttnLse, P);
 };
 
 constexpr int ROWS = 16;        // query rows of attn_rows's tile (the matrix columns)
@@ -849,7 +847,7 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t lo, uint32_t hi, float s) 
 
 // ln sum_j e^(s_j) of a row from its scores' reference m (to base 2) and the
 // sum of 2^(s - m); -inf of a row that sees nothing.
-__device__ __forceinline__ void put_lse(const AttnScored& p, long long row, int h, float m, float sum) {
+__device__ __forceinline__ void put_lse(const AttnLse& p, long long row, int h, float m, float sum) {
   p.lse[row * p.n_q + h] = (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
@@ -881,18 +879,18 @@ struct Ids {
 // tokens each of 16 sequences of 700 to 8,191 37 us (148 MB, 32 and 5); 64
 // sequences of 4,096, head_dim 64, 52 us (268 MB, 5.1 TB/s).  Streaming as many
 // bytes without any work takes 7, 12, 27 and 48 us here.
-template <int D, int W, bool SCORED>
+template <int D, int W, bool LSE>
 struct RowsLds {
   float lo[W][ROWS][D + 4];
   float lm[W][ROWS], ls[W][ROWS];
-  float le[SCORED ? W : 1][ROWS];
+  float le[LSE ? W : 1][ROWS];
 };
 
 template <int D, int W, class P>
 __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
   constexpr int KH = D / 64, DT = D / 16;  // 64-dimension halves of K, 16-dimension tiles of V
-  constexpr bool SCORED = IsScored<P>::value;
-  typedef RowsLds<D, W, SCORED> Lds;
+  constexpr bool SCORED = Has<P>::scores, LSE = Has<P>::lse;
+  typedef RowsLds<D, W, LSE> Lds;
   Lds& lds = *static_cast<Lds*>(smem);
   auto &lm = lds.lm, &ls = lds.ls;
   auto& lo = lds.lo;
@@ -1072,7 +1070,7 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
-      if constexpr (SCORED) ex *= al;
+      if constexpr (LSE) ex *= al;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= al;
     }
@@ -1083,11 +1081,9 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
       for (int j = 0; j < 4; ++j) {
         pr[4 * i + j] = __builtin_amdgcn_exp2f(SCORED ? sc[i][j] : fmaf(sc[i][j], p.scale, below));
       }
-    if constexpr (SCORED) {
-      if (p.lse) {
+    if constexpr (LSE) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ex += pr[i];
-      }
+      for (int i = 0; i < 16; ++i) ex += pr[i];
     }
     const bf16x2 one = bf16x2{(__bf16)1.f, (__bf16)1.f};
     bf16x8 pb[2];
@@ -1116,12 +1112,12 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
   }
 
   sum = sum_xor32(sum_xor16(sum));
-  if constexpr (SCORED) ex = sum_xor32(sum_xor16(ex));
+  if constexpr (LSE) ex = sum_xor32(sum_xor16(ex));
 
   // join the waves: o[d][i] is dimension 16d + 4g + i of row c
   if (mine) {
     if (g == 0) lm[wv][c] = m, ls[wv][c] = sum;
-    if constexpr (SCORED) {
+    if constexpr (LSE) {
       if (g == 0) lds.le[wv][c] = ex;
     }
 #pragma unroll
@@ -1140,12 +1136,12 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     for (int w = 0; w < W; ++w) {
       const float f = __builtin_amdgcn_exp2f(lm[w][row] - mref);
       tot += f * ls[w][row];
-      if constexpr (SCORED) te += f * lds.le[w][row];
+      if constexpr (LSE) te += f * lds.le[w][row];
       v += f * *reinterpret_cast<const f32x4*>(&lo[w][row][d]);
     }
     const int tk = (r0 + row) / G, oh = head * G + (r0 + row) % G;
-    if constexpr (SCORED) {
-      if (p.lse && d == 0) {
+    if constexpr (LSE) {
+      if (d == 0) {
         if (it.ns == 1) put_lse(p, s.row0 + tk, oh, mm, te);
         else p.ex[FEW][((long long)(it.slot + it.split) * p.c.n_kv + head) * ROWS + row] = te;
       }
@@ -1196,7 +1192,7 @@ struct TileLds {
 
 template <int D, class P>
 __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
-  constexpr bool SCORED = IsScored<P>::value;
+  constexpr bool SCORED = Has<P>::scores, LSE = Has<P>::lse;
   constexpr int KC = D / 16, DB = D / 32;    // 16-dimension pieces of a K row, 32-dimension blocks of V
   constexpr int NL = D * TILE / (256 * 16);  // 16-byte loads per thread of K, and of V
   typedef TileLds<D> Lds;
@@ -1357,6 +1353,14 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
         sc[a] = mfma32(*reinterpret_cast<const bf16x8*>(&lds.k[k & 1][(32 * a + c) * KS + 16 * j + 8 * h]), qv[j], sc[a]);
   };
 
+  const auto half_scores = [&](int k, int a) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[a][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < KC; ++j)
+      sc[a] = mfma32(*reinterpret_cast<const bf16x8*>(&lds.k[k & 1][(32 * a + c) * KS + 16 * j + 8 * h]), qv[j], sc[a]);
+  };
+
   // Step k's scores are there when its turn comes; its turn is: V of step
   // k + 1 to bf16, the weights, step k + 1's scores, the product with V, K of
   // step k + 2 to bf16.  What is staged was asked for a turn before.
@@ -1445,7 +1449,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
-      if constexpr (SCORED) ex *= al;
+      if constexpr (LSE) ex *= al;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1474,7 +1478,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
       for (int i = 0; i < 16; i += 2) {
         const float x = __builtin_amdgcn_exp2f(SCORED ? sc[a][i] : fmaf(sc[a][i], p.scale, below));
         const float y = __builtin_amdgcn_exp2f(SCORED ? sc[a][i + 1] : fmaf(sc[a][i + 1], p.scale, below));
-        if constexpr (SCORED) ex += x + y;
+        if constexpr (LSE) ex += x + y;
         const bf16x2 w = __builtin_convertvector(f32x2{x, y}, bf16x2);
         sum = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum, false);  // of the rounded weights
         pb[a][i / 8][i % 8] = w[0];
@@ -1489,18 +1493,29 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
           o[d] = mfma32(*reinterpret_cast<const bf16x8*>(&lds.v[buf][(32 * d + c) * VS + 32 * a + 16 * i + 8 * h]), pb[a][i], o[d]);
     };
     weights(0);
-    weights(1);
-    scores(k + 1);  // of the last step, of nothing: not used
-    add_v(0);
-    add_v(1);
+    if constexpr (SCORED) {
+      // a half's weights beside the other's products (1,024 capped tokens of
+      // head_dim 128 at 16,384 positions 191 us; as below 193, ragged prompts 220
+      // and 234)
+      half_scores(k + 1, 0);
+      add_v(0);
+      weights(1);
+      half_scores(k + 1, 1);
+      add_v(1);
+    } else {
+      weights(1);
+      scores(k + 1);  // of the last step, of nothing: not used
+      add_v(0);
+      add_v(1);
+    }
     stage_k(k + 2);
     load_k(k + 3);
     __syncthreads();
   }
   sum = sum_xor32(sum);
-  if constexpr (SCORED) {
+  if constexpr (LSE) {
     ex = sum_xor32(ex);
-    if (p.lse && mine && h == 0) {
+    if (mine && h == 0) {
       if (it.ns == 1) put_lse(p, s.row0 + tok, hd, m, ex);
       else p.ex[MANY][((long long)(it.slot + it.split) * p.c.n_kv + head) * TILE_ROWS + 32 * wv + c] = ex;
     }
@@ -1533,7 +1548,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
 
 template <int D, int W, class P>
 __global__ __launch_bounds__(W* kWave, D == 64 ? 3 : 2) void attn_rows(P p) {
-  __shared__ __align__(16) RowsLds<D, W, IsScored<P>::value> lds;
+  __shared__ __align__(16) RowsLds<D, W, Has<P>::lse> lds;
   rows_item<D, W>(p, (int)blockIdx.x, &lds);
 }
 template <int D, class P>
@@ -1547,7 +1562,7 @@ template <int D, class P>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_both(P p) {
   __shared__ __align__(16) union {
     TileLds<D> t;
-    RowsLds<D, 4, IsScored<P>::value> r;
+    RowsLds<D, 4, Has<P>::lse> r;
   } lds;
   const int many = p.d[MANY].items * p.c.n_kv;
   if ((int)blockIdx.x < many) tile_item<D>(p, (int)blockIdx.x, &lds);
@@ -1571,7 +1586,7 @@ __device__ __forceinline__ Parts parts_of(const Attn& p, const Item& it, int oh)
   x.ml = d.ml + at;
   return x;
 }
-__device__ __forceinline__ const float* ex_of(const AttnScored& p, const Item& it, const Parts& x) {
+__device__ __forceinline__ const float* ex_of(const AttnLse& p, const Item& it, const Parts& x) {
   return p.ex[it.kind] + (x.ml - p.d[it.kind].ml);
 }
 __device__ __forceinline__ void put_row4(const Rows& out, long long e, f32x4 a, float tot) {
@@ -1625,13 +1640,11 @@ __global__ __launch_bounds__(256) void attn_join_waves(P p) {
     if (NG == 4) tot = sum_xor16(tot);
     tot = sum_xor32(tot);
     if (grp == 0) put_row4(p.out, (it.s.row0 + it.rt) * p.out.ts + oh * p.out.hs + 4 * ln, a, tot);
-    if constexpr (IsScored<P>::value) {
-      if (p.lse) {
-        float te = 0.f;
-        for (int z = l; z < ns; z += kWave) te += __builtin_amdgcn_exp2f(x.ml[z * x.stride].x - mref) * ex_of(p, it, x)[z * x.stride];
-        te = wave_sum(te);
-        if (l == 0) put_lse(p, it.s.row0 + it.rt, oh, mm, te);
-      }
+    if constexpr (Has<P>::lse) {
+      float te = 0.f;
+      for (int z = l; z < ns; z += kWave) te += __builtin_amdgcn_exp2f(x.ml[z * x.stride].x - mref) * ex_of(p, it, x)[z * x.stride];
+      te = wave_sum(te);
+      if (l == 0) put_lse(p, it.s.row0 + it.rt, oh, mm, te);
     }
   }
 }
@@ -1662,11 +1675,9 @@ __global__ __launch_bounds__(256) void attn_join(P p) {
   const float w = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(q.x - mm);
   lw[tz] = w;
   const float tot = block_sum<4>(w * q.y, red1);
-  if constexpr (IsScored<P>::value) {
-    if (p.lse) {
-      const float te = block_sum<4>(tz < ns ? w * ex_of(p, it, x)[tz * x.stride] : 0.f, red1);
-      if (tz == 0) put_lse(p, it.s.row0 + it.rt, oh, mm, te);
-    }
+  if constexpr (Has<P>::lse) {
+    const float te = block_sum<4>(tz < ns ? w * ex_of(p, it, x)[tz * x.stride] : 0.f, red1);
+    if (tz == 0) put_lse(p, it.s.row0 + it.rt, oh, mm, te);
   }
   f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll

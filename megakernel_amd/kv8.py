@@ -372,13 +372,13 @@ def workspace_bytes(cache: Cache, batch: Batch, n_q: int, scores: Scores | None 
     """Bytes of :func:`attention`'s workspace for these sizes (0: none), with
     scores and a log-sum-exp as the call will have them."""
     scored = scores is not None or lse
-    key = (cache.n_kv, cache.head_dim, cache.block, n_q, (scores.window if scores else 0) if scored else None)
+    key = (cache.n_kv, cache.head_dim, cache.block, n_q, (scores.window if scores else 0, lse) if scored else None)
     need = batch._need.get(key)
     if need is None:
         lib = _lib.load()
         if scored:
             x = _scores(scores, batch, n_q)
-            need = lib.megakernel_op_kv8_scored_workspace_bytes(cache._ref, batch._ref, x._ref, n_q)
+            need = lib.megakernel_op_kv8_scored_workspace_bytes(cache._ref, batch._ref, x._ref, n_q, lse)
         else:
             need = lib.megakernel_op_kv8_workspace_bytes(cache._ref, batch._ref, n_q)
         batch._need[key] = _lib.check(lib, need, "op_kv8_workspace_bytes")
