@@ -927,7 +927,8 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     const int top = min((t1 * TILE - 1) >> lb, p.b.width - 1);  // the last entry that this item may need
     return Ids{row[min((t * TILE + 16 * (c >> 2)) >> lb, top)], row[min((t * TILE + 16 * g) >> lb, top)]};
   };
-  const auto there = [&](int id, int pos) { return pos < s.len && id >= 0 && id < p.c.n_blocks; };
+  // (a run of 16 that no row sees is as good as missing: its block may never have been written)
+  const auto there = [&](int id, int pos) { return pos < s.len && id >= 0 && id < p.c.n_blocks && (!SCORED || pos + 16 > rows.from); };
   const unsigned bytes = (unsigned)(p.c.n_kv * D) << lb;  // of K or V of one block, all heads
   const uint8_t *kb = p.c.k + ((long long)head * D << lb), *vb = p.c.v + ((long long)head * D << lb);
   const float *ksb = p.c.ks + head, *vsb = p.c.vs + head;
@@ -1260,7 +1261,8 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     return row[min(pos >> lb, top)];
   };
   const auto confirm = [&](int w, int& tab) {  // which of them are there; the others' place is taken by block 0
-    const bool ok = first_of(16 * w) + 16 * l < end && tab >= 0 && tab < p.c.n_blocks;
+    const int pos = first_of(16 * w) + 16 * l;  // nor what no row sees: its block may never have been written
+    const bool ok = pos < end && tab >= 0 && tab < p.c.n_blocks && (!SCORED || pos + 16 > rows.from);
     tab = ok ? tab : 0;
     return __ballot(ok);
   };

@@ -294,6 +294,8 @@ def rotary(q, k, inv_freq, pos, q_out, k_out, interleaved: bool = False, amplitu
     n_kv = k.shape[1]
     _whole(pos, torch.int32, (tokens,), device, "pos")
     _whole(inv_freq, torch.float32, (None,), device, "inv_freq")
+    if not 1 <= inv_freq.shape[0] <= dim // 2 or dim % 2:
+        raise ValueError(f"inv_freq turns {2 * inv_freq.shape[0]} dimensions of heads of {dim} (2 to all, and heads even)")
     qs, ks = (tokens, n_q, dim), (tokens, n_kv, dim)
     rows = (_rows(q, qs, device, "q"), _rows(k, ks, device, "k"), _rows(q_out, qs, device, "q_out"),
             _rows(k_out, ks, device, "k_out"))
@@ -460,8 +462,8 @@ def weigh(cache: Cache, batch: Batch, q, lse, mass, scale: float | None = None, 
 def _kept(cache: Cache, batch: Batch, kept, kept_len):
     _whole(kept, torch.int32, (batch.n_seq, cache.n_kv, None), cache.device, "kept")
     _whole(kept_len, torch.int32, (batch.n_seq,), cache.device, "kept_len")
-    if kept.shape[2] < 1:
-        raise ValueError("kept needs room for at least 1 position")
+    if not 1 <= kept.shape[2] <= 1 << 30:  # the library's integers have 32 bits
+        raise ValueError(f"kept has room for {kept.shape[2]} positions (1 to 2^30)")
 
 
 def select(cache: Cache, batch: Batch, mass, kept, kept_len, recent: int = 0, sinks: int = 0):
@@ -474,6 +476,8 @@ def select(cache: Cache, batch: Batch, mass, kept, kept_len, recent: int = 0, si
     _one_gpu(cache, batch)
     _kept(cache, batch, kept, kept_len)
     a = _mass(mass, cache, batch.n_seq, batch.table.shape[1] * cache.block, "mass")
+    if recent < 0 or sinks < 0 or recent + sinks > kept.shape[2]:
+        raise ValueError(f"recent {recent} and sinks {sinks} (at least 0, together at most {kept.shape[2]}, kept's positions)")
     if batch.n_seq:
         _call("megakernel_op_kv8_select", cache.device, cache._ref, batch._ref, a, kept.shape[2], recent, sinks,
               kept.data_ptr(), kept_len.data_ptr())
@@ -493,8 +497,8 @@ def compact(cache: Cache, batch: Batch, kept, kept_len, new_table, mass=None, ne
     _kept(cache, batch, kept, kept_len)
     device = cache.device
     _whole(new_table, torch.int32, (batch.n_seq, None), device, "new_table")
-    if new_table.shape[1] < 1:
-        raise ValueError("new_table needs a width of at least 1")
+    if not 1 <= new_table.shape[1] * cache.block <= 1 << 30:
+        raise ValueError(f"new_table has {new_table.shape[1]} blocks of {cache.block} positions (1 to 2^30 positions)")
     if (mass is None) != (new_mass is None):
         raise ValueError("mass and new_mass go together")
     a = b = None

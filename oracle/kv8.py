@@ -118,3 +118,98 @@ def norm_rope(x, gain, inv_freq, pos, eps: float):
     a = np.asarray(pos, np.float64)[:, None, None] * np.asarray(inv_freq, np.float64)
     c, s = np.cos(a), np.sin(a)
     return np.concatenate([y[..., :h] * c - y[..., h:] * s, y[..., h:] * c + y[..., :h] * s], -1), np.concatenate([np.abs(y[..., :h]) + np.abs(y[..., h:])] * 2, -1)
+
+
+class Scores:
+    """What scores are and what rows see (include/megakernel.h, megakernel_kv8_scores)."""
+
+    def __init__(self, softcap=0.0, slopes=None, window=0, first=None, prefix=None):
+        self.softcap, self.slopes, self.window, self.first, self.prefix = softcap, slopes, window, first, prefix
+
+    def span(self, i: int, t: int, p: int, length: int):
+        """[lo, hi) of row t at position p of sequence i."""
+        lo, hi = 0, p + 1
+        if self.window:
+            lo = max(lo, p + 1 - self.window)
+        if self.first is not None:
+            lo = max(lo, int(self.first[t]))
+        if self.prefix is not None and p >= 0:
+            hi = max(hi, int(self.prefix[i]))
+        return lo, min(hi, length)
+
+
+def scored_rows(pool: Pool, table, start, length, q, scale: float, x: Scores, tokens=None):
+    """Yields (sequence, row, head, positions, scores, weights, values, reach, bias) of
+    every row that sees something, or None for the last six: reach is
+    max_j sum_d |q_d k_jd| * scale and bias the largest |slope * distance|."""
+    group = q.shape[1] // pool.n_kv
+    for i in range(len(length)):
+        n = min(max(0, int(length[i])), len(table[i]) * pool.block)
+        at = [(j, pool.place(table[i], j)) for j in range(n)]
+        there = [(j, *pool.values(*a)) for j, a in at if a]
+        pos = np.array([y[0] for y in there], np.int64)
+        keys, vals = (np.stack([y[k] for y in there]) if there else None for k in (1, 2))
+        for t in range(start[i], start[i + 1]):
+            if tokens is not None and t not in tokens:
+                continue
+            p = int(length[i]) - int(start[i + 1]) + t
+            lo, hi = x.span(i, t, p, n)
+            seen = (pos >= lo) & (pos < hi) if there else np.zeros(0, bool)
+            for h in range(q.shape[1]):
+                if not seen.any():
+                    yield i, t, h, None, None, None, None, 0.0, 0.0
+                    continue
+                k, v, j = keys[seen, h // group], vals[seen, h // group], pos[seen]
+                s = k @ q[t, h] * scale
+                if x.softcap:
+                    s = x.softcap * np.tanh(s / x.softcap)
+                far = np.abs(j - p) * float(x.slopes[h]) if x.slopes is not None else np.zeros(len(j))
+                s = s - far
+                w = np.exp(s - s.max())
+                yield i, t, h, j, s, w / w.sum(), v, (np.abs(k) @ np.abs(q[t, h])).max() * scale, np.abs(far).max()
+
+
+def select(mass, length: int, keep: int, recent: int, sinks: int):
+    """The positions that stay of one sequence and head, in rising order."""
+    if length <= keep:
+        return list(range(length))
+    fixed = list(range(sinks)) + list(range(length - recent, length))
+    rest = range(sinks, length - recent)
+    # by falling weight, NaN last, then by rising position
+    order = sorted(rest, key=lambda j: (math.isnan(mass[j]), -mass[j] if not math.isnan(mass[j]) else 0.0, j))
+    return sorted(fixed + order[: keep - recent - sinks])
+
+
+def compact(pool: Pool, table, kept, kept_len, new_table):
+    """Rows moved to the blocks of new_table: read, then appended to blocks that start anew."""
+    n_seq, _, keep = kept.shape
+    rows = [max(0, min(int(n), keep, len(new_table[i]) * pool.block)) for i, n in enumerate(kept_len)]
+    got = []
+    for i in range(n_seq):
+        k, v = np.zeros((2, rows[i], pool.n_kv, pool.dim))
+        for h in range(pool.n_kv):
+            for r in range(rows[i]):
+                at = pool.place(table[i], int(kept[i, h, r]))
+                if at:
+                    kk, vv = pool.values(*at)
+                    k[r, h], v[r, h] = kk[h], vv[h]
+        got.append((k, v))
+    for i, (k, v) in enumerate(got):
+        pool.append([new_table[i]], [0, rows[i]], [rows[i]], k, v)
+
+
+def rotary(x, inv_freq, pos, interleaved: bool, amplitude: float):
+    """The rotation of the first 2 * len(inv_freq) dimensions; float64 [T][H][D], and |a| + |b| of each value's pair."""
+    x = np.asarray(x, np.float64)
+    n = 2 * len(inv_freq)
+    a, b = (x[..., 0:n:2], x[..., 1:n:2]) if interleaved else (x[..., : n // 2], x[..., n // 2 : n])
+    t = np.asarray(pos, np.float64)[:, None, None] * np.asarray(inv_freq, np.float64)
+    c, s = np.cos(t) * amplitude, np.sin(t) * amplitude
+    y, size = x.copy(), np.abs(x)
+    both = np.abs(a) + np.abs(b)
+    for out, first, second in ((y, a * c - b * s, b * c + a * s), (size, both, both)):
+        if interleaved:
+            out[..., 0:n:2], out[..., 1:n:2] = first, second
+        else:
+            out[..., : n // 2], out[..., n // 2 : n] = first, second
+    return y, size
