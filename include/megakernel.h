@@ -525,7 +525,8 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
  *   hi = p + 1, or prefix[sequence] if that is more (int [n_seq])
  * so `first` is where the row's document begins, `window` how many positions
  * it looks back on, its own among them, and the rows of a prefix see it whole.
- * softcap is 0 or 2^-30 to 2^30.  Positions are those of the cache: after
+ * softcap is 0 or 2^-30 to 1024; capped scores are off by up to 10 * 2^-24 of it.
+ * Positions are those of the cache: after
  * megakernel_op_kv8_compact the places that rows were moved to.  The arrays are
  * read when a call runs, and values beyond a sequence's bounds are cut to them. */
 typedef struct {

@@ -335,8 +335,8 @@ static bool scores_ok(const char* op, const megakernel_kv8_scores* x) {
     set_err("%s: slopes, first and prefix need 4-byte alignment", op);
     return false;
   }
-  if (!(x->softcap == 0.f || (x->softcap >= 0x1p-30f && x->softcap <= 0x1p30f)) || x->window < 0) {
-    set_err("%s: softcap=%g (0, or 2^-30 to 2^30), window=%d (0, or at least 1)", op, x->softcap, x->window);
+  if (!(x->softcap == 0.f || (x->softcap >= 0x1p-30f && x->softcap <= 1024.f)) || x->window < 0) {
+    set_err("%s: softcap=%g (0, or 2^-30 to 1024), window=%d (0, or at least 1)", op, x->softcap, x->window);
     return false;
   }
   return true;
@@ -356,7 +356,7 @@ static float scale_of(const char* op, const megakernel_kv8_scores* x, float scal
   return scale2;
 }
 static Scores scores_of(const megakernel_kv8_scores* x, float scale2) {
-  Scores r{x->slopes, x->first, x->prefix, x->window, x->softcap > 64.f, 0.f, 0.f};
+  Scores r{x->slopes, x->first, x->prefix, x->window, 0.f, 0.f};
   if (x->softcap > 0.f) {
     r.cap = x->softcap * 1.4426950408889634f;
     r.cap_in = 2.f * scale2 / x->softcap;

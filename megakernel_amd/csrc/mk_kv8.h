@@ -574,7 +574,6 @@ struct Scores {
   const int* first;     // [n_tokens], or null
   const int* prefix;    // [n_seq], or null
   int window;           // 0: none
-  int wide;             // the cap is large: tanh of small arguments by its series (see capped())
   float cap, cap_in;    // cap * log2(e) (0: none), 2 log2(e) scale / cap
 };
 // The attention with such scores, or with each row's log-sum-exp.
@@ -656,36 +655,21 @@ struct Bounds {
   }
 };
 
-// Scores to base 2 from q . k, where they are capped: cap * tanh(y) with
-// tanh(y) = 1 - 2 / (e^2y + 1), which is off by 2^-23 of the cap where y is
-// small.  For caps of up to 64 that is what rounding scores of tens costs
-// anyway; for larger ones tanh is its series where |y| is below 1/4 (the first
-// term left out is 2^-26.8 of the value).
-__device__ __forceinline__ float capped(const Scores& x, float s, float top) {  // top: the cap and what is added
-  const float t = __builtin_amdgcn_exp2f(s * x.cap_in);
-  return fmaf(-2.f * x.cap, __builtin_amdgcn_rcpf(t + 1.f), top);
-}
-__device__ __forceinline__ float capped_wide(const Scores& x, float s, float scale, float add) {
-  const float y = s * x.cap_in * 0.34657359027997264f;  // ln(2) / 2
-  const float z = y * y;
-  const float r = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
-  const int tall = opaque_v(__float_as_int(capped(x, s, x.cap + add)));  // both, and no branch for every score
-  return fabsf(y) < 0.25f ? fmaf(s * scale, r, add) : __int_as_float(tall);
-}
-// Scores of one row to base 2, with `add` added, in place: N of them, at(i) is
-// the position of the i-th less that of the row.
+// Scores of one row to base 2 from q . k, with `add` added, in place: N of them,
+// at(i) is the position of the i-th less that of the row.  A capped one is
+// cap * tanh(y) with tanh(y) = 1 - 2 / (e^2y + 1), off by up to 10 * 2^-24 of the
+// cap, which of caps of tens is what rounding scores of tens costs anyway.
 template <int N, class At>
 __device__ __forceinline__ void score(const Scores& x, float scale, float slope, float add, float* s, At at) {
   if (!x.cap) {
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = fmaf(s[i], scale, add);
-  } else if (!x.wide) {
+    asm volatile("");  // branches that stay branches: 64 scores of both kinds at once take registers that are not there
+  } else {
+    asm volatile("");
     const float top = x.cap + add;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = capped(x, s[i], top);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = capped_wide(x, s[i], scale, add);
+    for (int i = 0; i < N; ++i) s[i] = fmaf(-2.f * x.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * x.cap_in) + 1.f), top);
   }
   if (x.slopes) {
 #pragma unroll
@@ -1261,8 +1245,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     return row[min(pos >> lb, top)];
   };
   const auto confirm = [&](int w, int& tab) {  // which of them are there; the others' place is taken by block 0
-    const int pos = first_of(16 * w) + 16 * l;  // nor what no row sees: its block may never have been written
-    const bool ok = pos < end && tab >= 0 && tab < p.c.n_blocks && (!SCORED || pos + 16 > rows.from);
+    const bool ok = first_of(16 * w) + 16 * l < end && tab >= 0 && tab < p.c.n_blocks;
     tab = ok ? tab : 0;
     return __ballot(ok);
   };
@@ -1369,6 +1352,8 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
   if (tid < 2) lds.bad[tid] = 0;
   if (n > 0) {
     tab0 = window(0);
+    // of the first step's runs those that no row sees are as good as missing: their blocks may never have been written
+    if constexpr (SCORED) tab0 = first_of(0) + 16 * l + 16 > rows.from ? tab0 : -1;
     tab1 = window(1);
     ok0 = confirm(0, tab0);
     ok1 = confirm(1, tab1);
@@ -1496,9 +1481,8 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     };
     weights(0);
     if constexpr (SCORED) {
-      // a half's weights beside the other's products (1,024 capped tokens of
-      // head_dim 128 at 16,384 positions 191 us; as below 193, ragged prompts 220
-      // and 234)
+      // a half's weights beside the other's products (16 / 8 heads of 64, four
+      // prompts of 2,048 72 us; in the order below 76)
       half_scores(k + 1, 0);
       add_v(0);
       weights(1);

@@ -221,8 +221,8 @@ class Scores(_Fixed):
         for t, name, dtype in ((slopes, "slopes", torch.float32), (first, "first", torch.int32), (prefix, "prefix", torch.int32)):
             if t is not None:
                 _whole(t, dtype, (None,), device, name)
-        if not (softcap == 0 or 2.0 ** -30 <= softcap <= 2.0 ** 30) or not 0 <= window < 1 << 31:
-            raise ValueError(f"softcap {softcap} (0, or 2^-30 to 2^30), window {window} (0 to 2^31 - 1)")
+        if not (softcap == 0 or 2.0 ** -30 <= softcap <= 1024) or not 0 <= window < 1 << 31:
+            raise ValueError(f"softcap {softcap} (0, or 2^-30 to 1024), window {window} (0 to 2^31 - 1)")
         self.slopes, self.first, self.prefix = slopes, first, prefix
         self.softcap, self.window, self.device = float(softcap), int(window), device
         # an empty tensor has no address, and no row asks for what is in it

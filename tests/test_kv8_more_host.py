@@ -145,7 +145,7 @@ def test_bad_batches(clib, batch, word):  # noqa: F811
 
 BAD_SCORES = [(None, "null scores"), (_x(slopes=FAKE + 2), "alignment"), (_x(first=FAKE + 1), "alignment"), (_x(prefix=FAKE + 3), "alignment"),
               (_x(softcap=-1.0), "softcap=-1"), (_x(softcap=float("nan")), "softcap=nan"), (_x(softcap=float("inf")), "softcap=inf"),
-              (_x(softcap=1e-20), "softcap"), (_x(window=-1), "window=-1")]
+              (_x(softcap=1e-20), "softcap"), (_x(softcap=1025.0), "softcap=1025"), (_x(window=-1), "window=-1")]
 
 
 @pytest.mark.parametrize("x,word", BAD_SCORES)
@@ -172,7 +172,7 @@ def test_other_refusals_of_attention_with_scores(clib):  # noqa: F811
     _refused(clib, att(c, b, x, r, far, FAKE + 2, 8, 1.0, None, 0, None), "lse")
     for scale in (0.0, -1.0, float("inf"), float("nan"), 3e38):
         _refused(clib, att(c, b, x, r, far, None, 8, scale, None, 0, None), "scale")
-    _refused(clib, att(c, b, _ref(_x(softcap=2.0 ** 30)), r, far, None, 8, 1e-35, None, 0, None), "too far from softcap")
+    _refused(clib, att(c, b, _ref(_x(softcap=1024.0)), r, far, None, 8, 1e-37, None, 0, None), "too far from softcap")
     _refused(clib, att(c, b, _ref(_x(softcap=2.0 ** -30)), r, far, None, 8, 1e33, None, 0, None), "too far from softcap")
     long = _ref(_batch(table_width=1024))
     plain, more = (clib.megakernel_op_kv8_scored_workspace_bytes(c, long, x, 8, n) for n in (0, 1))
@@ -279,7 +279,7 @@ def test_python_refuses_host_tensors(monkeypatch):
         kv8.rotary(q, q, torch.zeros(32), torch.zeros(3, **i32), q, q)
 
 
-@pytest.mark.parametrize("kw,word", [(dict(softcap=-1.0), "softcap"), (dict(softcap=math.nan), "softcap"), (dict(softcap=2.0 ** 31), "softcap"),
+@pytest.mark.parametrize("kw,word", [(dict(softcap=-1.0), "softcap"), (dict(softcap=math.nan), "softcap"), (dict(softcap=1025.0), "softcap"),
                                      (dict(window=-1), "window"), (dict(window=2 ** 31), "window"), (dict(window=2 ** 32 + 5), "window")])
 def test_python_refuses_scores(kw, word):
     with pytest.raises(ValueError, match=word):
