@@ -619,13 +619,21 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
   if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
   Weigh p{cache_of(cache), batch_of(batch), rows_of(q), lse, mass_of(mass), n_q, group, scale2, scores_of(scores, scale2)};
   long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all;
-  const bool many = rows > 32ll * batch->n_seq;
-  // Steps of 64 positions: a wave's with few rows, a workgroup's with many, of 32
-  // where those would not be two workgroups for every CU.  More than one step each
-  // where that is more workgroups than run at once.
-  const long long steps = (kv + TILE - 1) / TILE * batch->n_seq;
-  const bool half = many && steps * cache->n_kv < 1024;
+  // Steps of 64 positions: a wave's with few rows, a workgroup's with many.  The
+  // workgroup takes 4 us to start on one, and pays where rows are so many that a
+  // wave would be long at them while others have none (us of weigh_few /
+  // weigh_many, head_dim 64; one sequence of 4,096 positions, 16 tokens 5.7 / 7.4, 32
+  // 7.3 / 7.6, 64 10.4 / 8.3; 16 of 1,024, 64 tokens 12 / 24, 256 about 33 / 36; 16 of
+  // 4,096, 64 tokens 33 / 74; 128: 64 tokens 12.4 / 9.5, 17 / 29, 57 / 95).
+  const long long steps = (kv + TILE - 1) / TILE * batch->n_seq, items = steps * cache->n_kv;
+  const long long most = cache->head_dim == 64 ? 512 : 384, enough = items / 4 < 32 ? 32 : items / 4 > most ? most : items / 4;
+  const bool many = rows > enough * batch->n_seq;
+  // In steps of 32 positions where those of 64 are not two workgroups for every
+  // CU (1,024 tokens in steps of 32 / 64, head_dim 128: at 1,024 positions 13 / 20,
+  // 2,048 21 / 22, 4,096 39 / 34, 8,192 72 / 64).
+  const bool half = many && items < 512;
   long long groups = half ? 2 * steps : many ? steps : (steps + 3) / 4;
+  // more than one step each where that is more workgroups than run at once
   if (groups > 4096 / cache->n_kv) groups = 4096 / cache->n_kv;
   groups = (groups < 1 ? 1 : groups) * cache->n_kv;
   auto go = [&](auto kern, int threads) { return launch(kern, groups, threads, static_cast<hipStream_t>(stream), p); };
@@ -654,6 +662,7 @@ int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel
   Choose p{mass_of(mass), batch->kv_len, kept, kept_len, cache->n_kv, keep, recent, sinks, (int)all};
   const long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all, most = kv - recent - sinks;
   auto go = [&](auto kern) { return launch(kern, groups, 1024, static_cast<hipStream_t>(stream), p); };
+  // so much LDS that two workgroups share a CU, or that 32,768 weights stay in it
   return launched(op, most <= 4096 ? go(choose<4>) : go(choose<32>));
 }
 
@@ -733,7 +742,9 @@ int megakernel_op_rotary(const megakernel_rows* q, const megakernel_rows* k, con
                             : (d32 ? go(rotate_pairs<false, true>, interleaved) : go(rotate_pairs<false, false>, interleaved)));
   }
   const long long units = (long long)n_tokens * (head_dim / 16);
-  const bool many = units * (n_q + n_kv) > 1 << 16;
+  // four heads share a set of sines where that still fills the chip (us with one /
+  // four, 24 heads of 128, bf16: 512 tokens 3.7 / 4.1, 1,024 4.75 / 4.6, 4,096 14.5 / 10.1)
+  const bool many = units * (n_q + n_kv) > 1 << 17;
   groups = (units * (many ? (n_q + n_kv + 3) / 4 : n_q + n_kv) + 255) / 256;
   if (!grid_ok(op, groups)) return -1;
   auto pick = [&](auto il, auto n) {

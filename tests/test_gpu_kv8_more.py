@@ -222,11 +222,12 @@ def test_scores_of_many_rows(case, kind):
 
 
 @pytest.mark.parametrize("kind", ["plain", "documents", "all"])
-@pytest.mark.parametrize("dim,group", [(64, 1), (64, 3), (128, 1), (128, 5)])
-def test_weights_of_many_steps_and_heads(dim, group, kind):
-    """Enough steps times KV heads for workgroups of 64 positions."""
+@pytest.mark.parametrize("dim,group,lens,new", [(64, 1, [560], [170]), (64, 3, [640], [60]), (128, 1, [560], [170]), (128, 5, [700], [40]),
+                                                (64, 2, [260, 70, 300, 0, 33], [70, 40, 41, 0, 33])])
+def test_weights_of_many_steps_and_heads(dim, group, lens, new, kind):
+    """Enough steps times KV heads for workgroups of 64 positions, and in the last case for a wave to each."""
     _say(f"weights of many steps D={dim} group {group} {kind}")
-    c = Case(16, 64, dim, [260, 70, 300, 0, 33], [70, 40, 41, 0, 33], seed=dim + group, missing=0.1, gap=1)
+    c = Case(16, 64, dim, lens, new, seed=dim + group, missing=0.1, gap=1)
     _check(c, 64 * group, _scores_of(kind, c, 64 * group))
 
 
