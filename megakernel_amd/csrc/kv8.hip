@@ -1,5 +1,5 @@
 // Host side of the paged 8-bit KV cache's operators (megakernel_op_qk_norm_rope,
-// megakernel_op_kv8_*): argument checks and launches.  Every call only
+// megakernel_op_rotary, megakernel_op_kv8_*): argument checks and launches.  Every call only
 // enqueues on the caller's stream: no allocation, no copy, no wait, so it can
 // be captured into a graph.  Lengths and block tables stay on the device; the
 // grids come from the row count alone, and each workgroup finds its sequence

@@ -70,7 +70,10 @@ __device__ __forceinline__ int first_token(const Weigh& p, const Step& x) {
 
 // Few rows: a wave holds the K of 64 positions and goes through the query rows,
 // 16 at a time, on v_mfma_f32_16x16x32_bf16 (the positions' layout is that of
-// rows_item()); its weights stay in 16 sums a lane until the end.
+// rows_item()); its weights stay in 16 sums a lane until the end.  Bound by K's way
+// here: one token to each of 16 sequences of 512 to 4,096, head_dim 64 (19 MB of K),
+// takes 8.6 us, of which 2.7 are the launch and the rest three loads in a row;
+// 16 of 4,096, 4 tokens each, 12.4, head_dim 128 22 (67 MB, 3.1 TB/s).
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void weigh_few(Weigh p) {
   constexpr int KH = D / 64;
@@ -147,7 +150,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void weigh_few(Weigh p) {
 // time, and 8 / PS groups that deal the rows.  Sums stay in 16 registers a lane, and
 // meet over lanes and groups, in a fixed order, at the end.
 // 1,024 tokens of 16 / 8 heads of 128 at the end of 16,384 positions take 118 us (one
-// side by side 130), capped 142 (155); 1,024 tokens without a past 21 (14), 26 (16).
+// side by side 130), capped 139 (155); 1,024 tokens without a past 20 (13), 26 (16).
 // What bounds it is q's way from the L2 (a tile for every 1,024 scores) beside the
 // vector unit, which one wave alone can give an operation only every eight cycles:
 // positions are so few that four waves fit a SIMD.
@@ -318,7 +321,8 @@ __device__ __forceinline__ unsigned lanes_below(unsigned long long m) {
 // a digit are in COPIES by lane.  Up to PER * 1,024 candidates stay in LDS, each wave's own; of
 // more every look reads them again.  (In registers every loop over them is
 // straight code of 32 turns, and fetching that took longer than running it:
-// 32,768 candidates 21.8 us.)
+// 8,192 candidates 15.7 us, here 10.)  32,768 candidates take 19 us, 4,096 7.5: a CU's
+// vector units are at them all the time, some 60 operations for every 64.
 template <int PER>
 __global__ __launch_bounds__(1024) void choose(Choose p) {
   constexpr int NW = 16, COPIES = 16, U = 4;
@@ -476,7 +480,10 @@ __device__ __forceinline__ float top4(uint32_t w) {
 // dimensions of one row: lanes are rows there, so a load's bytes lie in as few
 // lines as there are old blocks among the rows (in pieces of 4 rows x 8
 // dimensions every byte was a line of its own).  Four lanes then trade dimensions
-// for rows, which makes the dwords of the new block.
+// for rows, which makes the dwords of the new block.  4,096 rows of 32,768, 8 heads of
+// 128, take 11 us (18 in pieces), 1,000 of each of 16 contexts of 512 to 4,096, heads of
+// 64, 14 (21): four loads in a row (lengths and kept positions, table, scales, codes),
+// and V's bytes one by one.
 template <int D, int T, int PASSES>
 __global__ __launch_bounds__(256) void move(Move p) {
   constexpr int HEADS = 256 / T, CH = D / 16;  // pieces of a K row

@@ -1,11 +1,16 @@
 """Operators of a paged 8-bit KV cache over the library's
-``megakernel_op_qk_norm_rope`` and ``megakernel_op_kv8_*`` entry points.
+``megakernel_op_qk_norm_rope``, ``megakernel_op_rotary`` and
+``megakernel_op_kv8_*`` entry points.
 
 What a server keeps next to the model: a pool of blocks that sequences share
 (:class:`Cache`), the sequences' block tables and lengths (:class:`Batch`),
 and the operators that take one layer from its QKV rows to its attention
-output: :func:`qk_norm_rope`, :func:`append`, :func:`attention`; :func:`read`
-gives rows of the cache back.  The reference has one contiguous bf16 cache
+output: :func:`qk_norm_rope` or :func:`rotary`, :func:`append`,
+:func:`attention`, whose scores may be capped, biased by distance or masked
+(:class:`Scores`); :func:`read` gives rows of the cache back.  A cache that grows
+too long is cut down by what its positions are worth: :func:`weigh` adds up
+the attention weights that each gets, :func:`select` chooses the heaviest, and
+:func:`compact` moves them to blocks of their own.  The reference has one contiguous bf16 cache
 (src/kv_cache.cuh:11-32) and these steps only inside its
 kernel (src/attention.cuh).
 
@@ -22,6 +27,12 @@ tensors that require one are refused.
     kv8.qk_norm_rope(q, k, q_gain, k_gain, inv_freq, pos, q, k)
     kv8.append(cache, batch, k, v)
     kv8.attention(cache, batch, q, out)
+
+    scores = kv8.Scores(softcap=30.0, window=4096)
+    kv8.attention(cache, batch, q, out, scores=scores, lse=lse)
+    kv8.weigh(cache, batch, q, lse, mass, scores=scores)
+    kv8.select(cache, batch, mass, kept, kept_len, recent=256, sinks=4)
+    kv8.compact(cache, batch, kept, kept_len, new_table, mass, new_mass)
 """
 from __future__ import annotations
 
