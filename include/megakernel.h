@@ -563,11 +563,11 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
                             const megakernel_rows* mass, int n_q, float scale, void* stream);
 
 /* The positions that stay of each sequence and KV head: kept [n_seq][n_kv][keep]
- * receives them in rising order, -1 behind the last; kept_len [n_seq] how many
- * there are, min(kv_len, keep).  Of a longer sequence these are its first `sinks`
- * and last `recent` positions and the heaviest of the others; of equal weights the
- * lower position stays, NaN weighs less than anything.  The batch's table_width,
- * kv_len and n_seq count, its rows do not. */
+ * receives them in rising order, -1 behind the last; kept_len [n_seq] (not kv_len
+ * itself) how many there are, min(kv_len, keep).  Of a longer sequence these are
+ * its first `sinks` and last `recent` positions and the heaviest of the others; of
+ * equal weights the lower position stays, NaN weighs less than anything.  The
+ * batch's table_width, kv_len and n_seq count, its rows do not. */
 int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const megakernel_rows* mass,
                              int keep, int recent, int sinks, int* kept, int* kept_len, void* stream);
 

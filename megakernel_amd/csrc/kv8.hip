@@ -656,6 +656,10 @@ int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel
     set_err("%s: null kept or kept_len, or not 4-byte aligned", op);
     return -1;
   }
+  if (kept_len == batch->kv_len) {  // heads would read what others have written
+    set_err("%s: kept_len must not be kv_len", op);
+    return -1;
+  }
   if (batch->n_seq == 0) return 0;
   const long long groups = (long long)batch->n_seq * cache->n_kv;
   if (!grid_ok(op, groups * 4)) return -1;

@@ -480,10 +480,10 @@ def _kept(cache: Cache, batch: Batch, kept, kept_len):
 def select(cache: Cache, batch: Batch, mass, kept, kept_len, recent: int = 0, sinks: int = 0):
     """The positions worth keeping of each sequence and KV head: kept
     [n_seq][n_kv][keep] (int32) receives them in rising order, -1 behind the last,
-    and kept_len [n_seq] (int32) their number, min(kv_len, keep).  Of a longer
-    sequence they are its first ``sinks``, its last ``recent`` and the heaviest of
-    the others by ``mass`` (:func:`weigh`); of equal weights the lower position,
-    and NaN last."""
+    and kept_len [n_seq] (int32, another tensor than the batch's lengths) their
+    number, min(kv_len, keep).  Of a longer sequence they are its first ``sinks``,
+    its last ``recent`` and the heaviest of the others by ``mass`` (:func:`weigh`);
+    of equal weights the lower position, and NaN last."""
     _one_gpu(cache, batch)
     _kept(cache, batch, kept, kept_len)
     a = _mass(mass, cache, batch.n_seq, batch.table.shape[1] * cache.block, "mass")

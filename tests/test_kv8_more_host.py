@@ -127,7 +127,7 @@ def _calls(lib, cache, batch):
     return [lambda: lib.megakernel_op_kv8_scored_workspace_bytes(cache, batch, _ref(_x()), 8, 1),
             lambda: lib.megakernel_op_kv8_attention_scored(cache, batch, _ref(_x()), r, _ref(_r(2 * FAKE)), None, 8, 1.0, None, 0, None),
             lambda: lib.megakernel_op_kv8_weigh(cache, batch, _ref(_x()), r, FAKE, m, 8, 1.0, None),
-            lambda: lib.megakernel_op_kv8_select(cache, batch, m, 4, 0, 0, FAKE, FAKE, None),
+            lambda: lib.megakernel_op_kv8_select(cache, batch, m, 4, 0, 0, FAKE, 2 * FAKE, None),
             lambda: lib.megakernel_op_kv8_compact(cache, batch, FAKE, FAKE, 4, 2 * FAKE, 4, None, None, None)]
 
 
@@ -202,11 +202,12 @@ def test_refusals_of_select(clib):  # noqa: F811
     c, b, m = _ref(_cache()), _ref(_batch()), _ref(_mass())
     sel = clib.megakernel_op_kv8_select
     for mass, word in BAD_MASSES:
-        _refused(clib, sel(c, b, _ref(mass), 4, 0, 0, FAKE, FAKE, None), word)
+        _refused(clib, sel(c, b, _ref(mass), 4, 0, 0, FAKE, 2 * FAKE, None), word)
     for keep, recent, sinks in ((0, 0, 0), (-1, 0, 0), (4, -1, 0), (4, 0, -1), (4, 3, 2), (4, 2 ** 31 - 1, 2 ** 31 - 1), (2 ** 30 + 1, 0, 0)):
         _refused(clib, sel(c, b, m, keep, recent, sinks, FAKE, FAKE, None), f"keep={keep}")
     for kept, lens in ((None, FAKE), (FAKE, None), (FAKE + 2, FAKE), (FAKE, FAKE + 1)):
         _refused(clib, sel(c, b, m, 4, 0, 0, kept, lens, None), "kept")
+    _refused(clib, sel(c, b, m, 4, 0, 0, 2 * FAKE, FAKE, None), "must not be kv_len")
 
 
 def test_refusals_of_compact(clib):  # noqa: F811
@@ -259,7 +260,7 @@ def test_empty_calls_do_nothing(clib):  # noqa: F811
         assert clib.megakernel_op_kv8_attention_scored(c, b, x, r, far, FAKE, 8, 1.0, None, 0, None) == 0
         assert clib.megakernel_op_kv8_weigh(c, b, x, r, FAKE, m, 8, 1.0, None) == 0
     none = _ref(_batch(n_seq=0))
-    assert clib.megakernel_op_kv8_select(c, none, m, 4, 0, 0, FAKE, FAKE, None) == 0
+    assert clib.megakernel_op_kv8_select(c, none, m, 4, 0, 0, FAKE, 2 * FAKE, None) == 0
     assert clib.megakernel_op_kv8_compact(c, none, FAKE, FAKE, 4, 2 * FAKE, 4, None, None, None) == 0
     assert clib.megakernel_op_rotary(r, r, FAKE, FAKE, far, _ref(_r(3 * FAKE)), 0, 8, 8, 64, 32, 1, 1.0, None) == 0
 
