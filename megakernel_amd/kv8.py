@@ -304,16 +304,17 @@ def rotary(q, k, inv_freq, pos, q_out, k_out, interleaved: bool = False, amplitu
     tokens, n_q, dim = q.shape
     n_kv = k.shape[1]
     _whole(pos, torch.int32, (tokens,), device, "pos")
-    _whole(inv_freq, torch.float32, (None,), device, "inv_freq")
-    if not 1 <= inv_freq.shape[0] <= dim // 2 or dim % 2:
-        raise ValueError(f"inv_freq turns {2 * inv_freq.shape[0]} dimensions of heads of {dim} (2 to all, and heads even)")
+    pairs = inv_freq.numel()
+    _whole(inv_freq, torch.float32, (pairs,), device, "inv_freq")
+    if not 1 <= pairs <= dim // 2 or dim % 2:
+        raise ValueError(f"inv_freq turns {2 * pairs} dimensions of heads of {dim} (2 to all, and heads even)")
     qs, ks = (tokens, n_q, dim), (tokens, n_kv, dim)
     rows = (_rows(q, qs, device, "q"), _rows(k, ks, device, "k"), _rows(q_out, qs, device, "q_out"),
             _rows(k_out, ks, device, "k_out"))
     if tokens == 0:
         return
     _call("megakernel_op_rotary", device, rows[0], rows[1], inv_freq.data_ptr(), pos.data_ptr(), rows[2], rows[3], tokens,
-          n_q, n_kv, dim, 2 * inv_freq.shape[0], bool(interleaved), amplitude)
+          n_q, n_kv, dim, 2 * pairs, bool(interleaved), amplitude)
 
 
 def rotary_frequencies(dims: int, theta: float = 1e6, scaling: str | None = None, factor: float = 1.0, original: int = 0,
@@ -471,7 +472,7 @@ def weigh(cache: Cache, batch: Batch, q, lse, mass, scale: float | None = None, 
 
 
 def _kept(cache: Cache, batch: Batch, kept, kept_len):
-    _whole(kept, torch.int32, (batch.n_seq, cache.n_kv, None), cache.device, "kept")
+    _whole(kept, torch.int32, (batch.n_seq, cache.n_kv, kept.shape[-1] if kept.dim() else None), cache.device, "kept")
     _whole(kept_len, torch.int32, (batch.n_seq,), cache.device, "kept_len")
     if not 1 <= kept.shape[2] <= 1 << 30:  # the library's integers have 32 bits
         raise ValueError(f"kept has room for {kept.shape[2]} positions (1 to 2^30)")
@@ -507,7 +508,7 @@ def compact(cache: Cache, batch: Batch, kept, kept_len, new_table, mass=None, ne
     _one_gpu(cache, batch)
     _kept(cache, batch, kept, kept_len)
     device = cache.device
-    _whole(new_table, torch.int32, (batch.n_seq, None), device, "new_table")
+    _whole(new_table, torch.int32, (batch.n_seq, new_table.shape[-1] if new_table.dim() else None), device, "new_table")
     if not 1 <= new_table.shape[1] * cache.block <= 1 << 30:
         raise ValueError(f"new_table has {new_table.shape[1]} blocks of {cache.block} positions (1 to 2^30 positions)")
     if (mass is None) != (new_mass is None):
