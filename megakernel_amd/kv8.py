@@ -327,8 +327,13 @@ def rotary_frequencies(dims: int, theta: float = 1e6, scaling: str | None = None
                   fastest pair as it is and divides the slowest by the factor;
     ``"parts"``   pairs that turn more than ``fast`` times within the
                   ``original`` context as they are, those that turn less than
-                  ``slow`` times divided by the factor, a ramp over the turns
-                  between; the amplitude is 0.1 ln(factor) + 1.
+                  ``slow`` times divided by the factor, and from the last of the
+                  first to the first of the last by equal steps from pair to
+                  pair (what Qwen3 and other models are published with for long
+                  contexts); the amplitude is 0.1 ln(factor) + 1;
+    ``"turns"``   the same with a ramp that is linear in the turns.  Models with
+                  this ramp differ in ``fast`` (32 or 4), and some have no
+                  amplitude: pass 1.0 to :func:`rotary` for those.
 
     Computed in double precision, rounded once to float32."""
     if dims < 2 or dims % 2:
@@ -341,14 +346,23 @@ def rotary_frequencies(dims: int, theta: float = 1e6, scaling: str | None = None
     inv = [theta ** (-2.0 * i / dims) for i in range(dims // 2)]
     if scaling == "linear":
         inv = [f / factor for f in inv]
-    elif scaling == "parts":
-        if original < 1 or not fast > slow > 0:
+    elif scaling in ("parts", "turns"):
+        if original < 1 or not math.inf > fast > slow > 0:
             raise ValueError(f"original {original} (at least 1), fast {fast} and slow {slow} (fast above slow above 0)")
-        stay = [min(max((original * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0) for f in inv]
+        if scaling == "turns":
+            stay = [min(max((original * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0) for f in inv]
+        else:
+            if theta <= 1:
+                raise ValueError(f"theta {theta} (above 1, or no pair is slower than another)")
+            # pair i turns original * theta^(-2i / dims) / 2 pi times: which i has so many turns
+            at = [dims * math.log(original / (2 * math.pi * turns)) / (2 * math.log(theta)) for turns in (fast, slow)]
+            first = min(max(math.floor(at[0]), 0), dims - 1)
+            last = max(min(math.ceil(at[1]), dims - 1), first + 1e-3)  # apart, or there is no ramp
+            stay = [1 - min(max((i - first) / (last - first), 0.0), 1.0) for i in range(dims // 2)]
         inv = [f * s + f / factor * (1 - s) for f, s in zip(inv, stay)]
         amplitude = 0.1 * math.log(factor) + 1
     elif scaling not in (None, "base"):
-        raise ValueError(f"scaling {scaling!r} (None, 'linear', 'base' or 'parts')")
+        raise ValueError(f"scaling {scaling!r} (None, 'linear', 'base', 'parts' or 'turns')")
     return torch.tensor(inv, dtype=torch.float64).to(torch.float32).to(device), amplitude
 
 

@@ -1,0 +1,61 @@
+"""Calls of the paged 8-bit KV cache's operators on the CPU: frequencies for
+long contexts against their definition, and what is refused before any GPU work
+(the addresses below are never dereferenced)."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from megakernel_amd import kv8
+
+
+# ------------------------------------------------------------- frequencies
+def _turns(dims, theta, original):
+    """How often each pair turns within the original context."""
+    return original * theta ** (-2.0 * np.arange(dims // 2) / dims) / (2 * math.pi)
+
+
+@pytest.mark.parametrize("dims,theta,factor,original,fast,slow", [
+    (128, 1e6, 4.0, 32768, 32.0, 1.0), (128, 1e6, 4.0, 8192, 32.0, 1.0), (64, 1e4, 4.0, 2048, 32.0, 1.0), (64, 5e5, 8.0, 8192, 16.0, 2.0),
+    (32, 1e4, 2.0, 512, 32.0, 1.0), (16, 10.0, 2.0, 64, 32.0, 1.0), (2, 1e4, 4.0, 4096, 32.0, 1.0), (64, 1e4, 1.0, 2048, 32.0, 1.0),
+    (64, 1e4, 4.0, 2, 32.0, 1.0), (8, 1e4, 4.0, 10 ** 9, 32.0, 1.0)])
+def test_parts_ramp_over_the_pairs(dims, theta, factor, original, fast, slow):
+    """Between the last whole pair that turns more than `fast` times and the first
+    that turns less than `slow` times the share falls by equal steps from pair to
+    pair; the ends are found here by counting pairs, not by a logarithm."""
+    got, amplitude = kv8.rotary_frequencies(dims, theta, "parts", factor, original=original, fast=fast, slow=slow, device="cpu")
+    assert amplitude == 0.1 * math.log(factor) + 1
+    # pairs beyond the last one go on with the same frequencies, down to dims - 1
+    turns = original * theta ** (-2.0 * np.arange(0, 4 * dims) / dims) / (2 * math.pi)
+    first = max(int((turns >= fast).sum()) - 1, 0)  # the last pair that is at least as fast
+    last = min(int((turns > slow).sum()), dims - 1)
+    plain = theta ** (-2.0 * np.arange(dims // 2) / dims)
+    share = np.clip((np.arange(dims // 2) - first) / max(last - first, 1e-3), 0, 1)
+    want = plain * (1 - share) + plain / factor * share
+    np.testing.assert_allclose(got.double().numpy(), want, rtol=2.0 ** -23)
+
+
+def test_turns_ramp_over_the_turns():
+    dims, theta, factor, original = 64, 1e4, 4.0, 2048
+    got, amplitude = kv8.rotary_frequencies(dims, theta, "turns", factor, original=original, fast=8.0, slow=2.0, device="cpu")
+    assert amplitude == 0.1 * math.log(factor) + 1
+    plain = theta ** (-2.0 * np.arange(dims // 2) / dims)
+    stay = np.clip((_turns(dims, theta, original) - 2.0) / 6.0, 0, 1)
+    np.testing.assert_allclose(got.double().numpy(), plain * stay + plain / factor * (1 - stay), rtol=2.0 ** -23)
+
+
+@pytest.mark.parametrize("scaling", ["parts", "turns"])
+@pytest.mark.parametrize("kw,word", [(dict(original=0), "original 0"), (dict(original=100, fast=1.0, slow=1.0), "fast 1.0"),
+                                     (dict(original=100, slow=0.0), "slow 0.0"),
+                                     (dict(original=100, fast=math.inf), "fast inf"), (dict(original=100, fast=math.nan), "fast nan")])
+def test_ramps_that_are_refused(scaling, kw, word):
+    with pytest.raises(ValueError, match=word):
+        kv8.rotary_frequencies(64, scaling=scaling, factor=2.0, device="cpu", **kw)
+
+
+def test_parts_need_pairs_of_different_speeds():
+    for theta in (1.0, 0.5):
+        with pytest.raises(ValueError, match=f"theta {theta}"):
+            kv8.rotary_frequencies(64, theta, "parts", 2.0, original=100, device="cpu")
