@@ -39,6 +39,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import sys
 
 import torch
 from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device
@@ -340,8 +341,15 @@ def rotary_frequencies(dims: int, theta: float = 1e6, scaling: str | None = None
         raise ValueError(f"dims {dims} must be even and at least 2")
     if not (theta > 0 and math.isfinite(theta) and factor >= 1 and math.isfinite(factor)):
         raise ValueError(f"theta {theta} (above 0), factor {factor} (at least 1)")
+    if scaling is None and factor != 1:
+        raise ValueError(f"factor {factor} needs a scaling ('linear', 'base', 'parts' or 'turns')")
     amplitude = 1.0
-    if scaling == "base" and dims > 2:
+    if scaling == "base" and factor != 1:
+        if dims == 2:
+            raise ValueError("dims 2: the base of a single pair scales nothing")
+        growth = math.log(factor) * dims / (dims - 2)
+        if growth + max(math.log(theta), 0.0) >= math.log(sys.float_info.max):
+            raise ValueError(f"theta {theta} times a power of factor {factor} is not finite")
         theta *= factor ** (dims / (dims - 2))
     inv = [theta ** (-2.0 * i / dims) for i in range(dims // 2)]
     if scaling == "linear":

@@ -59,3 +59,20 @@ def test_parts_need_pairs_of_different_speeds():
     for theta in (1.0, 0.5):
         with pytest.raises(ValueError, match=f"theta {theta}"):
             kv8.rotary_frequencies(64, theta, "parts", 2.0, original=100, device="cpu")
+
+
+@pytest.mark.parametrize("dims,theta,scaling,factor,word", [
+    (64, 1e4, None, 4.0, "factor 4.0 needs a scaling"), (2, 1e4, "base", 4.0, "dims 2"), (64, 1e4, "base", 1e308, "theta 10000.0"),
+    (64, 1e300, "base", 1e10, "theta 1e[+]300"), (4, 1e4, "base", 1e160, "theta 10000.0"),
+    (4, 1e-5, "base", 1e155, "theta 1e-05")])
+def test_factors_that_would_be_lost(dims, theta, scaling, factor, word):
+    with pytest.raises(ValueError, match=word):
+        kv8.rotary_frequencies(dims, theta, scaling, factor, device="cpu")
+
+
+def test_a_factor_of_one_changes_nothing():
+    plain, _ = kv8.rotary_frequencies(64, 1e4, device="cpu")
+    for scaling in (None, "linear", "base", "parts", "turns"):
+        got, amplitude = kv8.rotary_frequencies(64, 1e4, scaling, 1.0, original=2048, device="cpu")
+        assert got.equal(plain) and amplitude == 1.0
+    assert kv8.rotary_frequencies(2, 1e4, "base", 1.0, device="cpu")[0].tolist() == [1.0]
