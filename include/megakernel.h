@@ -432,7 +432,9 @@ float megakernel_op_last_ms(void);
 /* Rows of heads: element d of head h of token t at p[t * token_stride +
  * h * head_stride + d], strides in elements.  Rows start at multiples of 16
  * bytes.  Rows that are written may not overlap each other, nor what a call
- * reads, but for an output of the norms that is its own input. */
+ * reads, but for an output of the norms or of the rotation that is its own
+ * input, start, type and strides alike.  Tensors of one call that lie on each
+ * other are refused where both are dense or have the same strides. */
 typedef struct {
   void* p;
   long long token_stride, head_stride;
@@ -563,8 +565,8 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
                             const megakernel_rows* mass, int n_q, float scale, void* stream);
 
 /* The positions that stay of each sequence and KV head: kept [n_seq][n_kv][keep]
- * receives them in rising order, -1 behind the last; kept_len [n_seq] (not kv_len
- * itself) how many there are, min(kv_len, keep).  Of a longer sequence these are
+ * receives them in rising order, -1 behind the last; kept_len [n_seq] (not on kv_len)
+ * how many there are, min(kv_len, keep).  Of a longer sequence these are
  * its first `sinks` and last `recent` positions and the heaviest of the others; of
  * equal weights the lower position stays, NaN weighs less than anything.  The
  * batch's table_width, kv_len and n_seq count, its rows do not. */

@@ -13,6 +13,7 @@
 
 #include "megakernel.h"
 #include "mk_host.h"
+#include "mk_overlap.h"
 
 namespace mk {
 namespace kv8 {
@@ -59,30 +60,39 @@ static bool apart(const char* op, const char* name, const megakernel_rows* r, in
   return true;
 }
 
-// Two tensors, one of them written, that cannot be the same.
-static bool two(const char* op, const char* names, const megakernel_rows* a, const megakernel_rows* b) {
-  if (a->p != b->p) return true;
-  set_err("%s: %s must not be the same rows", op, names);
+static Span span_of(const megakernel_rows* r, long long tokens, int heads, long long head_dim) {
+  const int sz = type_size(r->type);
+  return Span{(uintptr_t)r->p, tokens, heads, r->token_stride * sz, r->head_stride * sz, head_dim * sz};
+}
+static Span span_of(const void* words, long long n) { return Span{(uintptr_t)words, 1, 1, 0, 0, 4 * n}; }  // int or fp32
+
+// Two tensors, one of them written, that cannot be the same or lie on each other.
+static bool two(const char* op, const char* names, const Span& a, const Span& b) {
+  if (a.p != b.p && !overlap(a, b)) return true;
+  set_err("%s: %s must not be the same rows, or lie on each other", op, names);
   return false;
 }
 
 // Queries and keys that are turned: one type in and one out, and outputs in
 // place of inputs only where a lane writes what it alone has read.
-static bool same_types(const char* op, const megakernel_rows* q, const megakernel_rows* k, const megakernel_rows* q_out,
-                       const megakernel_rows* k_out) {
+static bool turned_ok(const char* op, const megakernel_rows* q, const megakernel_rows* k, const megakernel_rows* q_out,
+                      const megakernel_rows* k_out, int n_tokens, int n_q, int n_kv, int head_dim) {
   if (q->type != k->type || q_out->type != k_out->type) {
     set_err("%s: q and k must have one type (%d, %d), and so must q_out and k_out (%d, %d)", op, q->type, k->type,
             q_out->type, k_out->type);
     return false;
   }
-  auto moved = [](const megakernel_rows* a, const megakernel_rows* b) {
-    return a->p == b->p && (a->type != b->type || a->token_stride != b->token_stride || a->head_stride != b->head_stride);
+  const Span sq = span_of(q, n_tokens, n_q, head_dim), sk = span_of(k, n_tokens, n_kv, head_dim);
+  const Span dq = span_of(q_out, n_tokens, n_q, head_dim), dk = span_of(k_out, n_tokens, n_kv, head_dim);
+  auto moved = [](const megakernel_rows* a, const megakernel_rows* b, const Span& x, const Span& y) {
+    if (a->p != b->p) return overlap(x, y);
+    return a->type != b->type || a->token_stride != b->token_stride || a->head_stride != b->head_stride;
   };
-  if (moved(q, q_out) || moved(k, k_out)) {
-    set_err("%s: an output in place of its input needs the same type and strides", op);
+  if (moved(q, q_out, sq, dq) || moved(k, k_out, sk, dk)) {
+    set_err("%s: an output in place of its input needs the same start, type and strides", op);
     return false;
   }
-  return true;
+  return n_tokens == 0 || (two(op, "q_out and k_out", dq, dk) && two(op, "q_out and k", dq, sk) && two(op, "k_out and q", dk, sq));
 }
 
 static bool cache_ok(const char* op, const megakernel_kv8_cache* c) {
@@ -395,6 +405,10 @@ static int attend(const char* op, const megakernel_kv8_cache* cache, const megak
     return -1;
   }
   if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
+  const Span sq = span_of(q, batch->n_tokens, n_q, cache->head_dim), so = span_of(out, batch->n_tokens, n_q, cache->head_dim);
+  const Span sl = span_of(lse, (long long)batch->n_tokens * n_q);
+  if (!two(op, "out and q", so, sq)) return -1;
+  if (LSE && (!two(op, "lse and q", sl, sq) || !two(op, "lse and out", sl, so))) return -1;
   P p;
   p.c = cache_of(cache);
   p.b = batch_of(batch);
@@ -498,9 +512,8 @@ int megakernel_op_qk_norm_rope(const megakernel_rows* q, const megakernel_rows* 
     set_err("%s: null or unaligned gains (16 bytes), inv_freq or pos (4)", op);
     return -1;
   }
-  if (!same_types(op, q, k, q_out, k_out)) return -1;
+  if (!turned_ok(op, q, k, q_out, k_out, n_tokens, n_q, n_kv, head_dim)) return -1;
   if (n_tokens == 0) return 0;
-  if (!two(op, "q_out and k_out", q_out, k_out) || !two(op, "q_out and k", q_out, k) || !two(op, "k_out and q", k_out, q)) return -1;
   const int hpw = 1024 / head_dim;
   const long long waves = (long long)n_tokens * ((n_q + n_kv + hpw - 1) / hpw), groups = (waves + 3) / 4;
   if (!grid_ok(op, groups)) return -1;
@@ -557,7 +570,8 @@ int megakernel_op_kv8_read(const megakernel_kv8_cache* cache, const megakernel_k
   while (heads < cache->n_kv && items * cache->n_kv > 2048ll * heads) heads *= 2;
   const long long groups = items * ((cache->n_kv + heads - 1) / heads);
   if (groups == 0) return 0;
-  if (!two(op, "k_out and v_out", k_out, v_out) || !grid_ok(op, groups)) return -1;
+  const Span sk = span_of(k_out, batch->n_tokens, cache->n_kv, cache->head_dim);
+  if (!two(op, "k_out and v_out", sk, span_of(v_out, batch->n_tokens, cache->n_kv, cache->head_dim)) || !grid_ok(op, groups)) return -1;
   auto go = [&](auto kern) {
     return launch(kern, groups, 256, static_cast<hipStream_t>(stream), cache_of(cache), batch_of(batch), rows_of(k_out),
                   rows_of(v_out), heads);
@@ -617,6 +631,10 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
   const float scale2 = scale_of(op, scores, scale);
   if (!scale2) return -1;
   if (batch->n_tokens == 0 || batch->n_seq == 0) return 0;
+  const Span sm = span_of(mass, batch->n_seq, cache->n_kv, all);
+  if (!two(op, "mass and lse", sm, span_of(lse, (long long)batch->n_tokens * n_q)) ||
+      !two(op, "mass and q", sm, span_of(q, batch->n_tokens, n_q, cache->head_dim)))
+    return -1;
   Weigh p{cache_of(cache), batch_of(batch), rows_of(q), lse, mass_of(mass), n_q, group, scale2, scores_of(scores, scale2)};
   long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all;
   // Steps of 64 positions: a wave's with few rows, a workgroup's with many.  The
@@ -656,11 +674,16 @@ int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel
     set_err("%s: null kept or kept_len, or not 4-byte aligned", op);
     return -1;
   }
-  if (kept_len == batch->kv_len) {  // heads would read what others have written
-    set_err("%s: kept_len must not be kv_len", op);
+  const Span sl = span_of(kept_len, batch->n_seq), sk = span_of(kept, (long long)batch->n_seq * cache->n_kv * keep);
+  const Span from = span_of(batch->kv_len, batch->n_seq), sm = span_of(mass, batch->n_seq, cache->n_kv, all);
+  if (kept_len == batch->kv_len || overlap(sl, from)) {  // heads would read what others have written
+    set_err("%s: kept_len must not be kv_len, or lie on it", op);
     return -1;
   }
   if (batch->n_seq == 0) return 0;
+  if (!two(op, "kept and kv_len", sk, from) || !two(op, "kept and kept_len", sk, sl) || !two(op, "kept and mass", sk, sm) ||
+      !two(op, "kept_len and mass", sl, sm))
+    return -1;
   const long long groups = (long long)batch->n_seq * cache->n_kv;
   if (!grid_ok(op, groups * 4)) return -1;
   Choose p{mass_of(mass), batch->kv_len, kept, kept_len, cache->n_kv, keep, recent, sinks, (int)all};
@@ -685,8 +708,9 @@ int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakerne
             new_width, cache->block);
     return -1;
   }
-  if (new_table == batch->table) {
-    set_err("%s: new_table must not be the batch's table", op);
+  const Span fresh = span_of(new_table, (long long)batch->n_seq * new_width);
+  if (new_table == batch->table || overlap(fresh, span_of(batch->table, (long long)batch->n_seq * batch->table_width))) {
+    set_err("%s: new_table must not be the batch's table, or lie on it: rows would go where others are read", op);
     return -1;
   }
   if (!mass != !new_mass) {
@@ -694,8 +718,15 @@ int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakerne
     return -1;
   }
   if (mass && (!mass_ok(op, "mass", mass, batch->n_seq, cache->n_kv, all) ||
-               !mass_ok(op, "new_mass", new_mass, batch->n_seq, cache->n_kv, room) || !two(op, "mass and new_mass", mass, new_mass)))
+               !mass_ok(op, "new_mass", new_mass, batch->n_seq, cache->n_kv, room)))
     return -1;
+  if (mass) {
+    const Span to = span_of(new_mass, batch->n_seq, cache->n_kv, room);
+    if (!two(op, "mass and new_mass", span_of(mass, batch->n_seq, cache->n_kv, all), to) || !two(op, "new_mass and new_table", to, fresh) ||
+        !two(op, "new_mass and kept", to, span_of(kept, (long long)batch->n_seq * cache->n_kv * keep)) ||
+        !two(op, "new_mass and kept_len", to, span_of(kept_len, batch->n_seq)))
+      return -1;
+  }
   if (batch->n_seq == 0) return 0;
   const int pieces = cache->block * cache->head_dim / 16, heads = pieces < 256 ? 256 / pieces : 1;
   const long long per = ((long long)keep + cache->block - 1) / cache->block;
@@ -731,9 +762,8 @@ int megakernel_op_rotary(const megakernel_rows* q, const megakernel_rows* k, con
     set_err("%s: null or unaligned inv_freq or pos (4 bytes)", op);
     return -1;
   }
-  if (!same_types(op, q, k, q_out, k_out)) return -1;
+  if (!turned_ok(op, q, k, q_out, k_out, n_tokens, n_q, n_kv, head_dim)) return -1;
   if (n_tokens == 0) return 0;
-  if (!two(op, "q_out and k_out", q_out, k_out) || !two(op, "q_out and k", q_out, k) || !two(op, "k_out and q", k_out, q)) return -1;
   const Turn p{rows_of(q), rows_of(k), rows_of(q_out), rows_of(k_out), inv_freq, pos, n_tokens, n_q, n_kv, head_dim, turned, amplitude};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const bool s32 = q->type == MK_TYPE_F32, d32 = q_out->type == MK_TYPE_F32;

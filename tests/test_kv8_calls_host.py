@@ -9,6 +9,8 @@ import numpy as np
 import pytest
 
 from megakernel_amd import kv8
+from tests.test_kv8_host import FAKE, _batch, _cache, _r, _ref, _refused, clib  # noqa: F401
+from tests.test_kv8_more_host import _mass, _x
 
 
 # ------------------------------------------------------------- frequencies
@@ -76,3 +78,61 @@ def test_a_factor_of_one_changes_nothing():
         got, amplitude = kv8.rotary_frequencies(64, 1e4, scaling, 1.0, original=2048, device="cpu")
         assert got.equal(plain) and amplitude == 1.0
     assert kv8.rotary_frequencies(2, 1e4, "base", 1.0, device="cpu")[0].tolist() == [1.0]
+
+
+# --------------------------------------------------- tensors on each other
+# n_seq 2, 8 heads of 64, 5 tokens, table 4 blocks of 32; a view that starts
+# further on is not the same tensor, but lies on it
+def test_select_refuses_outputs_on_its_inputs(clib):  # noqa: F811
+    c, b, m = _ref(_cache()), _ref(_batch()), _ref(_mass())
+    sel = clib.megakernel_op_kv8_select
+    for off in (-4, 4):
+        _refused(clib, sel(c, b, m, 4, 0, 0, 2 * FAKE, FAKE + off, None), "kept_len must not be kv_len")
+        _refused(clib, sel(c, b, m, 4, 0, 0, 2 * FAKE, 2 * FAKE + 4 * 64 - 4, None), "kept and kept_len")
+        _refused(clib, sel(c, b, m, 4, 0, 0, FAKE + off, 2 * FAKE, None), "kept and kv_len")
+    _refused(clib, sel(c, b, m, 4, 0, 0, 4 * FAKE + 64, 2 * FAKE, None), "kept and mass")
+    _refused(clib, sel(c, b, m, 4, 0, 0, 2 * FAKE, 4 * FAKE + 4 * 2047, None), "kept_len and mass")
+
+
+def test_compact_refuses_new_tensors_on_old_ones(clib):  # noqa: F811
+    c, b, m = _ref(_cache()), _ref(_batch()), _ref(_mass())
+    com = clib.megakernel_op_kv8_compact
+    for off in (-28, -4, 4, 28):
+        _refused(clib, com(c, b, FAKE, FAKE, 4, FAKE + off, 4, None, None, None), "batch's table")
+    for off in (-4, 4, 512 * 8 - 4):
+        _refused(clib, com(c, b, FAKE, FAKE, 4, 2 * FAKE, 4, m, _ref(_mass(4 * FAKE + off)), None), "mass and new_mass")
+    new = _ref(_mass(8 * FAKE))
+    _refused(clib, com(c, b, FAKE, FAKE, 4, 8 * FAKE + 16, 4, m, new, None), "new_mass and new_table")
+    _refused(clib, com(c, b, 8 * FAKE + 16, FAKE, 4, 2 * FAKE, 4, m, new, None), "new_mass and kept")
+    _refused(clib, com(c, b, FAKE, 8 * FAKE, 4, 2 * FAKE, 4, m, new, None), "new_mass and kept_len")
+
+
+@pytest.mark.parametrize("name", ["rotary", "qk_norm_rope"])
+def test_turned_rows_may_lie_on_their_own_inputs_alone(clib, name):  # noqa: F811
+    def call(q, k, qo, ko, tokens=5):
+        a = [_ref(_r(p)) for p in (q, k, qo, ko)]
+        if name == "rotary":
+            return clib.megakernel_op_rotary(a[0], a[1], FAKE, FAKE, a[2], a[3], tokens, 8, 8, 64, 64, 0, 1.0, None)
+        return clib.megakernel_op_qk_norm_rope(a[0], a[1], FAKE, FAKE, FAKE, FAKE, a[2], a[3], tokens, 8, 8, 64, 1e-6, None)
+
+    q, k, qo, ko = FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE
+    for off in (-1024, -64, 16, 128, 4096):
+        _refused(clib, call(q, k, q + off, ko), "in place")
+        _refused(clib, call(q, k, qo, k + off), "in place")
+        _refused(clib, call(q, k, k + off, ko), "q_out and k")
+        _refused(clib, call(q, k, qo, q + off), "k_out and q")
+        _refused(clib, call(q, k, qo, qo + off), "q_out and k_out")
+    assert call(q, k, q + 16, ko, tokens=0) == 0
+
+
+def test_attention_read_and_weigh_refuse_outputs_on_other_tensors(clib):  # noqa: F811
+    c, b, x = _ref(_cache()), _ref(_batch()), _ref(_x())
+    att = clib.megakernel_op_kv8_attention_scored
+    for off in (-5104, 16, 1024, 5104):  # the last row's last, and first, 16 bytes
+        _refused(clib, clib.megakernel_op_kv8_attention(c, b, _ref(_r()), _ref(_r(FAKE + off)), 8, 1.0, None, 0, None), "out and q")
+        _refused(clib, clib.megakernel_op_kv8_read(c, b, _ref(_r()), _ref(_r(FAKE + off)), None), "k_out and v_out")
+    _refused(clib, att(c, b, x, _ref(_r()), _ref(_r(2 * FAKE)), FAKE + 5116, 8, 1.0, None, 0, None), "lse and q")
+    _refused(clib, att(c, b, x, _ref(_r()), _ref(_r(2 * FAKE)), 2 * FAKE - 156, 8, 1.0, None, 0, None), "lse and out")
+    w = clib.megakernel_op_kv8_weigh
+    _refused(clib, w(c, b, x, _ref(_r()), 4 * FAKE + 64, _ref(_mass()), 8, 1.0, None), "mass and lse")
+    _refused(clib, w(c, b, x, _ref(_r(4 * FAKE + 64)), FAKE, _ref(_mass()), 8, 1.0, None), "mass and q")
