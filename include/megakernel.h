@@ -521,13 +521,16 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
 /* What scores are beyond scale * q . k, and which positions a row sees beyond
  * the causal ones.  For the row at position p and a position j:
  *   s = softcap * tanh(scale * q . k / softcap)   (softcap 0: scale * q . k)
- *       - slopes[query head] * |p - j|            (fp32 [n_q], finite; NULL: none)
+ *       - slopes[query head] * |p - j|            (fp32 [n_q]; NULL: none; beyond
+ *                                                  +-2^94 they count as that)
  * seen if lo <= j < hi, with
  *   lo = max(0, first[row], p + 1 - window)       (int [n_tokens]; window 0: none)
  *   hi = p + 1, or prefix[sequence] if that is more (int [n_seq])
  * so `first` is where the row's document begins, `window` how many positions
  * it looks back on, its own among them, and the rows of a prefix see it whole.
  * softcap is 0 or 2^-30 to 1024; capped scores are off by up to 10 * 2^-24 of it.
+ * With slopes scores and log-sum-exps are off by up to 2^-13 of the slope (or, where
+ * blocks before a position are missing, 2^-22 of the bias across them).
  * Positions are those of the cache: after
  * megakernel_op_kv8_compact the places that rows were moved to.  The arrays are
  * read when a call runs, and values beyond a sequence's bounds are cut to them. */
@@ -559,7 +562,10 @@ int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const 
  * with the scores and the lse of megakernel_op_kv8_attention_scored() of the same
  * batch.  Positions of the batch's own rows start anew, so blocks need no initial
  * weights; positions past kv_len and sequences without rows are left alone.
- * Sums are fp32, in an order that depends on sizes alone. */
+ * Sums are fp32, in an order that depends on sizes alone.  As lse is fp32, a weight
+ * is off by up to 2^-21 |lse| of itself: rows whose scores are all in the millions
+ * (slopes that rise, or steep ones where the nearest positions are missing) have
+ * outputs but no weights. */
 int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
                             const megakernel_kv8_scores* scores, const megakernel_rows* q, const float* lse,
                             const megakernel_rows* mass, int n_q, float scale, void* stream);

@@ -661,6 +661,15 @@ struct Bounds {
   }
 };
 
+// A query head's slope to base 2.  Beyond +-2^94 it counts as that (NaN stays):
+// products with distances of up to 2^31 are then finite, and one position further
+// away leaves no weight long before.
+__device__ __forceinline__ float slope_of(const Scores& x, int hd) {
+  if (!x.slopes) return 0.f;
+  const float s = x.slopes[hd];
+  return (s > 0x1p94f ? 0x1p94f : s < -0x1p94f ? -0x1p94f : s) * 1.4426950408889634f;
+}
+
 // Scores of one row to base 2 from q . k, with `add` added, in place: N of them,
 // at(i) is the position of the i-th less that of the row.  A capped one is
 // cap * tanh(y) with tanh(y) = 1 - 2 / (e^2y + 1), off by up to 10 * 2^-24 of the
@@ -904,7 +913,7 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     b.join();
     rows = RowTile{rows.n_rows, b.from, b.shut, b.any, b.all};
     shut = v.lo, see = mine ? v.hi : 0;
-    if (p.x.slopes) slope = p.x.slopes[hd] * 1.4426950408889634f;
+    slope = slope_of(p.x, hd);
   }
   const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
   const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);
@@ -1218,7 +1227,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     b.join();
     rows = RowTile{rows.n_rows, b.from, b.shut, b.any, b.all};
     shut = v.lo, see = mine ? v.hi : 0;
-    if (p.x.slopes) slope = p.x.slopes[hd] * 1.4426950408889634f;
+    slope = slope_of(p.x, hd);
   }
   const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
   const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);

@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void weigh_few(Weigh p) {
 #pragma unroll
       for (int h = 0; h < 2 * KH; ++h) qv[h] = *reinterpret_cast<const bf16x8*>(qp + 64 * (h / 2) + 8 * (h % 2));
       const float ref = p.lse[(long long)(s.row0 + tok) * p.n_q + hd] * 1.4426950408889634f;
-      const float slope = p.x.slopes ? p.x.slopes[hd] * 1.4426950408889634f : 0.f;
+      const float slope = slope_of(p.x, hd);
       float sc[16];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(512, 4) void weigh_many(Weigh p) {
                                            (__attribute__((address_space(3))) void*)&tile[wv][64 * i], 16, 0, 0);
         const int hd = head * G + (mine ? y.set + dh : 0);
         y.lse = p.lse[(long long)(s.row0 + y.tok) * p.n_q + hd];
-        y.slope = p.x.slopes ? p.x.slopes[hd] : 0.f;
+        y.slope = slope_of(p.x, hd);
         return true;
       }
       return false;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(512, 4) void weigh_many(Weigh p) {
     y.u = first_token(p, x) / per * sets + rg;
     bool more = first < s.len && fetch(y);
     while (more) {
-      const float ref = y.lse * 1.4426950408889634f, slope = y.slope * 1.4426950408889634f;
+      const float ref = y.lse * 1.4426950408889634f, slope = y.slope;
       const Sight v = y.v;
       const int rel = first + 4 * h - (s.pos0 + y.tok);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // q is in LDS

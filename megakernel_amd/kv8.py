@@ -219,7 +219,7 @@ class Scores(_Fixed):
         softcap * tanh(scale * q.k / softcap) - slopes[head] * |p - j|
 
     without the tanh where ``softcap`` is 0, and without the bias where there
-    are no ``slopes`` (float32 [n_q], finite).  The row sees
+    are no ``slopes`` (float32 [n_q]; beyond +-2^94 they count as that).  The row sees
     max(0, first[row], p + 1 - window) <= j < max(p + 1, prefix[sequence]):
     ``window`` positions up to its own (0: all), none before its document
     (``first``, int32 [n_tokens]), and of a prefix all (``prefix``, int32
