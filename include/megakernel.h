@@ -588,7 +588,9 @@ int megakernel_op_kv8_select(const megakernel_kv8_cache* cache, const megakernel
  * new blocks are dropped, and rows of a block behind the last stay as they were.
  * new_table's blocks are none that the call reads, each in one entry only.  With
  * mass and new_mass (both or neither; new_mass [n_seq][n_kv][new_width * block])
- * the rows' weights move along.  kept_len is the new sequences' kv_len. */
+ * the rows' weights move along.  The new sequences have kept_len[i] positions; the
+ * kv_len of a batch of them is that plus its own new rows, for which new_table
+ * needs room. */
 int megakernel_op_kv8_compact(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch, const int* kept,
                               const int* kept_len, int keep, const int* new_table, int new_width, const megakernel_rows* mass,
                               const megakernel_rows* new_mass, void* stream);

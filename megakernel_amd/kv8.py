@@ -523,8 +523,11 @@ def compact(cache: Cache, batch: Batch, kept, kept_len, new_table, mass=None, ne
     :func:`append` to blocks that start anew.  These blocks are none that the
     batch's table names, and each stands in one entry; the old ones are free
     afterwards.  With ``mass`` and ``new_mass`` ([n_seq][n_kv][the new table's
-    positions]) the rows' weights move along.  A :class:`Batch` of new_table with
-    kept_len as its lengths goes on from there: its positions are places in the
+    positions]) the rows' weights move along.  kept_len counts what was kept
+    and no more: the :class:`Batch` of new_table that goes on from there has
+    lengths of kept_len plus its own new rows, which are the newest positions
+    (of kept_len alone they would be the last kept ones, and replace them), and
+    the table has blocks for them.  Its positions are places in the
     cache, so scores that count positions (a window, slopes, documents) count
     kept ones, and the rotation goes on from the sequence's own position."""
     _one_gpu(cache, batch)

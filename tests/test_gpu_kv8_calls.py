@@ -65,3 +65,49 @@ def test_a_slope_that_is_nan_reaches_its_own_head_alone():
     kv8.attention(c.cache, c.batch, q, out, scores=kv8.Scores(slopes=torch.tensor([0.5, float("nan"), 0.25, 0.0], device="cuda")))
     torch.cuda.synchronize()
     assert torch.isnan(out[:, 1]).all() and torch.isfinite(out[:, [0, 2, 3]]).all()
+
+
+# ------------------------------------------------------------ after eviction
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 32)])
+def test_rows_after_a_compaction_stand_behind_the_kept_ones(dim, block):
+    """As the usage has it: lengths are kept_len plus the new rows.  Kept rows, their
+    weights and the recent positions among them stay as compaction left them; new
+    rows are attended to with them and start from no weight."""
+    _say(f"rows after a compaction D={dim} block {block}")
+    n_kv, n_q, keep, recent = 2, 4, 40, 8
+    c = Case(block, n_kv, dim, [100, 61, 12], [100, 61, 12], seed=dim + block, extra=3 * (96 // block) + 3)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    used = {int(b) for b in c.table.ravel()}
+    free = [b for b in range(c.pool.n_blocks) if b not in used]
+    width = 96 // block
+    new_table = i32(free[: 3 * width]).view(3, width).contiguous()
+    mass, new_mass = torch.rand((3, n_kv, c.table.shape[1] * block), device="cuda"), torch.full((3, n_kv, 96), 5.0, device="cuda")
+    kept, kept_len = torch.empty((3, n_kv, keep), dtype=torch.int32, device="cuda"), torch.empty(3, dtype=torch.int32, device="cuda")
+    kv8.select(c.cache, c.batch, mass, kept, kept_len, recent=recent)
+    kv8.compact(c.cache, c.batch, kept, kept_len, new_table, mass, new_mass)
+    assert kept_len.tolist() == [40, 40, 12] and kept[0, :, -recent:].tolist() == [list(range(92, 100))] * n_kv
+
+    def rows():  # what the cache holds of the kept rows
+        start = torch.cat([i32([0]), kept_len.cumsum(0, dtype=torch.int32)])
+        k, v = (torch.empty((92, n_kv, dim), device="cuda") for _ in range(2))
+        kv8.read(c.cache, kv8.Batch(new_table, start, kept_len, 92), k, v)
+        return torch.cat([k, v])
+
+    before, weights = rows(), new_mass.clone()
+    new = [1, 20, 0]
+    q_start = i32([0, 1, 21, 21])
+    kv_len = kept_len + (q_start[1:] - q_start[:-1])
+    batch = kv8.Batch(new_table, q_start, kv_len, 21)
+    k, v = 0.1 * c.rng.standard_normal((2, 21, n_kv, dim))  # smaller than what is there: no scale grows
+    kv8.append(c.cache, batch, *(torch.from_numpy(x).to(torch.bfloat16).cuda() * 2.0 ** -8 for x in (k, v)))
+    q, out = torch.from_numpy(c.rng.standard_normal((21, n_q, dim))).to(torch.bfloat16).cuda(), torch.empty((21, n_q, dim), dtype=torch.bfloat16, device="cuda")
+    lse = torch.empty((21, n_q), device="cuda")
+    kv8.attention(c.cache, batch, q, out, lse=lse)
+    kv8.weigh(c.cache, batch, q, lse, new_mass)
+    torch.cuda.synchronize()
+    assert torch.equal(rows(), before)
+    for i, (n, had) in enumerate(zip(new, kept_len.tolist())):
+        gained = (new_mass[i, :, : had + n] - torch.nn.functional.pad(weights[i, :, :had], (0, n))).double()
+        # each of a row's two heads gives 1 in all, off by 1e-5 of itself at most; new positions began at none
+        assert torch.all(gained >= -1e-5) and torch.all((gained.sum(-1) - 2 * n).abs() <= 1e-3), i
+        assert torch.all(new_mass[i, :, had + n :] == 5.0)
