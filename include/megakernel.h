@@ -554,6 +554,19 @@ int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const 
                                        const megakernel_rows* out, float* lse, int n_q, float scale, void* workspace,
                                        long long workspace_bytes, void* stream);
 
+/* Which kernels the attention of such a batch runs (scores NULL: without any), for
+ * reading profiles and for tests that mean one of them: MK_KV8_* together, or -1.
+ * ROWS takes 16 query rows a workgroup, TILE 128; both where sequences with few and
+ * many rows may meet.  SPLIT: contexts are dealt in parts, which a second launch
+ * joins, a row a workgroup or (JOIN_WAVES) four to a wave. */
+#define MK_KV8_ROWS 1
+#define MK_KV8_TILE 2
+#define MK_KV8_ROWS_SPLIT 4
+#define MK_KV8_TILE_SPLIT 8
+#define MK_KV8_JOIN_WAVES 16
+int megakernel_op_kv8_attention_kernels(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                        const megakernel_kv8_scores* scores, int n_q);
+
 /* What each cached position is worth: mass [n_seq][n_kv][positions] (fp32 rows;
  * token_stride from one sequence to the next, positions at least table_width *
  * block).  For sequence i, KV head h and position j

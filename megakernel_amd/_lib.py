@@ -99,6 +99,7 @@ SIGNATURES = {
     "megakernel_op_kv8_scored_workspace_bytes": (c_ll, [c_void_p, c_void_p, c_void_p, c_int, c_int]),
     "megakernel_op_kv8_attention_scored": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                                    c_float, c_void_p, c_ll, c_void_p]),
+    "megakernel_op_kv8_attention_kernels": (c_int, [c_void_p, c_void_p, c_void_p, c_int]),
     "megakernel_op_kv8_weigh": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float,
                                         c_void_p]),
     "megakernel_op_kv8_select": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,

@@ -313,6 +313,16 @@ static long long workspace(const Plan& p, int n_kv, int head_dim, bool lse) {
          (lse ? 4 * (part_rows(p, FEW, n_kv) + part_rows(p, MANY, n_kv)) : 0);
 }
 
+// Tokens whose rows may have splits to join.
+static long long joined_tokens(const Plan& p, const megakernel_kv8_batch* b, int group) {
+  const long long few = (long long)b->n_seq * (p.few / group);
+  return !p.target[MANY] && p.use[MANY] && b->n_tokens > few ? few : b->n_tokens;
+}
+// A workgroup for every row, or where rows are many a wave for four (us in all,
+// in a graph: one row of 32,768 positions 18.9 / 31.5, 1,056 rows of drafted
+// tokens 38.8 / 40.8, a prompt's 16,384 335 / 311).
+static bool join_each(long long tokens, int n_q) { return tokens * n_q <= 4096; }
+
 static bool heads_ok(const char* op, int n_q, int n_kv) {
   if (n_kv < 1 || n_kv > 1024 || n_q < 1 || n_q > 1024 || n_q % n_kv) {
     set_err("%s: n_q=%d must be a multiple of n_kv=%d (both 1..1024)", op, n_q, n_kv);
@@ -433,13 +443,8 @@ static int attend(const char* op, const megakernel_kv8_cache* cache, const megak
     p.ex[MANY] = p.ex[FEW] + part_rows(pl, FEW, cache->n_kv);
   }
   const long long few = pl.items[FEW] * cache->n_kv, many = pl.items[MANY] * cache->n_kv;
-  // tokens whose rows may have splits to join
-  long long tokens = batch->n_tokens;
-  if (!pl.target[MANY] && pl.use[MANY] && tokens > (long long)batch->n_seq * (pl.few / p.group)) tokens = (long long)batch->n_seq * (pl.few / p.group);
-  // a workgroup for every row, or where rows are many a wave for four (us in all,
-  // in a graph: one row of 32,768 positions 18.9 / 31.5, 1,056 rows of drafted
-  // tokens 38.8 / 40.8, a prompt's 16,384 335 / 311)
-  const bool each = tokens * n_q <= 4096;
+  const long long tokens = joined_tokens(pl, batch, p.group);
+  const bool each = join_each(tokens, n_q);
   const long long joins = !need ? 0 : each ? tokens * n_q : (tokens * ((n_q + 3) / 4) + 3) / 4;
   if (!grid_ok(op, few * 2 + many) || !grid_ok(op, joins)) return -1;
   const bool d64 = cache->head_dim == 64;
@@ -607,6 +612,18 @@ int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const 
   const auto go = lse ? attend<AttnLse> : attend<AttnScored>;
   return go("op_kv8_attention_scored", cache, batch, scores, q, out, lse, n_q, scale, d_workspace, workspace_bytes,
             static_cast<hipStream_t>(stream));
+}
+
+int megakernel_op_kv8_attention_kernels(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
+                                        const megakernel_kv8_scores* scores, int n_q) {
+  const char* op = "op_kv8_attention_kernels";
+  if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || (scores && !scores_ok(op, scores)) || !heads_ok(op, n_q, cache->n_kv)) return -1;
+  const Plan p = plan(cache, batch, n_q, scores ? scores->window : 0);
+  int r = 0;
+  if (p.use[FEW]) r |= MK_KV8_ROWS | (p.target[FEW] ? MK_KV8_ROWS_SPLIT : 0);
+  if (p.use[MANY]) r |= MK_KV8_TILE | (p.target[MANY] ? MK_KV8_TILE_SPLIT : 0);
+  if ((p.target[FEW] || p.target[MANY]) && !join_each(joined_tokens(p, batch, n_q / cache->n_kv), n_q)) r |= MK_KV8_JOIN_WAVES;
+  return r;
 }
 
 int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,

@@ -421,6 +421,22 @@ def workspace_bytes(cache: Cache, batch: Batch, n_q: int, scores: Scores | None 
     return need
 
 
+_KERNELS = ("rows", "tile", "rows split", "tile split", "join by waves")  # bits of MK_KV8_*
+
+
+def attention_kernels(cache: Cache, batch: Batch, n_q: int, scores: Scores | None = None) -> set[str]:
+    """Which kernels :func:`attention` runs for these sizes: "rows" (16 query rows a
+    workgroup), "tile" (128), both where sequences with few and many rows may meet;
+    "rows split" and "tile split" where contexts are dealt in parts; "join by waves"
+    where these are joined by waves, not by a workgroup for each row.  For reading
+    profiles, and for tests that mean one of them."""
+    _one_gpu(cache, batch)
+    lib = _lib.load()
+    x = None if scores is None else _scores(scores, batch, n_q)._ref
+    bits = _lib.check(lib, lib.megakernel_op_kv8_attention_kernels(cache._ref, batch._ref, x, n_q), "op_kv8_attention_kernels")
+    return {name for i, name in enumerate(_KERNELS) if bits >> i & 1}
+
+
 def attention(cache: Cache, batch: Batch, q, out, scale: float | None = None, workspace=None, scores: Scores | None = None,
               lse=None):
     """Causal attention of q [n_tokens][n_q][head_dim] (bf16) over the cache

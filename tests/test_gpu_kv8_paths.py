@@ -1,0 +1,127 @@
+"""GPU parity of the paged 8-bit KV cache's operators on the kernels that long
+prompts and large batches run, against oracle/kv8.py (64 bits) with the tolerances
+of test_gpu_kv8_more.py.  A window cuts the contexts that the attention's kernel is
+chosen by, so each test that means one kernel says so and asks which it is."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from megakernel_amd import kv8
+from oracle import kv8 as okv8
+from tests import test_gpu_kv8_more as more
+from tests.test_gpu_kv8 import Case, _hint, _say
+
+pytestmark = pytest.mark.gpu
+
+
+def _kernels(c, n_q, x):
+    return kv8.attention_kernels(c.cache, c.batch, n_q, more._given(x))
+
+
+def _some(c, every, seed):
+    """Every so many of the batch's tokens, and the first and last of each sequence."""
+    at = set(range(int(c.start[0]) + seed % every, int(c.start[-1]), every))
+    for a, b in zip(c.start[:-1], c.start[1:]):
+        at |= {int(a), int(b) - 1} if b > a else set()
+    return at
+
+
+# ------------------------------------------------- the kernel for many rows
+KINDS = ["window 1", "window 20", "window 64", "window 129", "documents", "nothing", "prefix", "long prefix", "rising", "all"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("block,n_kv,group,dim,lens,new", [(16, 64, 2, 64, [390], [240]), (32, 64, 2, 128, [280], [171]),
+                                                           (64, 64, 3, 64, [200, 45, 9], [170, 1, 9]), (16, 64, 3, 128, [190, 45], [131, 2])])
+def test_scores_in_tiles_of_128_rows(block, n_kv, group, dim, lens, new, kind):
+    """Whole contexts in the kernel for many rows, alone and beside sequences of few."""
+    n_q = n_kv * group
+    c = Case(block, n_kv, dim, lens, new, seed=block + dim + sum(lens), missing=0.1)
+    x = more._scores_of(kind, c, n_q)
+    _say(f"tiles {block} {n_kv}x{group} D={dim} {lens} {kind} {_kernels(c, n_q, x)}")
+    assert _kernels(c, n_q, x) == ({"tile"} if len(lens) == 1 else {"rows", "tile"})
+    more._check(c, n_q, x, tokens=_some(c, 19, KINDS.index(kind)), mass=False)
+
+
+@pytest.mark.parametrize("dim,n_kv,tokens,window", [(64, 64, 240, 2900), (128, 16, 550, 2100)])
+def test_scores_in_split_tiles_under_a_window(dim, n_kv, tokens, window):
+    """A window that is long enough for its tiles to be split; blocks before it were
+    never written, and hold NaN codes and NaN scales."""
+    length, n_q = window + tokens + 500, 2 * n_kv
+    c = Case(128, n_kv, dim, [length], [tokens], seed=dim, fill=False)
+    x = okv8.Scores(window=window)
+    seen = length - tokens + 1 - window  # the first position that some row sees
+    for j in range(seen // 128, len(c.table[0])):
+        b = int(c.table[0, j])
+        c.pool.k[b], c.pool.v[b] = (c.rng.integers(0, 0x60, s).astype(np.uint8) for s in (c.pool.k[b].shape, c.pool.v[b].shape))
+        c.pool.ks[b], c.pool.vs[b] = 2.0 ** -6, 2.0 ** -3
+    c.table[0, seen // 128 + 3] = -1
+    c.upload()
+    _say(f"split tiles under a window D={dim} {_kernels(c, n_q, x)}")
+    assert {"tile", "tile split"} <= _kernels(c, n_q, x)
+    rows = {0, 1, 63, 64, tokens // 2, tokens - 2, tokens - 1}
+    more._check(c, n_q, x, tokens=rows, mass=False)
+    more._check(c, n_q, okv8.Scores(window=window, softcap=20.0), tokens=rows, mass=False)
+
+
+@pytest.mark.parametrize("dim,tokens", [(64, 240), (128, 171)])
+@pytest.mark.parametrize("block", [16, 32])
+def test_tiles_leave_unseen_garbage_out(dim, tokens, block):
+    """A fresh pool holds NaN codes and NaN scales; blocks before a window or a
+    document were never written, a block that some rows see is missing."""
+    length, n_kv, n_q = tokens + 90, 64, 128
+    for x, seen in ((okv8.Scores(window=22), 69), (okv8.Scores(window=1), 90), (okv8.Scores(first=np.full(tokens, 70)), 70),
+                    (okv8.Scores(window=64, first=np.full(tokens, 33), softcap=9.0), 33)):
+        c = Case(block, n_kv, dim, [length], [tokens], seed=22, fill=False)
+        for j in range(seen // 16 * 16 // block, len(c.table[0])):
+            b = int(c.table[0, j])
+            c.pool.k[b], c.pool.v[b] = (c.rng.integers(0, 0x60, s).astype(np.uint8) for s in (c.pool.k[b].shape, c.pool.v[b].shape))
+            c.pool.ks[b], c.pool.vs[b] = 2.0 ** -6, 2.0 ** -3
+        c.table[0, 160 // block] = -1
+        c.upload()
+        _say(f"tiles and garbage D={dim} block {block} window {x.window} from {seen} {_kernels(c, n_q, x)}")
+        assert _kernels(c, n_q, x) == {"tile"}
+        more._check(c, n_q, x, tokens=_some(c, 17, seen), mass=False)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_split_tiles_leave_garbage_before_documents_out(dim):
+    """Documents alone, announced as long: the kernel for many rows, split."""
+    c = Case(16, 2, dim, [400], [60], seed=23, fill=False)
+    for j in range(128 // 16, len(c.table[0])):
+        b = int(c.table[0, j])
+        c.pool.k[b], c.pool.v[b], c.pool.ks[b], c.pool.vs[b] = 0x38, 0xB8, 0.5, 0.25
+    c.table[0, 12] = -1
+    c.upload()
+    _hint(c, 1 << 20)
+    for first in (128, 131, 143, 201):  # in the first run of 16, and steps further on
+        x = okv8.Scores(first=np.where(np.arange(60) % 7, first, 300))
+        _say(f"split tiles and garbage D={dim} first {first} {_kernels(c, 4, x)}")
+        assert {"tile", "tile split"} <= _kernels(c, 4, x)
+        more._check(c, 4, x)
+
+
+@pytest.mark.parametrize("dim,tokens", [(64, 240), (128, 171)])
+def test_tiles_keep_nan_from_rows_that_do_not_see_it(dim, tokens):
+    """NaN before a window, before a document and behind a prefix, in steps that
+    some rows of a tile see whole, some in part and some not at all."""
+    n_kv, n_q, past = 64, 128, 50
+    c = Case(16, n_kv, dim, [past + tokens], [tokens], seed=24)
+    b = [int(c.table[0, p // 16]) for p in range(past + tokens)]
+    c.pool.v[b[70], :, 5, 70 % 16] = 0x7F
+    c.pool.v[b[3], 0, 9, 3] = 0xFF
+    c.pool.k[b[64], 1, 0, 7] = 0x7F
+    c.upload()
+    x = okv8.Scores(window=30, prefix=[60])
+    _say(f"tiles and NaN D={dim} {_kernels(c, n_q, x)}")
+    assert _kernels(c, n_q, x) == {"tile"}
+    near = {t for p in (50, 59, 60, 63, 64, 69, 70, 93, 94, 99, 100, 127, 128) for t in (p - past, p - past + 1)} | {tokens - 1}
+    _, out, _, _ = more._check(c, n_q, x, nan_ok=True, tokens=near, mass=False)
+    assert torch.isnan(out[20:50, :2, 5]).all() and not torch.isnan(out[50:, :2]).any()       # 70 is seen from 70 to 99
+    assert not torch.isnan(out[:14, 2:4, 5]).any() and torch.isnan(out[14:44, 2:4]).all()     # key 64, of KV head 1, from 64 to 93
+    docs = okv8.Scores(first=np.where(np.arange(past, past + tokens) >= 80, 71, 4))
+    assert _kernels(c, n_q, docs) == {"tile"}
+    _, out, _, _ = more._check(c, n_q, docs, nan_ok=True, tokens=near, mass=False)
+    assert torch.isnan(out[20:30, :, 5]).all() and not torch.isnan(out[30:, 0]).any()

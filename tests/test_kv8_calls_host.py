@@ -136,3 +136,29 @@ def test_attention_read_and_weigh_refuse_outputs_on_other_tensors(clib):  # noqa
     w = clib.megakernel_op_kv8_weigh
     _refused(clib, w(c, b, x, _ref(_r()), 4 * FAKE + 64, _ref(_mass()), 8, 1.0, None), "mass and lse")
     _refused(clib, w(c, b, x, _ref(_r(4 * FAKE + 64)), FAKE, _ref(_mass()), 8, 1.0, None), "mass and q")
+
+
+# ------------------------------------------------------- which kernels run
+ROWS, TILE, ROWS_SPLIT, TILE_SPLIT, JOIN_WAVES = 1, 2, 4, 8, 16
+
+
+@pytest.mark.parametrize("n_kv,dim,batch,x,want", [
+    (8, 64, dict(table_width=64, n_seq=1, n_tokens=1), {}, ROWS), (8, 64, dict(table_width=4096, n_seq=1, n_tokens=1), {}, ROWS | ROWS_SPLIT),
+    (8, 64, dict(table_width=4096, n_seq=1, n_tokens=1), dict(window=100), ROWS), (8, 128, dict(table_width=256, n_seq=1, n_tokens=4096), {}, TILE),
+    (8, 128, dict(table_width=256, n_seq=1, n_tokens=4096), dict(window=64), TILE), (8, 64, dict(table_width=256, n_seq=3, n_tokens=4096), {}, ROWS | TILE),
+    (2, 64, dict(table_width=16, n_seq=1, n_tokens=300, max_kv=1 << 20), {}, TILE | TILE_SPLIT | JOIN_WAVES),
+    (2, 64, dict(table_width=16, n_seq=1, n_tokens=200, max_kv=1 << 20), dict(softcap=5.0), TILE | TILE_SPLIT)])
+def test_kernels_of_an_attention(clib, n_kv, dim, batch, x, want):  # noqa: F811
+    c, b = _ref(_cache(n_kv=n_kv, head_dim=dim, block=16)), _ref(_batch(**batch))
+    assert clib.megakernel_op_kv8_attention_kernels(c, b, _ref(_x(**x)), 16) == want
+    # what is split has partials
+    assert (clib.megakernel_op_kv8_scored_workspace_bytes(c, b, _ref(_x(**x)), 16, 0) > 0) == bool(want & (ROWS_SPLIT | TILE_SPLIT))
+
+
+def test_kernels_of_an_attention_that_is_refused(clib):  # noqa: F811
+    q = clib.megakernel_op_kv8_attention_kernels
+    _refused(clib, q(None, _ref(_batch()), None, 8), "null cache")
+    _refused(clib, q(_ref(_cache()), None, None, 8), "null batch")
+    _refused(clib, q(_ref(_cache()), _ref(_batch()), _ref(_x(window=-1)), 8), "window=-1")
+    _refused(clib, q(_ref(_cache()), _ref(_batch()), None, 12), "n_q=12")
+    assert q(_ref(_cache()), _ref(_batch()), None, 8) == q(_ref(_cache()), _ref(_batch()), _ref(_x()), 8) == 1
