@@ -125,3 +125,20 @@ def test_tiles_keep_nan_from_rows_that_do_not_see_it(dim, tokens):
     assert _kernels(c, n_q, docs) == {"tile"}
     _, out, _, _ = more._check(c, n_q, docs, nan_ok=True, tokens=near, mass=False)
     assert torch.isnan(out[20:30, :, 5]).all() and not torch.isnan(out[30:, 0]).any()
+
+
+# --------------------------------------------------------- the join by waves
+@pytest.mark.parametrize("kind", ["cap", "slopes", "documents", "nothing", "prefix", "all"])
+@pytest.mark.parametrize("dim,n_kv,group,lens,new", [(64, 2, 3, [900], [700]), (128, 2, 3, [900], [700]), (64, 1, 7, [700, 5, 400], [400, 5, 250]),
+                                                     (128, 3, 3, [800, 33], [500, 1])])
+def test_scores_joined_by_waves(dim, n_kv, group, lens, new, kind):
+    """More rows than a workgroup each, four heads of a token to a wave, with heads
+    left over; _check() runs every call without and with log-sum-exps."""
+    n_q = n_kv * group
+    c = _hint(Case(16, n_kv, dim, lens, new, seed=dim + n_q, missing=0.05), 1 << 20)
+    x = more._scores_of(kind, c, n_q)
+    if kind == "all":
+        x.window = 0  # a short window leaves nothing to split
+    _say(f"joined by waves D={dim} {n_kv}x{group} {lens} {kind} {_kernels(c, n_q, x)}")
+    assert {"tile split", "join by waves"} <= _kernels(c, n_q, x) and n_q % 4
+    more._check(c, n_q, x, tokens=_some(c, 11, len(kind)), mass=False)
