@@ -142,3 +142,17 @@ def test_scores_joined_by_waves(dim, n_kv, group, lens, new, kind):
     _say(f"joined by waves D={dim} {n_kv}x{group} {lens} {kind} {_kernels(c, n_q, x)}")
     assert {"tile split", "join by waves"} <= _kernels(c, n_q, x) and n_q % 4
     more._check(c, n_q, x, tokens=_some(c, 11, len(kind)), mass=False)
+
+
+# ------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("src,dst", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                     (torch.float32, torch.float32)])
+@pytest.mark.parametrize("tokens,n_q,n_kv,dim,turned,layout", [
+    (4701, 7, 1, 128, 64, "packed"), (4801, 5, 2, 128, 128, "in place"), (1101, 3, 2, 1024, 512, "heads"), (5501, 9, 3, 80, 16, "in place"),
+    (9001, 3, 1, 128, 32, "in place"), (5303, 2, 1, 272, 272, "packed")])
+def test_rotary_of_four_heads_a_thread(tokens, n_q, n_kv, dim, turned, layout, src, dst, interleaved):
+    """Twice as many pieces as a thread takes four heads from on: head counts that are
+    no multiple of four and one that is, parts and all of a head, all layouts."""
+    assert tokens * (dim // 16) * (n_q + n_kv) > 1 << 18
+    more.test_rotary(tokens, n_q, n_kv, dim, turned, layout, src, dst, interleaved)
