@@ -9,11 +9,14 @@ import pytest
 import torch
 
 from megakernel_amd import kv8
+from oracle import fp8
 from oracle import kv8 as okv8
 from tests import test_gpu_kv8_more as more
-from tests.test_gpu_kv8 import Case, _hint, _say
+from tests.test_gpu_kv8 import U, Case, _f64, _hint, _say
 
 pytestmark = pytest.mark.gpu
+
+TINY = 2.0 ** -126
 
 
 def _kernels(c, n_q, x):
@@ -156,3 +159,80 @@ def test_rotary_of_four_heads_a_thread(tokens, n_q, n_kv, dim, turned, layout, s
     no multiple of four and one that is, parts and all of a head, all layouts."""
     assert tokens * (dim // 16) * (n_q + n_kv) > 1 << 18
     more.test_rotary(tokens, n_q, n_kv, dim, turned, layout, src, dst, interleaved)
+
+
+# -------------------------------------------------------------------- weigh
+def _check_weigh(c, n_q, x):
+    """lse and weights of every row against 64 bits, one head after the other."""
+    q = c.rows(n_q, torch.bfloat16, 1.5)
+    given, width = more._given(x), c.table.shape[1] * c.block
+    out, lse = torch.empty((c.tokens, n_q, c.dim), dtype=torch.bfloat16, device="cuda"), torch.empty((c.tokens, n_q), device="cuda")
+    old = torch.from_numpy(c.rng.random((len(c.lens), c.n_kv, width), dtype=np.float32))
+    mass, qc = old.cuda(), q.cuda()
+    kv8.attention(c.cache, c.batch, qc, out, scores=given, lse=lse)
+    kv8.weigh(c.cache, c.batch, qc, lse, mass, scores=given)
+    torch.cuda.synchronize()
+    got, got_lse, group, scale = _f64(mass), _f64(lse), n_q // c.n_kv, c.dim ** -0.5
+    table = fp8.e4m3_decode_table().astype(np.float64)
+    for i, length in enumerate(int(v) for v in c.lens):
+        a, b = int(c.start[i]), int(c.start[i + 1])
+        ids = c.table[i, : -(-length // c.block)]
+        there = np.repeat((ids >= 0) & (ids < c.pool.n_blocks), c.block)[:length]
+        ids = np.where((ids >= 0) & (ids < c.pool.n_blocks), ids, 0)
+        p, j = np.arange(length - (b - a), length)[:, None], np.arange(length)[None]
+        spans = np.array([x.span(i, t, length - b + t, length) for t in range(a, b)])
+        seen = (j >= spans[:, :1]) & (j < spans[:, 1:]) & there
+        for h in range(c.n_kv):
+            keys = (table[c.pool.k[ids, h]] * c.pool.ks[ids, h][:, None, None]).reshape(-1, c.dim)[:length]
+            want, tol = np.zeros(length), np.zeros(length)
+            want[: length - (b - a)] = _f64(old[i, h, : length - (b - a)])
+            tol += ((b - a) * group + 32) * U * np.abs(want)
+            for hd in range(h * group, (h + 1) * group):
+                qh = _f64(q[a:b, hd])
+                s = qh @ keys.T * scale
+                reach = (np.abs(qh) @ np.abs(keys).T * scale).max(1)
+                if x.softcap:
+                    s = x.softcap * np.tanh(s / x.softcap)
+                s[~seen] = -np.inf
+                top = s.max(1, keepdims=True)
+                none = np.isinf(top[:, 0])
+                top[none] = 0
+                w = np.exp(s - top)
+                total = w.sum(1, keepdims=True)
+                with np.errstate(divide="ignore"):
+                    ref = top + np.log(total)
+                w /= np.where(none[:, None], 1, total)
+                big = np.abs(np.where(seen, s, 0)).max(1)
+                e = (c.dim + 3) * U * reach + 10 * U * x.softcap + 3 * U * big
+                ref0 = np.where(none, 0, ref[:, 0])
+                tol_lse = e + (length + 16) * U + 4 * U * np.abs(ref0) + length * TINY
+                assert np.all((np.abs(got_lse[a:b, hd] - ref[:, 0]) <= tol_lse) | (got_lse[a:b, hd] == ref[:, 0])), (i, hd)
+                want += w.sum(0)
+                per_row = 2 * e + tol_lse + 4 * U * (big + np.abs(ref0)) + ((b - a) * group + 36) * U
+                tol += (w * per_row[:, None]).sum(0) + (b - a) * TINY
+            off = np.abs(got[i, h, :length] - want) > tol
+            assert not off.any(), (i, h, int(off.sum()), np.argwhere(off)[:3].ravel(), got[i, h, :length][off][:3], want[off][:3], tol[off][:3])
+            assert np.array_equal(got[i, h, length:], _f64(old[i, h, length:]))
+
+
+@pytest.mark.parametrize("x", [okv8.Scores(), okv8.Scores(window=900, softcap=30.0)], ids=["plain", "capped window"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_by_waves_that_take_several_steps(dim, x):
+    """More steps times KV heads than run at once, few rows: 16 workgroups a head for
+    34 times four steps of two sequences."""
+    _say(f"weights, waves of several steps D={dim}")
+    c = Case(64, 256, dim, [4300, 800], [1, 2], seed=dim, missing=0.02)
+    assert -(-4300 // 64) * 2 // 4 > 4096 // 256
+    _check_weigh(c, 256, x)
+
+
+@pytest.mark.parametrize("kind", ["plain", "capped window", "documents"])
+@pytest.mark.parametrize("dim,lens,new", [(64, [1500], [530]), (128, [1340], [400])])
+def test_weights_by_workgroups_that_take_several_steps(dim, lens, new, kind):
+    """The same with many rows: 16 workgroups a head for 24 (21) steps."""
+    _say(f"weights, workgroups of several steps D={dim} {kind}")
+    c = Case(32, 256, dim, lens, new, seed=dim + 1, missing=0.02)
+    assert -(-lens[0] // 64) > 4096 // 256 and new[0] > (512 if dim == 64 else 384)
+    pos = np.arange(lens[0] - new[0], lens[0])
+    _check_weigh(c, 256, {"plain": okv8.Scores(), "capped window": okv8.Scores(window=300, softcap=30.0),
+                          "documents": okv8.Scores(first=pos // 211 * 211)}[kind])
