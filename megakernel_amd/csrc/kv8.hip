@@ -654,19 +654,26 @@ int megakernel_op_kv8_weigh(const megakernel_kv8_cache* cache, const megakernel_
     return -1;
   Weigh p{cache_of(cache), batch_of(batch), rows_of(q), lse, mass_of(mass), n_q, group, scale2, scores_of(scores, scale2)};
   long long kv = batch->max_kv && batch->max_kv < all ? batch->max_kv : all;
-  // Steps of 64 positions: a wave's with few rows, a workgroup's with many.  The
-  // workgroup takes 4 us to start on one, and pays where rows are so many that a
-  // wave would be long at them while others have none (us of weigh_few /
-  // weigh_many, head_dim 64; one sequence of 4,096 positions, 16 tokens 5.7 / 7.4, 32
-  // 7.3 / 7.6, 64 10.4 / 8.3; 16 of 1,024, 64 tokens 12 / 24, 256 about 33 / 36; 16 of
-  // 4,096, 64 tokens 33 / 74; 128: 64 tokens 12.4 / 9.5, 17 / 29, 57 / 95).
   const long long steps = (kv + TILE - 1) / TILE * batch->n_seq, items = steps * cache->n_kv;
-  const long long most = cache->head_dim == 64 ? 512 : 384, enough = items / 4 < 32 ? 32 : items / 4 > most ? most : items / 4;
-  const bool many = rows > enough * batch->n_seq;
-  // In steps of 32 positions where those of 64 are not two workgroups for every
-  // CU (1,024 tokens in steps of 32 / 64, head_dim 128: at 1,024 positions 13 / 20,
-  // 2,048 21 / 22, 4,096 39 / 34, 8,192 72 / 64).
-  const bool half = many && items < 512;
+  // Of weigh_many in steps of 32 positions where those of 64 are not two workgroups
+  // for every CU (1,024 tokens in steps of 32 / 64, head_dim 128: at 1,024 positions
+  // 13 / 20, 2,048 21 / 22, 4,096 39 / 34, 8,192 72 / 64).
+  const bool small = items < 512;
+  // Steps of 64 positions: a wave's with few rows, a workgroup's with many.  512 such
+  // workgroups run at once and take 4 us and more to start, a wave is long at many
+  // rows: where one round of workgroups is all, they pay from 80 rows a sequence on,
+  // else from as many as a third of the steps, until the waves' own way is bound by
+  // its operations (us of weigh_few / weigh_many, 16 / 8 heads; head_dim 64, one
+  // sequence of 1,024 positions, 32 rows 6.4 / 6.6, 64 8.0 / 6.5; of 4,096, 64 rows
+  // 8.0 / 8.3, 128 11.2 / 9.1; of 8,192, 320 rows 17.1 / 17.6, 384 20.5 / 18.7; three
+  // of 1,024, 128 rows 11.2 / 11.1; 16 of 1,024, 512 rows 29 / 37, 1,024 51 / 52; 8 of
+  // 4,096, 1,024 rows 91 / 99, 1,536 133 / 129; 16 of 4,096, 1,024 rows 178 / 182, 1,536
+  // 262 / 239; 128: one of 4,096, 64 rows 9.5 / 9.5, 128 13.0 / 10.2; of 8,192, 320 rows
+  // 20.5 / 21.3, 384 24.3 / 22.9; 8 of 4,096, 320 rows 70 / 73, 512 105 / 93; 16 of 4,096,
+  // 384 rows 133 / 143, 512 172 / 168).
+  const long long most = (small ? 2 * items : items) <= 512 ? 80 : cache->head_dim == 64 ? 1280 : 512;
+  const long long enough = items / 3 < 32 ? 32 : items / 3 > most ? most : items / 3;
+  const bool many = rows > enough * batch->n_seq, half = many && small;
   long long groups = half ? 2 * steps : many ? steps : (steps + 3) / 4;
   // more than one step each where that is more workgroups than run at once
   if (groups > 4096 / cache->n_kv) groups = 4096 / cache->n_kv;

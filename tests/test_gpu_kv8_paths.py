@@ -226,13 +226,27 @@ def test_weights_by_waves_that_take_several_steps(dim, x):
     _check_weigh(c, 256, x)
 
 
-@pytest.mark.parametrize("kind", ["plain", "capped window", "documents"])
-@pytest.mark.parametrize("dim,lens,new", [(64, [1500], [530]), (128, [1340], [400])])
+@pytest.mark.parametrize("dim,lens,new,kind", [(64, [1400], [1400], "plain"), (64, [1400], [1400], "capped window"), (128, [1340], [620], "plain"),
+                                               (128, [1340], [620], "capped window"), (128, [1340], [620], "documents")])
 def test_weights_by_workgroups_that_take_several_steps(dim, lens, new, kind):
-    """The same with many rows: 16 workgroups a head for 24 (21) steps."""
+    """The same with many rows, more than waves are ever given: 16 workgroups a head
+    for 22 (21) steps."""
     _say(f"weights, workgroups of several steps D={dim} {kind}")
     c = Case(32, 256, dim, lens, new, seed=dim + 1, missing=0.02)
-    assert -(-lens[0] // 64) > 4096 // 256 and new[0] > (512 if dim == 64 else 384)
+    assert -(-lens[0] // 64) > 4096 // 256 and new[0] > (1280 if dim == 64 else 512)
     pos = np.arange(lens[0] - new[0], lens[0])
     _check_weigh(c, 256, {"plain": okv8.Scores(), "capped window": okv8.Scores(window=300, softcap=30.0),
                           "documents": okv8.Scores(first=pos // 211 * 211)}[kind])
+
+
+@pytest.mark.parametrize("kind", ["plain", "documents", "all"])
+@pytest.mark.parametrize("dim,n_kv,group,lens,new", [(64, 64, 1, [620], [330]), (64, 64, 3, [640], [120]), (128, 64, 1, [620], [330]),
+                                                     (128, 64, 5, [700], [80]), (64, 8, 2, [4096], [64]), (128, 4, 40, [900, 90], [9, 6])])
+def test_weights_by_workgroups(dim, n_kv, group, lens, new, kind):
+    """Half as many rows again as workgroups of 64 positions pay from on (a third of the
+    steps, or 80), heads that fill a tile, and more than it has rows."""
+    n_q, items = n_kv * group, -(-max(lens) // 64) * len(lens) * n_kv
+    _say(f"weights by workgroups D={dim} {n_kv}x{group} {lens} {kind}")
+    c = Case(16, n_kv, dim, lens, new, seed=dim + group, missing=0.1, gap=1)
+    assert sum(new) * group >= 1.5 * len(lens) * (80 if items <= 256 or items == 512 else items / 3)
+    more._check(c, n_q, more._scores_of(kind, c, n_q))
