@@ -206,10 +206,11 @@ struct Plan {
 // Lengths are on the device, so what is chosen here goes by the sizes that
 // the host has: rows, sequences, and how long contexts may get (max_kv).
 // Every choice is right for any lengths.
-static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q, int window = 0) {
+static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, int n_q, const megakernel_kv8_scores* x = nullptr) {
   Plan p{};
   const int group = n_q / c->n_kv;
   const bool d64 = c->head_dim == 64;
+  const int window = x ? x->window : 0;
   const long long rows = (long long)b->n_tokens * group;
   long long kv = b->max_kv ? b->max_kv : (long long)b->table_width * c->block;
   if (window && kv > (long long)window + TILE) kv = (long long)window + TILE;  // a window lies across one step more
@@ -275,9 +276,14 @@ static Plan plan(const megakernel_kv8_cache* c, const megakernel_kv8_batch* b, i
       // workgroups are many (us with 8 / 4 / 2 waves, head_dim 64; 256
       // workgroups of 16 steps 8.0 / 8.9 / 12.7, of 64 16 / 20 / 34; 512 of 24
       // 14.2 / 12.8 / 18.9, of 64 27 / 29 / 46; 1,024 of 4 14 / 10 / 8.5, of 16
-      // 19 / 13 / 15, of 64 53 / 50 / 52; 4,096 of 1 50 / 25 / 18).
+      // 19 / 13 / 15, of 64 53 / 50 / 52; 4,096 of 1 50 / 25 / 18).  With scores the
+      // kernels hold 135 registers and more, three waves a SIMD: of eight waves one
+      // workgroup fits a CU, of four three, so from a workgroup a CU on it is four
+      // (capped, head_dim 64, 8 / 4 waves; 264 workgroups of 64 steps 36 / 30, 320 of
+      // 50 30 / 27, of 64 37 / 32, of 128 73 / 64, 512 of 64 44.5 / 43.9; 128: 68 / 66,
+      // 54 / 52, 73 / 71, 144 / 144, 95 / 94).
       const long long low = (rows / ROWS > b->n_seq ? rows / ROWS : b->n_seq) * c->n_kv;
-      p.waves = low >= 1024 ? (steps <= 8 ? 2 : 4) : steps <= (low > 256 ? 48 : 8) ? 4 : 8;
+      p.waves = low >= 1024 ? (steps <= 8 ? 2 : 4) : (x && low > 256) || steps <= (low > 256 ? 48 : 8) ? 4 : 8;
     }
     p.items[FEW] = tiles + p.target[FEW];
     p.slots[FEW] = 2ll * p.target[FEW];
@@ -408,7 +414,7 @@ static int attend(const char* op, const megakernel_kv8_cache* cache, const megak
   }
   const float scale2 = scale_of(op, x, scale);
   if (!scale2) return -1;
-  const Plan pl = plan(cache, batch, n_q, SCORED ? x->window : 0);
+  const Plan pl = plan(cache, batch, n_q, x);
   const long long need = workspace(pl, cache->n_kv, cache->head_dim, LSE);
   if (need && (!d_workspace || !aligned(d_workspace, 16) || workspace_bytes < need)) {
     set_err("%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", op, need, d_workspace ? workspace_bytes : 0);
@@ -602,7 +608,7 @@ long long megakernel_op_kv8_scored_workspace_bytes(const megakernel_kv8_cache* c
                                                    const megakernel_kv8_scores* scores, int n_q, int with_lse) {
   const char* op = "op_kv8_scored_workspace_bytes";
   if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || !scores_ok(op, scores) || !heads_ok(op, n_q, cache->n_kv)) return -1;
-  return workspace(plan(cache, batch, n_q, scores->window), cache->n_kv, cache->head_dim, with_lse != 0);
+  return workspace(plan(cache, batch, n_q, scores), cache->n_kv, cache->head_dim, with_lse != 0);
 }
 
 int megakernel_op_kv8_attention_scored(const megakernel_kv8_cache* cache, const megakernel_kv8_batch* batch,
@@ -618,7 +624,7 @@ int megakernel_op_kv8_attention_kernels(const megakernel_kv8_cache* cache, const
                                         const megakernel_kv8_scores* scores, int n_q) {
   const char* op = "op_kv8_attention_kernels";
   if (!cache_ok(op, cache) || !batch_ok(op, batch, cache->block) || (scores && !scores_ok(op, scores)) || !heads_ok(op, n_q, cache->n_kv)) return -1;
-  const Plan p = plan(cache, batch, n_q, scores ? scores->window : 0);
+  const Plan p = plan(cache, batch, n_q, scores);
   int r = 0;
   if (p.use[FEW]) r |= MK_KV8_ROWS | (p.target[FEW] ? MK_KV8_ROWS_SPLIT : 0);
   if (p.use[MANY]) r |= MK_KV8_TILE | (p.target[MANY] ? MK_KV8_TILE_SPLIT : 0);

@@ -130,6 +130,22 @@ def test_tiles_keep_nan_from_rows_that_do_not_see_it(dim, tokens):
     assert torch.isnan(out[20:30, :, 5]).all() and not torch.isnan(out[30:, 0]).any()
 
 
+# ---------------------------------------------------- the kernel for few rows
+@pytest.mark.parametrize("kind", ["cap", "slopes", "window 129", "documents", "prefix", "all"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n_kv,lens,hint", [(64, [90, 300, 1, 64] * 8, 300), (64, [700, 33, 650, 129, 700], 700), (2, [700, 80, 640], 700)],
+                         ids=["two waves", "four waves", "eight waves"])
+def test_scores_of_workgroups_of_two_to_eight_waves(n_kv, lens, hint, dim, kind):
+    """Many short contexts (2,048 workgroups of at most five steps), more workgroups
+    than CUs (320, eleven steps), and few (6)."""
+    n_q = 2 * n_kv
+    c = _hint(Case(32, n_kv, dim, lens, [1] * len(lens), seed=dim + n_kv, missing=0.05), hint)
+    x = more._scores_of(kind, c, n_q)
+    _say(f"waves {n_kv} heads {len(lens)} sequences D={dim} {kind} {_kernels(c, n_q, x)}")
+    assert _kernels(c, n_q, x) == {"rows"}
+    more._check(c, n_q, x)
+
+
 # --------------------------------------------------------- the join by waves
 @pytest.mark.parametrize("kind", ["cap", "slopes", "documents", "nothing", "prefix", "all"])
 @pytest.mark.parametrize("dim,n_kv,group,lens,new", [(64, 2, 3, [900], [700]), (128, 2, 3, [900], [700]), (64, 1, 7, [700, 5, 400], [400, 5, 250]),
