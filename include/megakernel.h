@@ -528,7 +528,9 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
  *   hi = p + 1, or prefix[sequence] if that is more (int [n_seq])
  * so `first` is where the row's document begins, `window` how many positions
  * it looks back on, its own among them, and the rows of a prefix see it whole.
- * softcap is 0 or 2^-30 to 1024; capped scores are off by up to 10 * 2^-24 of it.
+ * softcap is 0 or 2^-30 to 1024; a capped score is off by up to 13 * 2^-24 of itself
+ * beyond what q . k is, and by 2 * 2^-24 of the cap besides where another that is
+ * computed with it passes half the cap.
  * With slopes scores and log-sum-exps are off by up to 2^-13 of the slope (or, where
  * blocks before a position are missing, 2^-22 of the bias across them).
  * Positions are those of the cache: after

@@ -382,10 +382,13 @@ static float scale_of(const char* op, const megakernel_kv8_scores* x, float scal
   return scale2;
 }
 static Scores scores_of(const megakernel_kv8_scores* x, float scale2) {
-  Scores r{x->slopes, x->first, x->prefix, x->window, 0.f, 0.f};
+  Scores r{x->slopes, x->first, x->prefix, x->window, 0.f, 0.f, {}};
   if (x->softcap > 0.f) {
     r.cap = x->softcap * 1.4426950408889634f;
-    r.cap_in = 2.f * scale2 / x->softcap;
+    r.cap_in = scale2 / r.cap;
+    // (tanh(sqrt(w)) / sqrt(w) - 1) / w at Chebyshev's nodes of [0, 1/4]
+    const float q[4] = {-0x1.555546p-2f, 0x1.110246p-3f, -0x1.b560bap-5f, 0x1.26e43ep-6f};
+    for (int i = 0; i < 4; ++i) r.c[i] = r.cap * q[i];
   }
   return r;
 }

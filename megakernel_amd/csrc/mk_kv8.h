@@ -574,14 +574,16 @@ struct Scores {
   const int* first;     // [n_tokens], or null
   const int* prefix;    // [n_seq], or null
   int window;           // 0: none
-  float cap, cap_in;    // cap * log2(e) (0: none), 2 log2(e) scale / cap
+  float cap, cap_in;    // cap * log2(e) (0: none), scale / cap
+  float c[4];           // cap * log2(e) times the coefficients of Q of score()
 };
 // The attention with such scores, or with each row's log-sum-exp: the same
 // kernels, compiled once more.  Scores are formed less the row's reference, so
-// what is not asked for costs a branch a step, a cap three operations for each
-// score, two of them slow (1,024 tokens of 16 / 8 heads of 128 at 16,384 positions:
-// causal 153 us, with scores 160, capped 195; four prompts of 2,048 tokens, heads of
-// 64, 67, 72, 104), the log-sum-exp one.  Steps that a row tile sees none of are
+// what is not asked for costs a branch a step, a cap seven operations for each
+// score (where some pass half of it six, two of them slow; 1,024 tokens of 16 / 8 heads
+// of 128 at 16,384 positions: causal 167 us, with scores 160, capped 196; four prompts
+// of 2,048 tokens, heads of 64, 66, 73, 100; where most steps pass half the cap 15 %
+// more), the log-sum-exp one.  Steps that a row tile sees none of are
 // not walked: a window of 4,096 at 32,768 positions takes 12.5 us, the whole 18.
 struct AttnScored : Attn {
   Scores x;
@@ -661,19 +663,21 @@ struct Bounds {
   }
 };
 
-// A query head's slope to base 2.  Beyond +-2^94 it counts as that (NaN stays):
-// products with distances of up to 2^31 are then finite, and one position further
-// away leaves no weight long before.
-__device__ __forceinline__ float slope_of(const Scores& x, int hd) {
-  if (!x.slopes) return 0.f;
-  const float s = x.slopes[hd];
+// A slope to base 2.  Beyond +-2^94 it counts as that (NaN stays): products with
+// distances of up to 2^31 are then finite, and one position further away leaves no
+// weight long before.
+__device__ __forceinline__ float slope_of(float s) {
   return (s > 0x1p94f ? 0x1p94f : s < -0x1p94f ? -0x1p94f : s) * 1.4426950408889634f;
 }
 
 // Scores of one row to base 2 from q . k, with `add` added, in place: N of them,
-// at(i) is the position of the i-th less that of the row.  A capped one is
-// cap * tanh(y) with tanh(y) = 1 - 2 / (e^2y + 1), off by up to 10 * 2^-24 of the
-// cap, which of caps of tens is what rounding scores of tens costs anyway.
+// at(i) is the position of the i-th less that of the row.  A capped one is cap *
+// tanh(y).  Where the wave's are all at most half the cap, tanh(y) = y (1 + y^2 Q(y^2))
+// with Q interpolated at Chebyshev's nodes to 2^-24: off by 8 * 2^-24 of itself at
+// most.  Else (e^2y - 1) / (e^2y + 1), which e^2y near 1 puts off by 2 * 2^-24 of the
+// cap, beside some score that is not small against it.  (For all scores that form,
+// or 1 - 2 / (e^2y + 1), is as fast, but made log-sum-exps of small scores up to 60
+// times less exact than fp32 has them.)
 template <int N, class At>
 __device__ __forceinline__ void score(const Scores& x, float scale, float slope, float add, float* s, At at) {
   if (!x.cap) {
@@ -682,9 +686,28 @@ __device__ __forceinline__ void score(const Scores& x, float scale, float slope,
     asm volatile("");  // branches that stay branches: 64 scores of both kinds at once take registers that are not there
   } else {
     asm volatile("");
-    const float top = x.cap + add;
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = fmaf(-2.f * x.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * x.cap_in) + 1.f), top);
+    for (int i = 0; i < N; ++i) {
+      s[i] *= x.cap_in;
+      most = fmaxf(most, fabsf(s[i]));
+    }
+    if (!__any(most > 0.5f)) {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float w = s[i] * s[i], q = fmaf(fmaf(fmaf(w, x.c[3], x.c[2]), w, x.c[1]), w, x.c[0]);
+        s[i] = fmaf(s[i], fmaf(w, q, x.cap), add);
+      }
+    } else {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        // (e^2y stays finite, and a NaN one)
+        const float t = __builtin_amdgcn_exp2f(s[i] > 40.f ? 115.f : s[i] * 2.8853900817779268f);
+        s[i] = fmaf((t - 1.f) * x.cap, __builtin_amdgcn_rcpf(t + 1.f), add);
+      }
+    }
   }
   if (x.slopes) {
 #pragma unroll
@@ -913,7 +936,7 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     b.join();
     rows = RowTile{rows.n_rows, b.from, b.shut, b.any, b.all};
     shut = v.lo, see = mine ? v.hi : 0;
-    slope = slope_of(p.x, hd);
+    if (p.x.slopes) slope = slope_of(p.x.slopes[hd]);
   }
   const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
   const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);
@@ -1227,7 +1250,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     b.join();
     rows = RowTile{rows.n_rows, b.from, b.shut, b.any, b.all};
     shut = v.lo, see = mine ? v.hi : 0;
-    slope = slope_of(p.x, hd);
+    if (p.x.slopes) slope = slope_of(p.x.slopes[hd]);
   }
   const int t00 = rows.from / TILE, tiles = (rows.any + TILE - 1) / TILE - t00;
   const int t0 = t00 + it.step(it.split, tiles), t1 = t00 + it.step(it.split + 1, tiles);

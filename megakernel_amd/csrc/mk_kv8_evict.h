@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void weigh_few(Weigh p) {
 #pragma unroll
       for (int h = 0; h < 2 * KH; ++h) qv[h] = *reinterpret_cast<const bf16x8*>(qp + 64 * (h / 2) + 8 * (h % 2));
       const float ref = p.lse[(long long)(s.row0 + tok) * p.n_q + hd] * 1.4426950408889634f;
-      const float slope = slope_of(p.x, hd);
+      const float slope = p.x.slopes ? slope_of(p.x.slopes[hd]) : 0.f;
       float sc[16];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -149,8 +149,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void weigh_few(Weigh p) {
 // workgroup are PS side by side, which ask for the same tiles at about the same
 // time, and 8 / PS groups that deal the rows.  Sums stay in 16 registers a lane, and
 // meet over lanes and groups, in a fixed order, at the end.
-// 1,024 tokens of 16 / 8 heads of 128 at the end of 16,384 positions take 118 us (one
-// side by side 130), capped 139 (155); 1,024 tokens without a past 20 (13), 26 (16).
+// 1,024 tokens of 16 / 8 heads of 128 at the end of 16,384 positions take 121 us (one
+// side by side 130), capped 151; 1,024 tokens without a past 20 (14, capped 17).
 // What bounds it is q's way from the L2 (a tile for every 1,024 scores) beside the
 // vector unit, which one wave alone can give an operation only every eight cycles:
 // positions are so few that four waves fit a SIMD.
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(512, 4) void weigh_many(Weigh p) {
                                            (__attribute__((address_space(3))) void*)&tile[wv][64 * i], 16, 0, 0);
         const int hd = head * G + (mine ? y.set + dh : 0);
         y.lse = p.lse[(long long)(s.row0 + y.tok) * p.n_q + hd];
-        y.slope = slope_of(p.x, hd);
+        y.slope = p.x.slopes ? p.x.slopes[hd] : 0.f;  // (nothing here waits for it)
         return true;
       }
       return false;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(512, 4) void weigh_many(Weigh p) {
     y.u = first_token(p, x) / per * sets + rg;
     bool more = first < s.len && fetch(y);
     while (more) {
-      const float ref = y.lse * 1.4426950408889634f, slope = y.slope;
+      const float ref = y.lse * 1.4426950408889634f, slope = slope_of(y.slope);
       const Sight v = y.v;
       const int rel = first + 4 * h - (s.pos0 + y.tok);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // q is in LDS

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from megakernel_amd import kv8
+from oracle import kv8 as okv8
 from tests.test_gpu_kv8 import Case, _f64, _hint, _say
 
 pytestmark = pytest.mark.gpu
@@ -111,3 +112,74 @@ def test_rows_after_a_compaction_stand_behind_the_kept_ones(dim, block):
         # each of a row's two heads gives 1 in all, off by 1e-5 of itself at most; new positions began at none
         assert torch.all(gained >= -1e-5) and torch.all((gained.sum(-1) - 2 * n).abs() <= 1e-3), i
         assert torch.all(new_mass[i, :, had + n :] == 5.0)
+
+
+# --------------------------------------------------------------------- caps
+def _one_hot(c, n_q, size):
+    """Queries of one dimension each, so that a score is one product, exact in fp32."""
+    q = np.zeros((c.tokens, n_q, c.dim))
+    d = c.rng.integers(0, c.dim, (c.tokens, n_q, 1))
+    np.put_along_axis(q, d, size * c.rng.standard_normal((c.tokens, n_q, 1)), 2)
+    return torch.from_numpy(q).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap,size,of_cap", [(50.0, 0.25, 0), (1024.0, 1.0, 0), (1024.0, 0.01, 0), (2.0 ** -30, 2.0 ** -38, 0), (3.0, 3.0, 2), (40.0, 40.0, 2)])
+@pytest.mark.parametrize("hint", [64, 1 << 20])
+def test_capped_scores_keep_what_small_ones_are(dim, cap, size, of_cap, hint):
+    """Log-sum-exps and weights of one to four positions.  A score is one product: its
+    scale and quotient by the cap 3 u of it, the polynomial 8 u, the sum with the
+    reference 2 u; where some score passes half the cap, 2 u of the cap besides
+    (of_cap).  Sums of at most four weights and the logarithm: 20 u, and 4 u |lse|."""
+    _say(f"small scores under a cap of {cap} D={dim} hint {hint}")
+    rng = np.random.default_rng(int(cap) + dim)
+    lens = [1, 2, 3, 4] * 8 + [int(v) for v in rng.integers(1, 5, 30)]
+    c = _hint(Case(16, 2, dim, lens, [1] * len(lens), seed=dim), hint)
+    c.pool.ks[:] = 2.0 ** -1
+    c.upload()
+    q, n_q, u = _one_hot(c, 4, size), 4, 2.0 ** -24
+    x = okv8.Scores(softcap=cap)
+    given, qc = kv8.Scores(softcap=cap), q.cuda()
+    out, lse = torch.empty((c.tokens, n_q, dim), dtype=torch.bfloat16, device="cuda"), torch.empty((c.tokens, n_q), device="cuda")
+    mass = torch.zeros((len(lens), 2, c.table.shape[1] * 16), device="cuda")
+    kv8.attention(c.cache, c.batch, qc, out, scale=1.0, scores=given, lse=lse)
+    for _ in range(4):  # older positions gather, the row's own starts anew
+        kv8.weigh(c.cache, c.batch, qc, lse, mass, scale=1.0, scores=given)
+    torch.cuda.synchronize()
+    got, want_mass, tol_mass = _f64(lse), np.zeros(mass.shape), np.zeros(mass.shape)
+    largest = 0.0
+    for i, t, h, j, s, w, v, reach, bias in okv8.scored_rows(c.pool, c.table, c.start, c.lens, _f64(q), 1.0, x):
+        largest = max(largest, np.abs(s).max() / cap)
+        e = 13 * u * np.abs(s).max() + of_cap * u * cap
+        ref = s.max() + np.log(np.exp(s - s.max()).sum())
+        assert abs(got[t, h] - ref) <= e + 20 * u + 4 * u * abs(ref), (i, h, got[t, h], ref)
+        times = np.where(j == c.lens[i] - 1, 1, 4)
+        want_mass[i, h // 2, j] += times * w
+        tol_mass[i, h // 2, j] += times * w * (2 * e + 40 * u + 8 * u * (np.abs(s) + abs(ref)) + 40 * u)
+    assert (largest > 0.5) == (of_cap > 0)
+    assert np.all(np.abs(_f64(mass) - want_mass) <= tol_mass)
+
+
+def test_scores_far_beyond_a_cap():
+    """Scores of up to fp32's infinity are the cap, NaN stays NaN, in one step."""
+    _say("scores beyond a cap")
+    c = Case(16, 1, 64, [16, 16], [1, 1], seed=2)
+    c.pool.ks[:] = 2.0 ** 119
+    b = [int(v) for v in c.table[:, 0]]
+    c.pool.k[b[0], 0] = 0
+    c.pool.k[b[0], 0, :, 0] = [0x7E, 0xFE] * 8     # +-448, the largest
+    c.pool.k[b[1], 0] = c.pool.k[b[0], 0]
+    c.pool.k[b[1], 0, 5, 1] = 0x7F                 # a NaN, times zero or not
+    c.pool.ks[b[1]] = 2.0 ** 3
+    c.upload()
+    q = torch.zeros((2, 1, 64), dtype=torch.bfloat16, device="cuda")
+    q[:, 0, 0] = 1e6                               # 448 * 2^119 * 1e6 is infinite
+    out, lse = torch.empty_like(q), torch.empty((2, 1), device="cuda")
+    for cap in (5.0, 1000.0):
+        kv8.attention(c.cache, c.batch, q, out, scale=1.0, scores=kv8.Scores(softcap=cap), lse=lse)
+        torch.cuda.synchronize()
+        assert abs(float(lse[0, 0]) - (cap + np.log(8 + 8 * np.exp(-2 * cap)))) <= 2.0 ** -24 * (8 * cap + 40)
+        want = np.mean([c.pool.values(b[0], p)[1][0] for p in range(0, 16, 2)], axis=0)
+        low = np.mean([np.abs(c.pool.values(b[0], p)[1][0]) for p in range(16)], axis=0)
+        assert np.all(np.abs(_f64(out[0, 0]) - want) <= 2.0 ** -6 * low + 8 * np.exp(-2 * cap) * low)
+        assert torch.isnan(lse[1, 0]) and torch.isnan(out[1, 0]).all()
