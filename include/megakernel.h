@@ -531,8 +531,6 @@ int megakernel_op_kv8_attention(const megakernel_kv8_cache* cache, const megaker
  * softcap is 0 or 2^-30 to 1024; a capped score is off by up to 13 * 2^-24 of itself
  * beyond what q . k is, and by 2 * 2^-24 of the cap besides where another that is
  * computed with it passes half the cap.
- * With slopes scores and log-sum-exps are off by up to 2^-13 of the slope (or, where
- * blocks before a position are missing, 2^-22 of the bias across them).
  * Positions are those of the cache: after
  * megakernel_op_kv8_compact the places that rows were moved to.  The arrays are
  * read when a call runs, and values beyond a sequence's bounds are cut to them. */

@@ -580,11 +580,15 @@ struct Scores {
 // The attention with such scores, or with each row's log-sum-exp: the same
 // kernels, compiled once more.  Scores are formed less the row's reference, so
 // what is not asked for costs a branch a step, a cap seven operations for each
-// score (where some pass half of it six, two of them slow; 1,024 tokens of 16 / 8 heads
-// of 128 at 16,384 positions: causal 167 us, with scores 160, capped 196; four prompts
-// of 2,048 tokens, heads of 64, 66, 73, 100; where most steps pass half the cap 15 %
-// more), the log-sum-exp one.  Steps that a row tile sees none of are
-// not walked: a window of 4,096 at 32,768 positions takes 12.5 us, the whole 18.
+// score (where some pass half of it six, two of them slow), slopes three, the
+// log-sum-exp one.  1,024 tokens of 16 / 8 heads of 128 at 16,384 positions: causal 167
+// us, with scores 160, capped 196, with slopes 176; four prompts of 2,048 tokens, heads
+// of 64, 66, 73, 101 (where most steps pass half the cap 15 % more), 87.  (Of biased
+// scores less the reference from the start near ones were rounded beside far ones'
+// biases, which log-sum-exps showed; 3 to 5 % less time.)  Steps that a row tile sees
+// none of are not walked: a window of 4,096 at 32,768 positions takes 12.5 us, the
+// whole 18.  The 128-row tiles without log-sum-exps leave three registers of head_dim
+// 128 in scratch memory, with few rows beside them two of 64 (12 to 16 bytes a lane).
 struct AttnScored : Attn {
   Scores x;
 };
@@ -1029,12 +1033,16 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
       load_k(t + W, next.k);
     }
     // scores of positions pv + 4i + j of row c
+    // less the row's reference from the start (SCORED), but for biased ones: of far
+    // positions the reference is their bias, and beside it near ones would be rounded
+    float base = below;
+    if constexpr (SCORED) base = p.x.slopes ? 0.f : below;
     if constexpr (SCORED) {
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = sc[i / 4][i % 4];
       const int rel = pv - (s.pos0 + tok);
-      score<16>(p.x, p.scale, slope, below, x, [&](int i) { return rel + i; });
+      score<16>(p.x, p.scale, slope, base, x, [&](int i) { return rel + i; });
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i / 4][i % 4] = x[i];
     }
@@ -1081,21 +1089,24 @@ __device__ __forceinline__ void rows_item(const P& p, int item, void* smem) {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) mt = fmaxf(mt, sc[i][j]);
-    mt = SCORED ? mt - below : mt * p.scale;
-    if (__any(mt > up)) {  // joined over the row's four lanes only here
+    mt = SCORED ? mt - base : mt * p.scale;
+    const bool rise = __any(mt > up);
+    if (rise) {  // joined over the row's four lanes only here
       const float mn = fmaxf(m, max_xor32(max_xor16(mt))), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
-      if constexpr (SCORED) {  // scores are less the reference from the start
-        const float d = (mn == -INFINITY ? 0.f : -mn) - below;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] += d;
-      }
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
       if constexpr (LSE) ex *= al;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= al;
+    }
+    if constexpr (SCORED) {
+      if (rise || p.x.slopes) {
+        const float d = below - base;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] += d;
+      }
     }
     float pr[16];
 #pragma unroll
@@ -1432,6 +1443,8 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
       if (k & 16) tab0 = x;
       else tab1 = x;
     }
+    float base = below;  // as in rows_item()
+    if constexpr (SCORED) base = p.x.slopes ? 0.f : below;
     // score i of half a: position 32a + 16(i/8) + 8h + i%8 of the step
     const auto place = [](int a, int i) { return 32 * a + 16 * (i / 8) + i % 8; };
     if constexpr (SCORED) {
@@ -1441,7 +1454,7 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = sc[a][i];
-        score<16>(p.x, p.scale, slope, below, x, [&](int i) { return rel + place(a, i); });
+        score<16>(p.x, p.scale, slope, base, x, [&](int i) { return rel + place(a, i); });
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[a][i] = x[i];
       }
@@ -1460,17 +1473,11 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[a][i]);
-    mt = SCORED ? mt - below : mt * p.scale;
-    if (__any(mt > up)) {
+    mt = SCORED ? mt - base : mt * p.scale;
+    const bool rise = __any(mt > up);
+    if (rise) {
       const float mn = fmaxf(m, max_xor32(mt)), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
-      if constexpr (SCORED) {  // scores are less the reference from the start
-        const float d = (mn == -INFINITY ? 0.f : -mn) - below;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[a][i] += d;
-      }
       below = mn == -INFINITY ? 0.f : -mn;
       up = mn + RISE;
       sum *= al;
@@ -1479,6 +1486,15 @@ __device__ __forceinline__ void tile_item(const P& p, int item, void* smem) {
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= al;
+    }
+    if constexpr (SCORED) {
+      if (rise || p.x.slopes) {
+        const float d = below - base;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[a][i] += d;
+      }
     }
     if (__builtin_expect((first + TILE > rows.all || (SCORED && first < rows.shut) || gone) && lds.bad[buf] == k + 1, 0)) {
       // the NaN that stage_v() took out, put into the rows that see them

@@ -13,6 +13,14 @@ from tests.test_gpu_kv8 import Case, _f64, _hint, _say
 pytestmark = pytest.mark.gpu
 
 
+def _one_hot(c, n_q, size):
+    """Queries of one dimension each, so that a score is one product, exact in fp32."""
+    q = np.zeros((c.tokens, n_q, c.dim))
+    d = c.rng.integers(0, c.dim, (c.tokens, n_q, 1))
+    np.put_along_axis(q, d, size * c.rng.standard_normal((c.tokens, n_q, 1)), 2)
+    return torch.from_numpy(q).to(torch.bfloat16)
+
+
 # ------------------------------------------------------------------- slopes
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("lens,new,hint", [([100], [40], 64), ([100], [40], 1 << 20), ([100, 33], [1, 2], 64)])
@@ -20,10 +28,9 @@ def test_slopes_as_steep_as_fp32_holds(dim, lens, new, hint):
     """Slopes whose products with distances pass fp32's range: falling ones leave a
     row its own position, rising ones the farthest, position 0: a single weight that
     is not zero, so outputs are that position's values but for the weight's division
-    by itself and the output's rounding.  Log-sum-exps are finite and no more is
-    asked of them: a score is rounded beside the row's reference, which after a first
-    step is -slope times a distance of at least 1, 2^94 and more, half a step of
-    which (2^70) is beyond every score."""
+    by itself and the output's rounding.  Log-sum-exps of falling ones are its score, a
+    sum of D products (with the scale's roundings (D + 3) u of their magnitudes), to
+    base 2 and back (8 u)."""
     _say(f"steep slopes D={dim} {lens} hint {hint}")
     steep = [3.4028234e38, 2.4e38, 2.0 ** 94, 1e20, -3.4028234e38, -2.4e38]
     c = _hint(Case(16, 2, dim, lens, new, seed=dim), hint)
@@ -36,8 +43,32 @@ def test_slopes_as_steep_as_fp32_holds(dim, lens, new, hint):
         for t in range(c.start[i], c.start[i + 1]):
             p = lens[i] - int(c.start[i + 1]) + t
             for h in range(n_q):
-                _, v = c.pool.values(*c.pool.place(c.table[i], p if steep[h] > 0 else 0))
+                k, v = c.pool.values(*c.pool.place(c.table[i], p if steep[h] > 0 else 0))
                 assert np.all(np.abs(_f64(out[t, h]) - v[h // 3]) <= 2.0 ** -7 * np.abs(v[h // 3])), (t, h)
+                s, reach = (f(k[h // 3]) @ f(_f64(q[t, h])) * dim ** -0.5 for f in (np.asarray, np.abs))
+                assert steep[h] < 0 or abs(float(lse[t, h]) - s) <= 2.0 ** -24 * ((dim + 3) * reach + 8 * abs(s)), (t, h)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,new,hint", [([700, 1999], [1, 3], 2000), ([700], [60], 1 << 20), ([1300], [1], 1 << 20)])
+def test_biased_scores_keep_what_near_ones_are(dim, lens, new, hint):
+    """Log-sum-exps of rows whose first steps lie far away.  A raw score is one product
+    (13 u of it as in the test of caps), a bias and its sums 4 u of it, each position's by its weight;
+    of positions with a weight above fp32's smallest, 104 / slope and less, sums (u
+    each) and the logarithm (20 u), and 4 u |lse|."""
+    _say(f"near scores under slopes D={dim} {lens} hint {hint}")
+    slopes = [0.7, 3.0, 20.0, 0.3, 150.0, 1e4]
+    c = _hint(Case(32, 2, dim, lens, new, seed=dim), hint)
+    q, n_q, u = _one_hot(c, 6, 1.0), 6, 2.0 ** -24
+    out, lse = torch.empty((c.tokens, n_q, dim), dtype=torch.bfloat16, device="cuda"), torch.empty((c.tokens, n_q), device="cuda")
+    kv8.attention(c.cache, c.batch, q.cuda(), out, scale=1.0, scores=kv8.Scores(slopes=torch.tensor(slopes, device="cuda")), lse=lse)
+    torch.cuda.synchronize()
+    got = _f64(lse)
+    for i, t, h, j, s, w, v, reach, bias in okv8.scored_rows(c.pool, c.table, c.start, c.lens, _f64(q), 1.0, okv8.Scores(slopes=slopes)):
+        far = slopes[h] * np.abs(j - (int(c.lens[i]) - int(c.start[i + 1]) + t))
+        ref = s.max() + np.log(np.exp(s - s.max()).sum())
+        tol = u * (13 * (w @ np.abs(s + far)) + 4 * (w @ far) + min(len(j), 104 / slopes[h] + 2) + 20 + 4 * abs(ref))
+        assert abs(got[t, h] - ref) <= tol, (i, h, got[t, h], ref, tol)
 
 
 @pytest.mark.parametrize("slope", [2.4e38, 3.4028234e38])
@@ -115,14 +146,6 @@ def test_rows_after_a_compaction_stand_behind_the_kept_ones(dim, block):
 
 
 # --------------------------------------------------------------------- caps
-def _one_hot(c, n_q, size):
-    """Queries of one dimension each, so that a score is one product, exact in fp32."""
-    q = np.zeros((c.tokens, n_q, c.dim))
-    d = c.rng.integers(0, c.dim, (c.tokens, n_q, 1))
-    np.put_along_axis(q, d, size * c.rng.standard_normal((c.tokens, n_q, 1)), 2)
-    return torch.from_numpy(q).to(torch.bfloat16)
-
-
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("cap,size,of_cap", [(50.0, 0.25, 0), (1024.0, 1.0, 0), (1024.0, 0.01, 0), (2.0 ** -30, 2.0 ** -38, 0), (3.0, 3.0, 2), (40.0, 40.0, 2)])
 @pytest.mark.parametrize("hint", [64, 1 << 20])
