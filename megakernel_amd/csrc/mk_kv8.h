@@ -858,7 +858,9 @@ struct Bool {
 // where this takes 13.2; ragged prompts of 33 to 2,048, 71 / 55; 1,024 tokens
 // at the end of 32,768 positions, head_dim 128, 417 / 308 (root mean square
 // error over that of the values, bf16 outputs: 0.0017 / 0.0020, 0.0017 /
-// 0.0019, 0.0017 / 0.0021).
+// 0.0019, 0.0017 / 0.0021).  With scores, too: capped decode of 16 sequences of 512 to
+// 4,096 19.4 / 17.6, 4,096 tokens in documents 40 / 34.5, 1,024 capped ones at 16,384
+// 270 / 213.
 constexpr float RISE = 8.f;
 
 // Codes of the value NaN (0x7f, 0xff) in four bytes: 0x80 in each such byte.

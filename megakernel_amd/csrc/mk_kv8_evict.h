@@ -72,7 +72,7 @@ __device__ __forceinline__ int first_token(const Weigh& p, const Step& x) {
 // 16 at a time, on v_mfma_f32_16x16x32_bf16 (the positions' layout is that of
 // rows_item()); its weights stay in 16 sums a lane until the end.  Bound by K's way
 // here: one token to each of 16 sequences of 512 to 4,096, head_dim 64 (19 MB of K),
-// takes 8.6 us, of which 2.7 are the launch and the rest three loads in a row;
+// takes 9.0 us, of which 2.7 are the launch and the rest three loads in a row;
 // 16 of 4,096, 4 tokens each, 12.4, head_dim 128 22 (67 MB, 3.1 TB/s).
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void weigh_few(Weigh p) {

@@ -99,7 +99,8 @@ __device__ __forceinline__ void put1(void* p, long long e, float x) {
 }
 
 // Any even sizes and any alignment: a pair to a thread, with sines of its own and
-// loads of single elements.
+// loads of single elements (8,192 tokens of 24 heads of 128, half of each turned, rows
+// one element off: 52 us, aligned 21 in rotate()).
 template <bool SRC32, bool DST32>
 __global__ __launch_bounds__(256) void rotate_pairs(Turn p, int interleaved) {
   const unsigned pairs = (unsigned)p.dim / 2, heads = (unsigned)(p.n_q + p.n_kv);
