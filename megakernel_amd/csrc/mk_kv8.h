@@ -679,9 +679,9 @@ __device__ __forceinline__ float slope_of(float s) {
 // tanh(y).  Where the wave's are all at most half the cap, tanh(y) = y (1 + y^2 Q(y^2))
 // with Q interpolated at Chebyshev's nodes to 2^-24: off by 8 * 2^-24 of itself at
 // most.  Else (e^2y - 1) / (e^2y + 1), which e^2y near 1 puts off by 2 * 2^-24 of the
-// cap, beside some score that is not small against it.  (For all scores that form,
-// or 1 - 2 / (e^2y + 1), is as fast, but made log-sum-exps of small scores up to 60
-// times less exact than fp32 has them.)
+// cap, beside some score that is not small against it.  (1 - 2 / (e^2y + 1) for all
+// scores takes 2 to 5 % less, but made log-sum-exps of small ones up to 60 times less
+// exact than fp32 has them.)
 template <int N, class At>
 __device__ __forceinline__ void score(const Scores& x, float scale, float slope, float add, float* s, At at) {
   if (!x.cap) {
